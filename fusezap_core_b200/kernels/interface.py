@@ -453,3 +453,46 @@ class Ops:
         top_p[r] (float32; >= 1: off) then keeps, in falling order of value and rising index among equals, every token
         before which less than top_p[r] of the probability lies."""
         raise NotImplementedError
+
+    # ---- drafted tokens: a step whose portions are trees
+    def tree_attention(self, q: torch.Tensor, cache: Any, meta: Any, out: torch.Tensor, num_heads: int, num_kv_heads: int,
+                       head_dim: int, scale: float, window: int) -> None:
+        """`paged_attention` for rows that are the nodes of a tree (one tree per request, rows meta.seg[s] = (first row, rows, b,
+        state slot), node j in place b + j of the cache): out[n, h] = softmax_j((q[n, h] . K[j]) * scale) V[j] over the places j
+        with max(0, p - window + 1) <= j < b (window 0: 0 <= j < b), p = meta.pos[n] (the row's position, b + its depth), and over
+        the places b + i for the bits i set in meta.ancestors[n] (int32 (N, words), bit i % 32 of word i // 32; a node's own bit
+        among them; bits at and beyond the tree's rows count as unset). A place that a row does not see takes no part whatever
+        it holds. A row that sees no place, and a row of padding, gives zeros. meta.max_context: no b + rows is larger.
+        The places' pages: meta.table(cache.group). float32: a row's sums do not depend on the other requests of the step; a
+        table may cut long contexts of bfloat16 steps by the step's size."""
+        raise NotImplementedError
+
+    def verify_tree(self, logits: torch.Tensor, draft: torch.Tensor | None, temperature: torch.Tensor, uniform: torch.Tensor,
+                    tokens: torch.Tensor, parents: torch.Tensor, seg: torch.Tensor, path: torch.Tensor, count: torch.Tensor,
+                    next_ids: torch.Tensor) -> None:
+        """Which nodes of each request's tree stand against the target, and the token behind them. logits (N, V) float32: the
+        target's at every node; draft (N, V) float32: the drafter's at every node (row n gave n's children), or None: the children
+        were not drawn from probabilities; temperature (S,) float32, of both; uniform (N,) float64 in [0, 1): a child's own
+        number, the root's for the draw at the end; tokens, parents (N,) int32: parent = node within the request's rows, before the
+        child; node 0 is the root, whose token stands; seg (S, 4) int32 = (first row, rows, anything, anything), at most 1,024 rows.
+        From the root on, with p = softmax(logits / T) and q = softmax(draft / T) of the node (draft None: q is all on the child):
+        the node's children x in rising order: x stands if uniform * q(x) < p(x), and the walk goes on from it; else p = max(p - q, 0)
+        over its sum (if that is not 0) and q loses x, scaled to sum 1. No child stands: next_ids[s] is the token at which the
+        running sum of p, in index order, first exceeds uniform[root] * total. T <= 0: the first child that is the argmax
+        (the order of `argmax`) stands, else the argmax is the next token. float64. A row without a distribution (a NaN, +inf, or
+        nothing above -inf): no child stands and the draw gives V - 1.
+        Results, int32: count[s] kept nodes (the root among them; 0 for no rows, next_ids[s] = -1); path[first row + k] = node of the
+        k-th of them, -1 from count[s] to the request's last row; rows of `path` beside the requests' are left."""
+        raise NotImplementedError
+
+    def keep_rows(self, pool: torch.Tensor, table: torch.Tensor, seg: torch.Tensor, path: torch.Tensor, count: torch.Tensor) -> None:
+        """pool: a cache group's (slots, pages, .., page_size, width), any element type of 2 bytes and more; table (S, MB) int32 its
+        block tables. For every request s and k < count[s]: the row at place seg[s, 2] + path[seg[s, 0] + k] goes to place seg[s, 2] +
+        k, in all slots, keys and values, as if all were read before one is written. path (N,), count (S,) int32 as `verify_tree`
+        leaves them: rising nodes; a path that is none (or a place without a page) is an error and leaves the request's rows."""
+        raise NotImplementedError
+
+    def copy_pages(self, pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Page src[i] of a cache group's pool goes to page dst[i], in all slots; src, dst int32 (M,). A page may be a source
+        several times, but a destination only once and not both. A page outside the pool is an error and is left out."""
+        raise NotImplementedError

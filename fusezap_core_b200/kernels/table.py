@@ -116,6 +116,7 @@ class CudaOps(Ops):
             raise KernelError(f"the kernels run on a CUDA device only, not on {self.device}")
         if not torch.cuda.is_available():
             raise KernelError("no CUDA device is available; this engine has no CPU path")
+        self._index = self.device.index if self.device.index is not None else torch.cuda.current_device()
         self.core = load("fzb200_core")
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._err_host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
@@ -127,7 +128,7 @@ class CudaOps(Ops):
         if self.dtype == torch.bfloat16:
             self.tc = load("fzb200_tc")      # tcgen05 / TMA kernels
         self.use_tensor_cores = self.tc is not None
-        self._attn_tc = self._mix = self._mix_tc = self._latent = self._latent_tc = self._seq = self._seq_tc = self._rows = self._ssd = self._ssd_tc = self._gla = self._scan_tc = None   # libraries loaded (and built) when a part first asks for their kernels
+        self._attn_tc = self._mix = self._mix_tc = self._latent = self._latent_tc = self._seq = self._seq_tc = self._rows = self._ssd = self._ssd_tc = self._gla = self._scan_tc = self._drafts = None   # libraries loaded (and built) when a part first asks for their kernels
         self.prefill_tcgen05 = True        # False: long portions on the mma.sync flash-attention kernel
         self.fuse_swiglu = True            # gate/up product and SwiGLU in one kernel where the sizes allow it
         self.fuse_norm = True              # a sublayer's last product, the residual add and the norm behind it in one kernel
@@ -216,6 +217,13 @@ class CudaOps(Ops):
         if self._gla is None:
             self._gla = load("fzb200_gla")
         return self._gla
+
+    @property
+    def drafts(self):
+        """Drafted tokens: attention of a tree over the cache, the verdict on it, cache rows and pages moved."""
+        if self._drafts is None:
+            self._drafts = load("fzb200_drafts")
+        return self._drafts
 
     @property
     def scan_tc(self):
@@ -791,6 +799,116 @@ class CudaOps(Ops):
         weights = self._scratch("sampling weights", r * v, torch.float64)       # exp(x / T - max) of every token
         self._check(self.core.fz_sample_filtered(_p(logits), _p(temperature), _p(top_k), _p(top_p), _p(uniform), _p(weights),
                                                  _p(out), c_int(r), c_int(v), self._stream()), "sample_filtered")
+
+    # ---- drafted tokens
+    def _here(self, t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple) -> None:
+        """A contiguous tensor of exactly this dtype and shape on this table's device."""
+        if t.dtype is dtype and t.shape == shape and t.get_device() == self._index and t.is_contiguous():
+            return
+        if not t.is_cuda or t.get_device() != self._index:
+            raise KernelError(f"{name} is on {t.device}; this kernel table works on {self.device}")
+        if t.dtype != dtype:
+            raise KernelError(f"{name} has dtype {t.dtype}, expected {dtype}")
+        if tuple(t.shape) != tuple(shape):
+            raise KernelError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+        raise KernelError(f"{name} is not contiguous")
+
+    def _launch(self, call, what: str, args: tuple, ideal_bytes: int = 0, kernels: int = 1) -> None:
+        """Runs a C entry on this table's device, whichever is current, and its current stream."""
+        if torch.cuda.current_device() != self._index:
+            with torch.cuda.device(self._index):
+                status = call(*args, self._stream())
+        else:
+            status = call(*args, self._stream())
+        self._check(status, what, ideal_bytes)
+        self.launches += kernels - 1
+
+    def tree_attention(self, q, cache, meta, out, num_heads, num_kv_heads, head_dim, scale, window) -> None:
+        n = q.shape[0]
+        self._here(q, "q", self.dtype, (n, num_heads * head_dim))
+        self._here(out, "attention output", self.dtype, q.shape)
+        k, v, page_stride = self._pool(cache, num_kv_heads, head_dim)
+        if k.get_device() != self._index or v.get_device() != self._index:
+            raise KernelError(f"the cache is on {k.device}; this kernel table works on {self.device}")
+        table, seg, bits = meta.table(cache.group), meta.seg, meta.ancestors
+        segments, pages = table.shape
+        self._here(table, "block tables", torch.int32, (segments, pages))
+        self._here(seg, "segments", torch.int32, (segments, 4))
+        self._here(meta.pos, "positions", torch.int32, (n,))
+        self._here(meta.seq_row, "table rows", torch.int32, (n,))
+        self._here(bits, "ancestors", torch.int32, (n, bits.shape[-1]))
+        if self.drafts.fz_attn_tree_check(num_heads, num_kv_heads, head_dim) != 0:
+            raise KernelError(f"tree_attention: {num_heads} heads, {num_kv_heads} kv heads, head_dim {head_dim} (need heads % kv_heads == 0, "
+                              f"head_dim % 16 == 0 and head_dim <= 512)")
+        if n == 0:
+            return
+        # scratch of the call alone (from the stream's allocator, or the graph's that records it): two calls never share it
+        pieces = self.drafts.fz_attn_tree_pieces(meta.max_context, window)
+        part = torch.empty(n * num_heads * pieces * (head_dim + 2), dtype=torch.float32, device=self.device)
+        self._launch(self.drafts.fz_attn_tree, "tree_attention",
+                     (_p(q), _p(k), _p(v), _p(meta.pos), _p(meta.seq_row), _p(seg), segments, _p(bits), bits.shape[1], _p(table), pages,
+                      c_longlong(page_stride), cache.page_size, _p(out), _CODE[self.dtype], n, num_heads, num_kv_heads, head_dim,
+                      c_float(scale), window, pieces, _p(part), _p(self.err)), kernels=2)
+
+    def verify_tree(self, logits, draft, temperature, uniform, tokens, parents, seg, path, count, next_ids) -> None:
+        if logits.dim() != 2 or seg.dim() != 2:
+            raise KernelError(f"verify_tree: logits {tuple(logits.shape)}, segments {tuple(seg.shape)}")
+        n, vocab = logits.shape
+        segments = seg.shape[0]
+        self._here(logits, "logits", torch.float32, (n, vocab))
+        if draft is not None:
+            self._here(draft, "the drafter's logits", torch.float32, (n, vocab))
+        self._here(temperature, "temperature", torch.float32, (segments,))
+        self._here(uniform, "uniform", torch.float64, (n,))
+        self._here(tokens, "tokens", torch.int32, (n,))
+        self._here(parents, "parents", torch.int32, (n,))
+        self._here(seg, "segments", torch.int32, (segments, 4))
+        self._here(path, "path", torch.int32, (n,))
+        self._here(count, "count", torch.int32, (segments,))
+        self._here(next_ids, "next ids", torch.int32, (segments,))
+        if vocab == 0:
+            raise KernelError("verify_tree: the vocabulary is empty")
+        if segments == 0:
+            return
+        self._launch(self.drafts.fz_verify_tree, "verify_tree",
+                     (_p(logits), _p(draft), _p(temperature), _p(uniform), _p(tokens), _p(parents), _p(seg), segments, n, vocab, _p(path),
+                      _p(count), _p(next_ids), _p(self.err)))
+
+    def _group_pool(self, pool) -> tuple[int, int, int, int, int]:
+        """(slots, pages, parts, page size, bytes of a row) of a cache group's pool (see `KVNeed.pool_shape`, `LatentNeed.pool_shape`)."""
+        if not 4 <= pool.dim() <= 6:
+            raise KernelError(f"a cache pool has 4 to 6 dimensions, not {pool.dim()}")
+        self._here(pool, "cache pool", pool.dtype, pool.shape)
+        shape = pool.shape
+        parts = 1
+        for x in shape[2:-2]:
+            parts *= x
+        return shape[0], shape[1], parts, shape[-2], shape[-1] * pool.element_size()
+
+    def keep_rows(self, pool, table, seg, path, count) -> None:
+        slots, num_pages, parts, page_size, row_bytes = self._group_pool(pool)
+        segments, pages = table.shape
+        n = path.shape[0]
+        self._here(table, "block tables", torch.int32, (segments, pages))
+        self._here(seg, "segments", torch.int32, (segments, 4))
+        self._here(path, "path", torch.int32, (n,))
+        self._here(count, "count", torch.int32, (segments,))
+        if pool.numel() == 0 or segments == 0 or n == 0:
+            return
+        self._launch(self.drafts.fz_keep_rows, "keep_rows",
+                     (_p(pool), slots, num_pages, parts, page_size, row_bytes, _p(table), segments, pages, _p(seg), _p(path), _p(count), n,
+                      _p(self.err)))
+
+    def copy_pages(self, pool, src, dst) -> None:
+        slots, num_pages, parts, page_size, row_bytes = self._group_pool(pool)
+        m = src.shape[0]
+        self._here(src, "source pages", torch.int32, (m,))
+        self._here(dst, "destination pages", torch.int32, (m,))
+        if pool.numel() == 0 or m == 0:
+            return
+        self._launch(self.drafts.fz_copy_pages, "copy_pages",
+                     (_p(pool), slots, num_pages, c_longlong(parts * page_size * row_bytes), _p(src), _p(dst), m, _p(self.err)),
+                     2 * m * slots * parts * page_size * row_bytes)
 
     # ---- the gated parallel block
     def select_tokens(self, tokens, src, prev_ids, out) -> None:

@@ -1,0 +1,562 @@
+"""The kernels for drafted tokens against their definitions in 64 bits (`plain_drafts`), where they can go wrong: trees and chains of
+one node and more, empty contexts, contexts that end inside a page and inside a key tile, windows, rows that see nothing, places
+that hold no numbers, odd groups and head sizes, vocabularies that no vector divides."""
+from types import SimpleNamespace
+
+import numpy as np
+import pytest
+import torch
+
+import plain_drafts as plain
+
+pytestmark = pytest.mark.gpu
+DT = {"float32": torch.float32, "bfloat16": torch.bfloat16}
+NAN = float("nan")
+
+
+def ops_of(dtype):
+    from fusezap_core_b200.kernels import cuda_ops
+    return cuda_ops(dtype)
+
+
+def chain(n):
+    return [i - 1 for i in range(n)]
+
+
+def bushy(n, seed=0):
+    rng = np.random.default_rng(seed)
+    return [-1] + [int(rng.integers(max(0, i - 6), i)) for i in range(1, n)]
+
+
+# ---------------------------------------------------------------------------------------------- attention
+
+def tree_case(dtype, heads, kv, hd, page, requests, window=0, pad=0, seed=0, words=None, spare=3, poison=True):
+    """requests: (places before the tree, parents) each, or (places, None) for one that has no rows in the step. Every place of the
+    pool that belongs to no request's context or tree holds NaN."""
+    gen = torch.Generator().manual_seed(seed)
+    counts = [len(p) if p is not None else 0 for _, p in requests]
+    need = [-(-(b + n) // page) for (b, _), n in zip(requests, counts)]
+    total = sum(need) + spare
+    order = torch.randperm(total, generator=gen).tolist()
+    table = torch.full((len(requests), max(need + [1]) + 1), -1, dtype=torch.int32)
+    pool = torch.full((total, 2, kv, page, hd), NAN if poison else 7.0)
+    seg = torch.zeros(len(requests), 4, dtype=torch.int32)
+    n_rows = sum(counts) + pad
+    words = words or max(1, -(-max(counts) // 32))
+    pos, row, bits = torch.zeros(n_rows, dtype=torch.int32), torch.full((n_rows,), -1, dtype=torch.int32), np.zeros((n_rows, words), np.int32)
+    at = taken = 0
+    for s, ((b, parents), n) in enumerate(zip(requests, counts)):
+        pages = order[taken:taken + need[s]]
+        taken += need[s]
+        table[s, :need[s]] = torch.tensor(pages, dtype=torch.int32)
+        for place in range(b + n):
+            pool[pages[place // page], :, :, place % page] = torch.randn(2, kv, hd, generator=gen)
+        if parents is None:
+            continue
+        seg[s] = torch.tensor([at, n, b, -1])
+        pos[at:at + n] = torch.tensor([b + d for d in plain.depths_of(parents)])
+        row[at:at + n] = s
+        bits[at:at + n] = plain.ancestors_of(parents, words)
+        if window:      # pages that lie wholly before every row's window are given back
+            for pi in range(max(0, b - window + 1) // page):
+                table[s, pi] = -1
+        at += n
+    q = torch.randn(n_rows, heads * hd, generator=gen) * 2
+    meta = SimpleNamespace(pos=pos, seq_row=row, seg=seg, ancestors=torch.from_numpy(bits), tables=table,
+                           max_context=max([b + n for (b, _), n in zip(requests, counts)]))
+    return SimpleNamespace(q=q.to(DT[dtype]), pool=pool.to(DT[dtype]), meta=meta, heads=heads, kv=kv, hd=hd, page=page, window=window,
+                           scale=hd ** -0.5, dtype=dtype)
+
+
+def on_gpu(c):
+    m = c.meta
+    meta = SimpleNamespace(pos=m.pos.cuda(), seq_row=m.seq_row.cuda(), seg=m.seg.cuda(), ancestors=m.ancestors.cuda(), max_context=m.max_context)
+    tables = m.tables.cuda()
+    meta.table = lambda group: tables
+    pool = c.pool.cuda()
+    cache = SimpleNamespace(keys=pool[:, 0], values=pool[:, 1], page_size=c.page, group=0, write=True)
+    return c.q.cuda(), cache, meta
+
+
+def run_tree(c, ops=None):
+    q, cache, meta = on_gpu(c)
+    out = torch.full_like(q, NAN)
+    ops = ops or ops_of(c.dtype)
+    ops.tree_attention(q, cache, meta, out, c.heads, c.kv, c.hd, c.scale, c.window)
+    ops.check_errors()
+    return out
+
+
+def reference(c):
+    m = c.meta
+    return plain.attend(c.q, c.pool[:, 0], c.pool[:, 1], m.tables, m.seg, m.pos, m.seq_row, m.ancestors, c.heads, c.kv, c.hd, c.scale, c.window)
+
+
+def tree_tolerance(c, ref, size):
+    """Per value. A score is off by at most ds = (hd + 4) half steps of float32 times |q| |k| scale (and the exponent's own rounding),
+    which makes weights relatively 2 ds wrong together with their sum; the sums over L places are off by (L + 64) half steps relative to
+    sum w |v| (64: pieces, the division). bfloat16: the output's one rounding, and the weights' rounding to bfloat16 in the tensor-core
+    kernel, each half a step of 2^-8."""
+    unit = 2.0 ** -24
+    q = c.q.float().view(-1, c.hd).norm(dim=1).max()
+    finite = torch.nan_to_num(c.pool[:, 0].float(), nan=0.0, posinf=0.0, neginf=0.0)
+    k = finite.reshape(-1, c.hd).norm(dim=1).max()
+    ds = (c.hd + 4) * unit * float(q * k) * c.scale
+    tol = (2 * ds + (c.meta.max_context + 64) * unit) * size + 1e-30
+    return tol + (2.0 ** -8 * (ref.abs() + size) if c.dtype == "bfloat16" else unit * ref.abs())
+
+
+def assert_tree(c, out, rows=slice(None)):
+    ref, size = reference(c)
+    got, ref, size = out.double().cpu()[rows], ref[rows], size[rows]
+    assert torch.isfinite(got).all(), "not finite"
+    over = (got - ref).abs() - tree_tolerance(c, ref, size)
+    assert over.max() <= 0, f"off by {float((got - ref).abs().max()):.3e}, {float(over.max()):.3e} more than allowed, at {int(over.argmax())}"
+
+
+SIZES = [(4, 4, 64), (14, 2, 64), (32, 8, 128), (10, 2, 128), (3, 1, 32), (6, 2, 48), (40, 1, 128), (8, 2, 256), (2, 1, 512), (4, 2, 16)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("heads,kv,hd", SIZES)
+def test_tree_attention_sizes(dtype, heads, kv, hd):
+    c = tree_case(dtype, heads, kv, hd, 16, [(37, bushy(9)), (0, bushy(5, 1)), (130, chain(3)), (300, [-1])], pad=3)
+    assert_tree(c, run_tree(c))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("page", [1, 3, 4, 8, 16, 24, 48, 64])
+def test_tree_attention_pages(dtype, page):
+    c = tree_case(dtype, 8, 2, 64, page, [(127, bushy(6)), (128, bushy(7, 1)), (129, bushy(8, 2)), (16, bushy(17, 3)), (257, chain(4))])
+    assert_tree(c, run_tree(c))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("start", [0, 1, 15, 16, 17, 63, 64, 100, 127, 128, 256, 383, 1000])
+def test_tree_attention_context_lengths(dtype, start):
+    c = tree_case(dtype, 8, 2, 128, 16, [(start, bushy(11)), (start + 5, [-1])])
+    assert_tree(c, run_tree(c))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("nodes", [1, 2, 31, 32, 33, 64, 100, 257])
+@pytest.mark.parametrize("shape", [chain, bushy])
+def test_tree_attention_nodes(dtype, nodes, shape):
+    c = tree_case(dtype, 6, 2, 64, 16, [(90, shape(nodes)), (200, shape(max(1, nodes // 3)))], pad=2)
+    assert_tree(c, run_tree(c))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("window", [1, 2, 17, 64, 100, 129, 500])
+def test_tree_attention_windows(dtype, window):
+    c = tree_case(dtype, 8, 2, 64, 16, [(333, bushy(9)), (40, chain(12)), (64, bushy(5)), (0, chain(3)), (1000, chain(7))], window=window)
+    assert_tree(c, run_tree(c))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_tree_attention_long_contexts(dtype):
+    c = tree_case(dtype, 8, 2, 128, 16, [(5000, bushy(20)), (3001, bushy(33)), (20, chain(2))])
+    assert_tree(c, run_tree(c))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_tree_attention_many_requests_and_empty_ones(dtype):
+    rng = np.random.default_rng(5)
+    reqs = [(int(rng.integers(0, 200)), None if i % 7 == 3 else bushy(int(rng.integers(1, 8)), i)) for i in range(70)]
+    c = tree_case(dtype, 4, 2, 64, 16, reqs, pad=5)
+    out = run_tree(c)
+    assert_tree(c, out)
+    assert (out[-5:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_tree_attention_rows_that_see_nothing(dtype):
+    c = tree_case(dtype, 8, 2, 64, 16, [(0, bushy(6)), (50, bushy(6))])
+    c.meta.ancestors[2] = 0
+    c.meta.ancestors[8] = 0           # still sees its context
+    c.meta.ancestors[9] = -1          # bits beyond the tree's rows count as unset
+    out = run_tree(c)
+    assert (out[2] == 0).all()
+    assert_tree(c, out)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("bad", [NAN, float("inf")])
+def test_tree_attention_unseen_places_take_no_part(dtype, bad):
+    parents = [-1, 0, 0, 1, 2]
+    c = tree_case(dtype, 8, 2, 64, 16, [(45, parents), (20, parents)])
+    place = 45 + 2
+    c.pool[c.meta.tables[0, place // 16].long(), :, :, place % 16] = bad
+    sees = [2, 4]
+    out = run_tree(c)
+    assert not torch.isfinite(out[sees].float()).any()
+    c.pool[c.meta.tables[0, place // 16].long(), :, :, place % 16] = 1.0
+    assert_tree(c, out, [i for i in range(10) if i not in sees])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_tree_attention_places_before_the_window_take_no_part(dtype):
+    c = tree_case(dtype, 8, 2, 64, 16, [(333, chain(9))], window=70)
+    # place 264 is seen by the first two rows (positions 333 and ..: 333 - 70 + 1 = 264), 263 by none
+    for place in (263, 256):
+        c.pool[c.meta.tables[0, place // 16].long(), :, :, place % 16] = NAN
+    out = run_tree(c)
+    assert_tree(c, out)
+    place = 264
+    c.pool[c.meta.tables[0, place // 16].long(), :, :, place % 16] = NAN
+    out = run_tree(c)
+    assert not torch.isfinite(out[0].float()).any()
+    c.pool[c.meta.tables[0, place // 16].long(), :, :, place % 16] = 1.0
+    assert_tree(c, out, list(range(1, 9)))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_tree_attention_large_scores(dtype):
+    c = tree_case(dtype, 8, 2, 64, 16, [(150, bushy(9)), (700, chain(3))], poison=False)
+    c.q *= 16
+    c.pool[:, 0] *= 4
+    assert_tree(c, run_tree(c))
+
+
+def test_tree_attention_float32_rows_do_not_depend_on_the_step():
+    reqs = [(300, bushy(9)), (2000, chain(4)), (77, bushy(30, 2)), (0, [-1])]
+    c = tree_case("float32", 14, 2, 64, 16, reqs, seed=3)
+    whole = run_tree(c)
+    at = 0
+    for s, (b, parents) in enumerate(reqs):
+        n = len(parents)
+        m = c.meta
+        seg = m.seg[s:s + 1].clone()
+        seg[0, 0] = 0
+        alone = SimpleNamespace(**{**vars(c), "q": c.q[at:at + n], "meta": SimpleNamespace(
+            pos=m.pos[at:at + n], seq_row=torch.zeros(n, dtype=torch.int32), seg=seg, ancestors=m.ancestors[at:at + n], tables=m.tables[s:s + 1],
+            max_context=m.max_context)})
+        assert torch.equal(run_tree(alone), whole[at:at + n])
+        at += n
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_tree_attention_replayed_with_other_lengths(dtype):
+    """One recorded call, replayed after the metadata, the queries and the cache have changed under it."""
+    a = tree_case(dtype, 8, 2, 128, 16, [(900, bushy(9)), (40, chain(7))], seed=1)
+    b = tree_case(dtype, 8, 2, 128, 16, [(33, bushy(9, 4)), (880, chain(7))], seed=2, spare=3 + 0)
+    pages = max(a.pool.shape[0], b.pool.shape[0])
+    grow = lambda p: torch.cat([p, torch.full((pages - p.shape[0], *p.shape[1:]), NAN, dtype=p.dtype)])
+    a.pool, b.pool = grow(a.pool), grow(b.pool)
+    width = max(a.meta.tables.shape[1], b.meta.tables.shape[1])
+    for c in (a, b):
+        c.meta.tables = torch.cat([c.meta.tables, torch.full((2, width - c.meta.tables.shape[1]), -1, dtype=torch.int32)], 1)
+        c.meta.max_context = 1000
+    ops = ops_of(dtype)
+    q, cache, meta = on_gpu(a)
+    out = torch.empty_like(q)
+    ops.tree_attention(q, cache, meta, out, 8, 2, 128, a.scale, 0)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.tree_attention(q, cache, meta, out, 8, 2, 128, a.scale, 0)
+    q2, cache2, meta2 = on_gpu(b)
+    q.copy_(q2)
+    cache.keys.copy_(cache2.keys)
+    cache.values.copy_(cache2.values)
+    for name in ("pos", "seq_row", "seg", "ancestors"):
+        getattr(meta, name).copy_(getattr(meta2, name))
+    meta.table(0).copy_(meta2.table(0))
+    out.fill_(NAN)
+    g.replay()
+    ops.check_errors()
+    assert_tree(b, out)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_tree_attention_on_two_streams_at_once(dtype):
+    cases = [tree_case(dtype, 8, 2, 128, 16, [(900 + 50 * i, bushy(9, i)), (40, chain(7))], seed=i) for i in range(2)]
+    ops, streams, outs, keep = ops_of(dtype), [torch.cuda.Stream() for _ in cases], [], []
+    for c, s in zip(cases, streams):
+        keep.append(on_gpu(c))
+        outs.append(torch.empty_like(keep[-1][0]))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, s, (q, cache, meta), out in zip(cases, streams, keep, outs):
+            with torch.cuda.stream(s):
+                ops.tree_attention(q, cache, meta, out, 8, 2, 128, c.scale, 0)
+    torch.cuda.synchronize()
+    ops.check_errors()
+    for c, out in zip(cases, outs):
+        assert_tree(c, out)
+
+
+# ---------------------------------------------------------------------------------------------- verdict
+
+def verify_case(vocab, trees, drafter, seed=0, spread=2.0, error=0.5, greedy=lambda s: s % 4 == 3, pad=0):
+    """trees: parents of each request (an empty list: no rows). Children are drawn from the drafter without replacement, as far as the
+    vocabulary goes."""
+    rng = np.random.default_rng(seed)
+    n = sum(len(t) for t in trees) + pad
+    logits = (rng.standard_normal((n, vocab)) * spread).astype(np.float32)
+    draft = (logits + rng.standard_normal((n, vocab)) * error).astype(np.float32)
+    seg, parents, tokens, temperature = np.zeros((len(trees), 4), np.int32), np.full(n, -1, np.int32), np.zeros(n, np.int32), np.zeros(len(trees), np.float32)
+    at = 0
+    for s, t in enumerate(trees):
+        seg[s] = (at, len(t), 1000 * s, -1)
+        temperature[s] = 0.0 if greedy(s) else 0.5 + 0.25 * (s % 3)
+        drawn = {}
+        for j, p in enumerate(t):
+            parents[at + j] = p
+            if p < 0:
+                tokens[at + j] = rng.integers(vocab)
+                continue
+            z = draft[at + p] / (temperature[s] or 0.3) + rng.gumbel(size=vocab)
+            z[drawn.setdefault(p, [])] = -np.inf
+            tokens[at + j] = int(z.argmax())
+            if len(drawn[p]) + 1 < vocab:
+                drawn[p].append(tokens[at + j])
+        at += len(t)
+    return dict(logits=logits, draft=draft if drafter else None, temperature=temperature, uniform=rng.random(n), tokens=tokens, parents=parents, seg=seg)
+
+
+def run_verify(c):
+    n, S = len(c["tokens"]), len(c["seg"])
+    dev = {k: None if v is None else torch.from_numpy(v).cuda() for k, v in c.items()}
+    out = [torch.full((k,), -7, dtype=torch.int32, device="cuda") for k in (n, S, S)]
+    ops = ops_of("float32")
+    ops.verify_tree(dev["logits"], dev["draft"], dev["temperature"], dev["uniform"], dev["tokens"], dev["parents"], dev["seg"], *out)
+    ops.check_errors()
+    return [t.cpu().numpy() for t in out]
+
+
+def assert_verify(c):
+    path, count, ids = run_verify(c)
+    rpath, rcount, rids = plain.verify(c["logits"], c["draft"], c["temperature"], c["uniform"], c["tokens"], c["parents"], c["seg"])
+    rows = np.zeros(len(path), bool)
+    for row0, n, *_ in c["seg"]:
+        rows[row0:row0 + n] = True
+    np.testing.assert_array_equal(count, rcount)
+    np.testing.assert_array_equal(ids, rids)
+    np.testing.assert_array_equal(path[rows], rpath[rows])
+    assert (path[~rows] == -7).all(), "a row beside the requests' was written"
+    return count
+
+
+@pytest.mark.parametrize("drafter", [True, False])
+@pytest.mark.parametrize("vocab", [1, 2, 5, 63, 257, 1024, 4099, 32000, 50021, 128256])
+def test_verify_vocabularies(vocab, drafter):
+    assert_verify(verify_case(vocab, [bushy(9), chain(5), [-1], bushy(14, 3), chain(4), [-1, 0, 0, 0, 0]], drafter, seed=vocab, pad=2))
+
+
+@pytest.mark.parametrize("drafter", [True, False])
+@pytest.mark.parametrize("requests", [1, 14, 15, 33, 75, 300])
+def test_verify_requests(requests, drafter):
+    c = verify_case(4500 * 8 if requests < 40 else 8200, [[] if s % 9 == 5 else bushy(1 + s % 7, s) for s in range(requests)], drafter, seed=requests)
+    count = assert_verify(c)
+    assert not drafter or requests < 14 or count.max() > 2      # (the walk went somewhere)
+
+
+@pytest.mark.parametrize("drafter", [True, False])
+def test_verify_many_siblings(drafter):
+    """A drafter that is far off: most children fall, and p and q shrink child by child."""
+    trees = [[-1] + [0] * 12 + [1, 1, 5, 5, 12, 12, 13, 15]] * 6
+    assert_verify(verify_case(600, trees, drafter, seed=3, spread=1.0, error=2.5, greedy=lambda s: False))
+    assert_verify(verify_case(7, [[-1] + [0] * 9] * 40, drafter, seed=4, spread=1.0, error=2.0, greedy=lambda s: False))
+
+
+def test_verify_drafter_equal_to_the_target_keeps_its_first_children():
+    c = verify_case(3000, [chain(8), bushy(20)] * 3, True, error=0.0, greedy=lambda s: False)
+    c["draft"] = c["logits"].copy()
+    assert (assert_verify(c)[::2] == 8).all()
+
+
+def test_verify_tokens_left_out():
+    """Logits of -inf (tokens filtered away) at the start of every lane's run, the rows' ends, and all but one."""
+    c = verify_case(5000, [bushy(9), chain(5), bushy(7, 2)], True, seed=9, greedy=lambda s: s == 1)
+    c["logits"][:, :3000] = -np.inf
+    c["draft"][:, 4000:] = -np.inf
+    c["logits"][3, :] = -np.inf
+    c["logits"][3, 17] = 0.5
+    c["draft"][5, :] = -np.inf
+    c["draft"][5, 4999] = -3.0
+    assert_verify(c)
+
+
+def test_verify_rows_without_a_distribution():
+    for bad in (NAN, np.inf, None):
+        c = verify_case(5000, [chain(3), bushy(5)], False, seed=10, greedy=lambda s: False)
+        for row in (0, 3):
+            if bad is None:
+                c["logits"][row] = -np.inf
+            else:
+                c["logits"][row, 4321] = bad
+        count = assert_verify(c)
+        assert (count == 1).all()
+    c = verify_case(5000, [chain(3)], False, seed=11, greedy=lambda s: True)      # greedy: a NaN is the maximum, as in argmax
+    c["logits"][0, 77] = NAN
+    c["tokens"][1] = 77
+    assert assert_verify(c)[0] >= 2
+
+
+def test_verify_numbers_at_their_ends():
+    c = verify_case(4096 * 9, [chain(4)] * 20, True, seed=12, greedy=lambda s: False)
+    c["uniform"][:40] = 0.0
+    c["uniform"][40:] = 1.0 - 2.0 ** -53
+    assert_verify(c)
+
+
+def test_verify_small_and_large_temperatures():
+    c = verify_case(20000, [bushy(6, s) for s in range(8)], True, seed=13, greedy=lambda s: False)
+    c["temperature"][:] = [1e-3, 0.01, 0.1, 1.0, 3.0, 30.0, 1e3, 1e-2]
+    assert_verify(c)
+
+
+@pytest.mark.parametrize("drafter", [True, False])
+def test_verify_keeps_the_targets_distribution(drafter):
+    """Over many requests the first token behind the root (a child that stands, or the draw) is distributed as softmax(logits / T):
+    each token's share within five standard deviations."""
+    vocab, requests, t = 6, 20000, 0.7
+    rng = np.random.default_rng(14)
+    logits, draft = rng.standard_normal(vocab).astype(np.float32), rng.standard_normal(vocab).astype(np.float32)
+    q = plain.softmax64(draft, t)
+    first = rng.choice(vocab, requests, p=q)
+    left = np.where(np.arange(vocab) == first[:, None], 0.0, q)
+    second = (rng.random((requests, 1)) > np.cumsum(left / left.sum(1, keepdims=True), 1)).sum(1)
+    n = 3 * requests
+    tokens = np.stack([np.zeros(requests), first, second], 1).astype(np.int32).reshape(-1)
+    c = dict(logits=np.tile(logits, (n, 1)), draft=np.tile(draft, (n, 1)) if drafter else None, temperature=np.full(requests, t, np.float32),
+             uniform=rng.random(n), tokens=tokens, parents=np.tile(np.array([-1, 0, 0], np.int32), requests),
+             seg=np.stack([3 * np.arange(requests), np.full(requests, 3), np.zeros(requests), np.zeros(requests)], 1).astype(np.int32))
+    path, count, ids = run_verify(c)
+    got = np.where(count > 1, tokens[3 * np.arange(requests) + np.maximum(path[1::3], 0)], ids)
+    p = plain.softmax64(logits, t)
+    share = np.bincount(got, minlength=vocab) / requests
+    assert (np.abs(share - p) <= 5 * np.sqrt(p * (1 - p) / requests)).all(), (share, p)
+
+
+def test_verify_reports_bad_trees():
+    from fusezap_core_b200.kernels.table import KernelError
+    c = verify_case(100, [chain(3), chain(3)], False, greedy=lambda s: False)
+    c["tokens"][1] = 100
+    with pytest.raises(KernelError, match="embedding table"):
+        run_verify(c)
+    c = verify_case(100, [chain(1025), chain(2)], False, greedy=lambda s: True)
+    with pytest.raises(KernelError, match="outside the step"):
+        run_verify(c)
+    c = verify_case(100, [chain(3)], False)
+    c["seg"][0, 1] = 4
+    with pytest.raises(KernelError, match="outside the step"):
+        run_verify(c)
+
+
+# ---------------------------------------------------------------------------------------------- rows and pages moved
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(3, 2, 4, 16, 64), (2, 2, 1, 4, 5), (5, 3, 16, 24), (1, 16, 96), (2, 2, 2, 1, 8), (1, 2, 8, 8, 128), (1, 7, 3)])
+def test_keep_rows(dtype, shape):
+    slots, page = shape[0], shape[-2]
+    rng = np.random.default_rng(sum(shape))
+    spec = [(0, 9, [0, 2, 3, 8]), (5, 1, [0]), (16, 20, list(range(1, 20, 2))), (31, 6, [0, 1, 2]), (2, 0, []), (47, 40, sorted(rng.permutation(40)[:25].tolist())),
+            (11, 5, []), (9, 12, [11])]
+    need = [-(-(b + n) // page) for b, n, _ in spec]
+    order = rng.permutation(sum(need) + 2).tolist()
+    table = torch.full((len(spec), max(need)), -1, dtype=torch.int32)
+    seg, path, count, at, taken = torch.zeros(len(spec), 4, dtype=torch.int32), [], [], 0, 0
+    for s, (b, n, kept) in enumerate(spec):
+        table[s, :need[s]] = torch.tensor(order[taken:taken + need[s]], dtype=torch.int32)
+        seg[s] = torch.tensor([at, n, b, -1])
+        path += kept + [-1] * (n - len(kept))
+        count.append(len(kept))
+        at += n
+        taken += need[s]
+    path, count = torch.tensor(path + [-1], dtype=torch.int32), torch.tensor(count, dtype=torch.int32)
+    pool = torch.randn(slots, len(order), *shape[1:]).to(dtype)
+    want, got = pool.clone(), pool.cuda()
+    plain.keep(want, table, seg, path, count)
+    ops = ops_of("float32")
+    ops.keep_rows(got, table.cuda(), seg.cuda(), path.cuda(), count.cuda())
+    ops.check_errors()
+    assert torch.equal(got.cpu(), want)
+
+
+def test_keep_rows_leaves_a_request_whose_path_is_none():
+    from fusezap_core_b200.kernels.table import KernelError
+    ops = ops_of("float32")
+    table = torch.tensor([[0, 1], [2, -1]], dtype=torch.int32, device="cuda")
+    seg = torch.tensor([[0, 6, 1, -1], [6, 5, 3, -1]], dtype=torch.int32, device="cuda")
+    pool = torch.randn(2, 4, 2, 3, 4, 8, device="cuda")
+    good = [0, 2, 4, -1, -1, -1]
+    for path, count, why in (([0, 3, 2, -1, -1, -1], 3, "outside the step"), ([0, 2, 2, -1, -1, -1], 3, "outside the step"), ([0, 6, -1, -1, -1, -1], 2, "outside the step"),
+                             ([-1] * 6, 1, "outside the step"), (good, 7, "outside the step"), (good, 3, "no page")):
+        other = [0, 4, -1, -1, -1] if why == "no page" else [0, -1, -1, -1, -1]      # (its place 3 + 4 has no page)
+        was, now = pool.clone(), pool.clone()
+        ops.keep_rows(now, table, seg, torch.tensor(path + other, dtype=torch.int32, device="cuda"),
+                      torch.tensor([count, 2 if why == "no page" else 1], dtype=torch.int32, device="cuda"))
+        with pytest.raises(KernelError, match=why):
+            ops.check_errors()
+        bad = [0, 1] if why != "no page" else [2]
+        assert torch.equal(now[:, bad], was[:, bad])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(3, 2, 4, 16, 64), (2, 2, 1, 4, 5), (1, 1, 3), (2, 16, 24), (32, 2, 8, 16, 128), (1, 2, 8, 64, 128)])
+def test_copy_pages(dtype, shape):
+    gen = torch.Generator().manual_seed(1)
+    order = torch.randperm(23, generator=gen)
+    src, dst = order[:5][torch.randint(0, 5, (11,), generator=gen)].int(), order[5:16].int()
+    pool = torch.randn(shape[0], 23, *shape[1:], generator=gen).to(dtype)
+    want, got = pool.clone(), pool.cuda()
+    plain.copy(want, src, dst)
+    ops = ops_of("float32")
+    ops.copy_pages(got, src.cuda(), dst.cuda())
+    ops.check_errors()
+    assert torch.equal(got.cpu(), want)
+
+
+def test_copy_pages_leaves_out_pages_outside_the_pool():
+    from fusezap_core_b200.kernels.table import KernelError
+    ops = ops_of("float32")
+    pool = torch.randn(2, 5, 2, 3, 4, 8, device="cuda")
+    want = pool.clone()
+    want[:, 3] = want[:, 1]
+    ops.copy_pages(pool, torch.tensor([1, 5, 0, -1], dtype=torch.int32, device="cuda"), torch.tensor([3, 2, 5, 4], dtype=torch.int32, device="cuda"))
+    with pytest.raises(KernelError, match="no page"):
+        ops.check_errors()
+    assert torch.equal(pool, want)
+
+
+# ---------------------------------------------------------------------------------------------- refusals
+
+def test_refusals():
+    from fusezap_core_b200.kernels.table import KernelError
+    ops = ops_of("bfloat16")
+    c = tree_case("bfloat16", 8, 2, 64, 16, [(20, bushy(5))])
+    q, cache, meta = on_gpu(c)
+    out = torch.empty_like(q)
+
+    def refused(match, q=q, cache=cache, out=out, heads=8, kv=2, hd=64, **other):
+        m = SimpleNamespace(**{**vars(meta), **other})
+        with pytest.raises(KernelError, match=match):
+            ops.tree_attention(q, cache, m, out, heads, kv, hd, 0.1, 0)
+
+    refused("dtype", q=q.float())
+    refused("is on cpu", q=q.cpu())
+    refused("shape", out=out[:-1])
+    refused("shape", pos=meta.pos[:-1])
+    refused("dtype", ancestors=meta.ancestors.long())
+    refused("shape", seg=meta.seg[:, :3].contiguous())
+    refused("contiguous", q=torch.empty_like(q).t().contiguous().t())
+    refused("key pool", cache=SimpleNamespace(**{**vars(cache), "page_size": 8}))
+    refused("head_dim", q=torch.empty(5, 8 * 24, dtype=torch.bfloat16, device="cuda"), out=torch.empty(5, 8 * 24, dtype=torch.bfloat16, device="cuda"), hd=24,
+            cache=SimpleNamespace(**{**vars(cache), "keys": torch.empty(4, 2, 2, 16, 24, dtype=torch.bfloat16, device="cuda")[:, 0],
+                                     "values": torch.empty(4, 2, 2, 16, 24, dtype=torch.bfloat16, device="cuda")[:, 1]}))
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")
+    f = lambda *s: torch.zeros(s, device="cuda")
+    good = dict(logits=f(3, 10), draft=f(3, 10), temperature=f(1), uniform=f(3).double(), tokens=i32(3), parents=i32(3), seg=i32(1, 4), path=i32(3), count=i32(1), next_ids=i32(1))
+    for name, bad in (("logits", f(3, 10).bfloat16()), ("draft", f(3, 9)), ("temperature", f(2)), ("uniform", f(3)), ("tokens", i32(4)), ("parents", i32(3).long()),
+                      ("seg", i32(1, 3)), ("path", i32(2)), ("count", i32(2)), ("next_ids", i32(1).cpu())):
+        with pytest.raises(KernelError):
+            ops.verify_tree(**{**good, name: bad})
+    pool = torch.zeros(2, 4, 2, 1, 4, 8, device="cuda")
+    for bad in (dict(pool=pool.transpose(0, 1)), dict(pool=pool.cpu()), dict(table=i32(2, 2)), dict(path=i32(3).long()), dict(count=i32(2))):
+        with pytest.raises(KernelError):
+            ops.keep_rows(**{**dict(pool=pool, table=i32(1, 2), seg=i32(1, 4), path=i32(3), count=i32(1)), **bad})
+    for bad in (dict(src=i32(2)), dict(dst=i32(3).float()), dict(pool=pool[:, ::2])):
+        with pytest.raises(KernelError):
+            ops.copy_pages(**{**dict(pool=pool, src=i32(3), dst=i32(3)), **bad})
+    ops.check_errors()

@@ -31,7 +31,7 @@ struct Args {
   const int *pos, *seg, *table;
   int S, mb;
   long long page_stride;
-  int page_size, N, Hq, Hkv, hd, window, pieces;
+  int page_size, num_pages, N, Hq, Hkv, hd, window, pieces;
   float scale_log2;
   float *part_o, *part_ml;
   int* err;
@@ -90,7 +90,7 @@ attn_tree_context_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, 
       if (key >= seen_from && key < end && d < A.hd) {
         const int pi = key / A.page_size;
         const int page = pi < A.mb ? trow[pi] : -1;
-        if (page >= 0) src = (which ? v_pool : k_pool) + (long long)page * A.page_stride + head_off + (long long)(key - pi * A.page_size) * A.hd + d;
+        if (page >= 0 && page < A.num_pages) src = (which ? v_pool : k_pool) + (long long)page * A.page_stride + head_off + (long long)(key - pi * A.page_size) * A.hd + d;
         else atomicOr(A.err, FZ_ERR_NO_PAGE);
       }
       T* dst = which ? V + j * HD + d : K + j * KS + d;
@@ -225,13 +225,11 @@ attn_tree_context_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, 
 // Where a row's pieces lie in the general kernel's scratch.
 struct Pieces {
   const float *part_o, *part_ml;
-  int pieces, Hq, hd, window;
-  __device__ __forceinline__ int count(int s, int start, int, int, int) const {
-    const int places = start - context_first(start, window);
-    const int piece = piece_length(places);
-    return min(pieces, (places + piece - 1) / piece);
+  int pieces, Hq, window;
+  __device__ __forceinline__ Range range(int n, int h, int, int, int, int, int, int start, int) const {
+    const int places = start - context_first(start, window), piece = piece_length(places);
+    return {min(pieces, (places + piece - 1) / piece), ((size_t)n * Hq + h) * pieces, 1, 0, 0};
   }
-  __device__ __forceinline__ size_t slot(int n, int h, int, int, int i) const { return ((size_t)n * Hq + h) * pieces + i; }
 };
 
 template <typename T, int DPT, int RM, int KT>
@@ -281,20 +279,20 @@ FZ_API int fz_attn_tree_pieces(int max_context, int window) {
 // q, out: (N, Hq hd); seg (S, 4) = (first row, rows, first place of the tree, anything); ancestors (N, words): bit j of a row's
 // words: place `first place + j` is seen. part: N * Hq * pieces * (hd + 2) floats, 16-byte aligned.
 FZ_API int fz_attn_tree(const void* q, const void* k_pool, const void* v_pool, const int* pos, const int* seq_row, const int* seg, int S,
-                        const int* ancestors, int words, const int* table, int mb, long long page_stride, int page_size, void* out,
-                        int dtype, int N, int Hq, int Hkv, int hd, float scale, int window, int pieces, float* part, int* err,
+                        const int* ancestors, int words, const int* table, int mb, long long page_stride, int page_size, int num_pages,
+                        void* out, int dtype, int N, int Hq, int Hkv, int hd, float scale, int window, int pieces, float* part, int* err,
                         cudaStream_t stream) {
   if (N <= 0) return FZ_OK;
-  if (fz_attn_tree_check(Hq, Hkv, hd) != FZ_OK || S <= 0 || words <= 0 || mb <= 0 || page_size <= 0 || pieces <= 0 || pieces > 32) return FZ_BAD_SHAPE;
+  if (fz_attn_tree_check(Hq, Hkv, hd) != FZ_OK || S <= 0 || words <= 0 || mb <= 0 || page_size <= 0 || num_pages <= 0 || pieces <= 0 || pieces > 32) return FZ_BAD_SHAPE;
   if (Hq > 65535) return FZ_TOO_LARGE;
   if (dtype != FZ_F32 && dtype != FZ_BF16) return FZ_BAD_DTYPE;
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)part) & 15 || page_stride % (dtype == FZ_F32 ? 4 : 8)) return FZ_BAD_ALIGNMENT;
-  const Args A = {pos, seg, table, S, mb, page_stride, page_size, N, Hq, Hkv, hd, window, pieces, scale * 1.4426950408889634f,
+  const Args A = {pos, seg, table, S, mb, page_stride, page_size, num_pages, N, Hq, Hkv, hd, window, pieces, scale * 1.4426950408889634f,
             part, part + (size_t)N * Hq * pieces * hd, err};
   const int st = dtype == FZ_F32 ? context<float>(q, k_pool, v_pool, A, stream) : context<__nv_bfloat16>(q, k_pool, v_pool, A, stream);
   if (st != FZ_OK) return st;
-  const Pieces P = {A.part_o, A.part_ml, pieces, Hq, hd, window};
-  const TreeArgs R = {pos, seq_row, seg, ancestors, table, S, words, mb, page_stride, page_size, N, Hq, Hkv, hd, A.scale_log2, window, err};
+  const Pieces P = {A.part_o, A.part_ml, pieces, Hq, window};
+  const TreeArgs R = {pos, seq_row, seg, ancestors, table, S, words, mb, page_stride, page_size, num_pages, N, Hq, Hkv, hd, A.scale_log2, window, err};
   return dtype == FZ_F32 ? launch_merge<float>((const float*)q, (const float*)k_pool, (const float*)v_pool, (float*)out, P, R, stream)
                          : launch_merge<__nv_bfloat16>((const __nv_bfloat16*)q, (const __nv_bfloat16*)k_pool, (const __nv_bfloat16*)v_pool,
                                                        (__nv_bfloat16*)out, P, R, stream);

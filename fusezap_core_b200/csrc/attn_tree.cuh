@@ -43,10 +43,18 @@ struct TreeArgs {
   const int *pos, *seq_row, *seg, *ancestors, *table;
   int S, words, mb;
   long long page_stride;
-  int page_size, N, Hq, Hkv, hd;
+  int page_size, num_pages, N, Hq, Hkv, hd;
   float scale_log2;
   int window;
   int* err;
+};
+
+// Where a row's pieces of the context lie in the scratch (place `first + i * step` of its rows), and the context places [extra_from,
+// extra_to) that the row sees beside them.
+struct Range {
+  int pieces;
+  size_t first;
+  int step, extra_from, extra_to;
 };
 
 __device__ __forceinline__ float4 load4(const float* p) { return *(const float4*)p; }
@@ -66,7 +74,6 @@ constexpr int MERGE_WARPS = 8;
 // A warp per row and head; a lane has the dimensions 4 lane + 128 c. The context's pieces in rising order of their keys, then
 // the row's set bits in rising order, four keys at a time so that their loads and their sums over the lanes overlap. m, l, o:
 // maximum (exp2 domain), sum of weights and weighted values so far, float32.
-// `where.count` pieces of a row, `where.slot` their places in the scratch.
 template <typename T, typename Where, int CH>
 __global__ void __launch_bounds__(32 * MERGE_WARPS)
 attn_tree_merge_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, const T* __restrict__ v_pool, T* __restrict__ out,
@@ -77,9 +84,9 @@ attn_tree_merge_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, co
   if (h >= A.Hq) return;
   T* dst = out + ((size_t)n * A.Hq + h) * A.hd;
   const int s = A.seq_row[n];
-  const bool there = s >= 0 && s < A.S;
+  const bool there = s >= 0 && s < A.S && n >= A.seg[4 * s] && n - A.seg[4 * s] < A.seg[4 * s + 1];
   if (!there) {      // a padding row
-    if (s >= A.S && lane == 0) atomicOr(A.err, FZ_ERR_ROW_RANGE);
+    if (s >= 0 && lane == 0) atomicOr(A.err, FZ_ERR_ROW_RANGE);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
       if (4 * lane + 128 * c < A.hd) save4(dst + 4 * lane + 128 * c, make_float4(0.f, 0.f, 0.f, 0.f));
@@ -95,10 +102,12 @@ attn_tree_merge_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, co
     o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
     qv[c] = in ? load4(from + 4 * lane + 128 * c) : o[c];
   }
-  const int pieces = where.count(s, start, n - row0, h, kvh);
+  const int group = A.Hq / A.Hkv;
+  const Range range = where.range(n, h, s, n - row0, kvh, h - kvh * group, nodes, start, A.pos[n]);
+  const int pieces = range.pieces;
   for (int f0 = 0; f0 < pieces; f0 += 32) {
     const int here = min(32, pieces - f0);
-    const float2 ml = lane < here ? *(const float2*)(where.part_ml + 2 * where.slot(n, h, s, n - row0, f0 + lane)) : make_float2(-INFINITY, 0.f);
+    const float2 ml = lane < here ? *(const float2*)(where.part_ml + 2 * (range.first + (size_t)(f0 + lane) * range.step)) : make_float2(-INFINITY, 0.f);
     float top = ml.x;
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
@@ -114,7 +123,7 @@ attn_tree_merge_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, co
       const float w = __shfl_sync(0xffffffffu, e, f), add = __shfl_sync(0xffffffffu, ml.y, f);
       if (w == 0.f) continue;      // (a piece of which the row sees nothing may hold anything)
       l = fmaf(add, w, l);
-      const float* src = where.part_o + where.slot(n, h, s, n - row0, f0 + f) * A.hd;
+      const float* src = where.part_o + (range.first + (size_t)(f0 + f) * range.step) * A.hd;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         if (4 * lane + 128 * c < A.hd) {
@@ -125,68 +134,80 @@ attn_tree_merge_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, co
     }
   }
   const int* trow = A.table + (size_t)s * A.mb;
+  // up to four places (-1: none)
+  auto attend = [&](const int (&places)[4]) {
+    float4 kv[4][CH], vv[4][CH];
+    float sc[4];
+    bool ok[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      ok[u] = places[u] >= 0;
+      long long off = 0;
+      if (ok[u]) {
+        const int pi = places[u] / A.page_size;
+        const int page = pi < A.mb ? trow[pi] : -1;
+        ok[u] = page >= 0 && page < A.num_pages;
+        if (ok[u]) off = (long long)page * A.page_stride + ((long long)kvh * A.page_size + (places[u] - pi * A.page_size)) * A.hd;
+        else if (lane == 0) atomicOr(A.err, FZ_ERR_NO_PAGE);
+      }
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const bool in = ok[u] && 4 * lane + 128 * c < A.hd;
+        kv[u][c] = in ? load4(k_pool + off + 4 * lane + 128 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        vv[u][c] = in ? load4(v_pool + off + 4 * lane + 128 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      sc[u] = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        sc[u] = fmaf(qv[c].x, kv[u][c].x, sc[u]); sc[u] = fmaf(qv[c].y, kv[u][c].y, sc[u]);
+        sc[u] = fmaf(qv[c].z, kv[u][c].z, sc[u]); sc[u] = fmaf(qv[c].w, kv[u][c].w, sc[u]);
+      }
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) sc[u] += __shfl_xor_sync(0xffffffffu, sc[u], x);
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      sc[u] = ok[u] ? sc[u] * A.scale_log2 : -INFINITY;
+      mn = fmaxf(mn, sc[u]);
+    }
+    const float mu = mn == -INFINITY ? 0.f : mn, corr = exp2f(m - mu);
+    m = mn;
+    l *= corr;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) { o[c].x *= corr; o[c].y *= corr; o[c].z *= corr; o[c].w *= corr; }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (!ok[u]) continue;
+      const float e = exp2f(sc[u] - mu);
+      l += e;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        o[c].x = fmaf(vv[u][c].x, e, o[c].x); o[c].y = fmaf(vv[u][c].y, e, o[c].y);
+        o[c].z = fmaf(vv[u][c].z, e, o[c].z); o[c].w = fmaf(vv[u][c].w, e, o[c].w);
+      }
+    }
+  };
+  for (int x = range.extra_from; x < range.extra_to; x += 4) {
+    const int places[4] = {x, x + 1 < range.extra_to ? x + 1 : -1, x + 2 < range.extra_to ? x + 2 : -1, x + 3 < range.extra_to ? x + 3 : -1};
+    attend(places);
+  }
   for (int w0 = 0; w0 < A.words && 32 * w0 < nodes; ++w0) {
     unsigned bits = (unsigned)A.ancestors[(size_t)n * A.words + w0];
     if (nodes - 32 * w0 < 32) bits &= (1u << (nodes - 32 * w0)) - 1u;
     while (bits) {
-      float4 kv[4][CH], vv[4][CH];
-      float sc[4];
-      bool ok[4];
+      int places[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        ok[u] = bits != 0;
-        long long off = 0;
-        if (ok[u]) {
-          const int place = start + 32 * w0 + __ffs(bits) - 1;
-          bits &= bits - 1;
-          const int pi = place / A.page_size;
-          const int page = pi < A.mb ? trow[pi] : -1;
-          ok[u] = page >= 0;
-          if (ok[u]) off = (long long)page * A.page_stride + ((long long)kvh * A.page_size + (place - pi * A.page_size)) * A.hd;
-          else if (lane == 0) atomicOr(A.err, FZ_ERR_NO_PAGE);
-        }
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          const bool in = ok[u] && 4 * lane + 128 * c < A.hd;
-          kv[u][c] = in ? load4(k_pool + off + 4 * lane + 128 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
-          vv[u][c] = in ? load4(v_pool + off + 4 * lane + 128 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+        places[u] = bits ? start + 32 * w0 + __ffs(bits) - 1 : -1;
+        bits &= bits - 1;
       }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        sc[u] = 0.f;
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          sc[u] = fmaf(qv[c].x, kv[u][c].x, sc[u]); sc[u] = fmaf(qv[c].y, kv[u][c].y, sc[u]);
-          sc[u] = fmaf(qv[c].z, kv[u][c].z, sc[u]); sc[u] = fmaf(qv[c].w, kv[u][c].w, sc[u]);
-        }
-      }
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) sc[u] += __shfl_xor_sync(0xffffffffu, sc[u], x);
-      float mn = m;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        sc[u] = ok[u] ? sc[u] * A.scale_log2 : -INFINITY;
-        mn = fmaxf(mn, sc[u]);
-      }
-      const float mu = mn == -INFINITY ? 0.f : mn, corr = exp2f(m - mu);
-      m = mn;
-      l *= corr;
-#pragma unroll
-      for (int c = 0; c < CH; ++c) { o[c].x *= corr; o[c].y *= corr; o[c].z *= corr; o[c].w *= corr; }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (!ok[u]) continue;
-        const float e = exp2f(sc[u] - mu);
-        l += e;
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          o[c].x = fmaf(vv[u][c].x, e, o[c].x); o[c].y = fmaf(vv[u][c].y, e, o[c].y);
-          o[c].z = fmaf(vv[u][c].z, e, o[c].z); o[c].w = fmaf(vv[u][c].w, e, o[c].w);
-        }
-      }
+      attend(places);
     }
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;      // (a row that sees no key gives zeros)

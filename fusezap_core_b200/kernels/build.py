@@ -42,6 +42,7 @@ LIBRARIES: dict[str, list[str]] = {
     "fzb200_seq_tc": ["attn_sink_mma.cu"],                                   # bfloat16 only: that attention on tensor cores
     # drafted tokens: attention of a tree over the cache, the verdict on it, cache rows and pages moved (both dtypes)
     "fzb200_drafts": ["attn_tree.cu", "verify.cu", "cache_rows.cu"],
+    "fzb200_drafts_tc": ["attn_tree_tc.cu"],                                 # bfloat16 only: that attention on tensor cores
     "fzb200_tc": ["gemm_tc.cu"],                                             # bfloat16 only: tcgen05 / TMA products
     # bfloat16 only: attention over separate keys and values per kv head (tcgen05 / TMA / mma.sync); built when a model
     # with such a mixer asks for it

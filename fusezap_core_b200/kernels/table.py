@@ -128,7 +128,7 @@ class CudaOps(Ops):
         if self.dtype == torch.bfloat16:
             self.tc = load("fzb200_tc")      # tcgen05 / TMA kernels
         self.use_tensor_cores = self.tc is not None
-        self._attn_tc = self._mix = self._mix_tc = self._latent = self._latent_tc = self._seq = self._seq_tc = self._rows = self._ssd = self._ssd_tc = self._gla = self._scan_tc = self._drafts = None   # libraries loaded (and built) when a part first asks for their kernels
+        self._attn_tc = self._mix = self._mix_tc = self._latent = self._latent_tc = self._seq = self._seq_tc = self._rows = self._ssd = self._ssd_tc = self._gla = self._scan_tc = self._drafts = self._drafts_tc = None   # libraries loaded (and built) when a part first asks for their kernels
         self.prefill_tcgen05 = True        # False: long portions on the mma.sync flash-attention kernel
         self.fuse_swiglu = True            # gate/up product and SwiGLU in one kernel where the sizes allow it
         self.fuse_norm = True              # a sublayer's last product, the residual add and the norm behind it in one kernel
@@ -147,6 +147,7 @@ class CudaOps(Ops):
         self._meta_rows = None             # meta.seq_row of the step being run, for ops that take no `meta`
         self.scan_tensor_cores = True      # linear attention and delta-rule scans of long portions on tensor cores (bfloat16)
         self.ssd_tensor_cores = True       # state space scan of long portions on tensor cores (bfloat16)
+        self.tree_tensor_cores = True      # attention of drafted trees on tensor cores where the sizes allow it (bfloat16)
         self.split_decode_keys = True      # windowed attention with a sink: steps of single tokens cut a row's keys into runs
         self.sink_tensor_cores = True      # that attention on tensor cores for portions of SINK_MMA_ROWS rows and more (bfloat16)
         # the fewest query heads, and the fewest items of a query tile on the prompt kernel, among the attention layers
@@ -224,6 +225,14 @@ class CudaOps(Ops):
         if self._drafts is None:
             self._drafts = load("fzb200_drafts")
         return self._drafts
+
+    @property
+    def drafts_tc(self):
+        """That attention on tensor cores (bfloat16)."""
+        if self._drafts_tc is None:
+            self._drafts_tc = load("fzb200_drafts_tc")
+            self._drafts_tc.fz_attn_tree_tc_slots.restype = c_longlong
+        return self._drafts_tc
 
     @property
     def scan_tc(self):
@@ -843,11 +852,22 @@ class CudaOps(Ops):
         if n == 0:
             return
         # scratch of the call alone (from the stream's allocator, or the graph's that records it): two calls never share it
+        num_pages = k.shape[0]
+        if self.tree_tensor_cores and self.use_tensor_cores and \
+                self.drafts_tc.fz_attn_tree_tc_check(num_heads, num_kv_heads, head_dim, cache.page_size) == 0 and \
+                page_stride == 2 * num_kv_heads * cache.page_size * head_dim and v.data_ptr() - k.data_ptr() == page_stride:
+            slots = self.drafts_tc.fz_attn_tree_tc_slots(n, segments, num_heads, num_kv_heads)
+            part = torch.empty(slots * 128 * (head_dim + 2), dtype=torch.float32, device=self.device)
+            self._launch(self.drafts_tc.fz_attn_tree_tc, "tree_attention (tensor cores)",
+                         (_p(q), _p(k), _p(v), _p(meta.pos), _p(meta.seq_row), _p(seg), segments, _p(bits), bits.shape[1], _p(table), pages,
+                          c_longlong(page_stride), cache.page_size, num_pages, _p(out), n, num_heads, num_kv_heads, head_dim, c_float(scale),
+                          window, _p(part), _p(self.err)), kernels=2)
+            return
         pieces = self.drafts.fz_attn_tree_pieces(meta.max_context, window)
         part = torch.empty(n * num_heads * pieces * (head_dim + 2), dtype=torch.float32, device=self.device)
         self._launch(self.drafts.fz_attn_tree, "tree_attention",
                      (_p(q), _p(k), _p(v), _p(meta.pos), _p(meta.seq_row), _p(seg), segments, _p(bits), bits.shape[1], _p(table), pages,
-                      c_longlong(page_stride), cache.page_size, _p(out), _CODE[self.dtype], n, num_heads, num_kv_heads, head_dim,
+                      c_longlong(page_stride), cache.page_size, num_pages, _p(out), _CODE[self.dtype], n, num_heads, num_kv_heads, head_dim,
                       c_float(scale), window, pieces, _p(part), _p(self.err)), kernels=2)
 
     def verify_tree(self, logits, draft, temperature, uniform, tokens, parents, seg, path, count, next_ids) -> None:

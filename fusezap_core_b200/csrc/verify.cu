@@ -12,7 +12,7 @@
 // through distributed shared memory after which all blocks know the sums and take the same decisions. Only the rows of nodes
 // that the walk visits are read. A pass keeps its sums per warp, whose tokens are one run each, so the last pass before the draw
 // already says in whose run the drawn token lies: one warp walks that run again, in index order.
-// exp in float64 by a table of 2^(j/64) and a Taylor polynomial (the table-driven method of P. T. P. Tang, 1989): ten float64
+// exp in float64 by a table of 2^(j/256) and a Taylor polynomial (the table-driven method of P. T. P. Tang, 1989): ten float64
 // operations a token, so that a pass is not bound by them (a draw's place among 100,000 running sums needs more than 32 bits).
 #include "common.cuh"
 #include <cooperative_groups.h>
@@ -25,21 +25,20 @@ constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int MAX_NODES = 1024;      // nodes of a tree
 
 struct Ref {      // a row's scale: token x weighs exp((x - top) / T)
-  double scale, top;      // 64 log2(e) / T, and the row's maximum
+  double scale, top;      // 256 log2(e) / T, and the row's maximum
 };
 
-// The token's weight, tab[j] = 2^(j / 64); 1 for x = top exactly. -inf gives 0, NaN and +inf NaN. Here and where p and q are
-// made from weights the roundings are written out: every place that needs a token's p gets the same bits.
+// The token's weight, tab[j] = 2^(j / 256); 1 for x = top exactly. -inf gives 0; a row that holds a NaN or +inf is not asked for.
+// Here and where p and q are made from weights the roundings are written out: every place that needs a token's p gets the same
+// bits.
 __device__ __forceinline__ double weight(float x, const Ref& r, const double* tab) {
-  const double t = __dmul_rn(__dadd_rn((double)x, -r.top), r.scale);      // 64 log2 of the weight
-  if (!(t > -65000.0)) return t == t ? 0.0 : t;          // (below 2^-1015: nothing beside a maximum of 1)
-  const double big = 6755399441055744.0;                 // 1.5 * 2^52: the low bits of the sum are the nearest whole number
+  const double t = __dmul_rn(__dadd_rn((double)x, -r.top), r.scale);      // 256 log2 of the weight
+  const double big = 6755399441055744.0;                                  // 1.5 * 2^52: the low bits of the sum are the nearest whole number
   const double shifted = __dadd_rn(t, big), f = __dadd_rn(t, -__dadd_rn(shifted, -big));
   const int k = __double2loint(shifted);
-  constexpr double c1 = 0.010830424696249145, c2 = 5.86490495505617e-05, c3 = 2.1173137155464776e-07,
-                   c4 = 5.732851688640402e-10;      // (ln 2 / 64)^i / i!
-  const double e = __dmul_rn(tab[k & 63], fma(f, fma(f, fma(f, fma(f, c4, c3), c2), c1), 1.0));
-  return __hiloint2double(__double2hiint(e) + ((k >> 6) << 20), __double2loint(e));
+  constexpr double c1 = 0.0027076061740622863, c2 = 3.6655655969101062e-06, c3 = 3.3083026805413713e-09;      // (ln 2 / 256)^i / i!
+  const double e = __dmul_rn(tab[k & 255], fma(f, fma(f, fma(f, c3, c2), c1), 1.0));
+  return t > -260000.0 ? __hiloint2double(__double2hiint(e) + ((k >> 8) << 20), __double2loint(e)) : 0.0;      // (0 below 2^-1015)
 }
 
 __device__ __forceinline__ bool better(float v, int i, float bv, int bi) {      // numpy.argmax: a NaN is the maximum, then the lower index
@@ -57,44 +56,91 @@ __device__ __forceinline__ double warp_sum_d(double v) {
   return v;
 }
 
-struct Stat { float top; double sum; };
-__device__ __forceinline__ Stat join(const Stat& a, const Stat& b, double scale, const double* tab) {
-  if (a.top == b.top) return {a.top, a.sum + b.sum};      // (two without tokens: -inf, 0)
-  const Stat &hi = a.top > b.top ? a : b, &lo = a.top > b.top ? b : a;
-  if (lo.sum == 0.0) return {hi.top, hi.sum + lo.sum};
-  return {hi.top, fma(lo.sum, weight(lo.top, Ref{scale, (double)hi.top}, tab), hi.sum)};
-}
-
 struct Slot {      // what a block tells the others after a pass
   float top_p, top_q;
   double sum_p, sum_q;
-  int arg;
+  int arg, bad;
 };
 
 struct Shared {
-  double tab[64];
-  Slot slot[2];
+  double tab[256];
+  Slot slot[2], all;
   float top_p[WARPS], top_q[WARPS];
   double sum_p[WARPS], sum_q[WARPS], run[WARPS];
   int arg[WARPS];
+  // the request's tree
+  double uniform[MAX_NODES];
+  int token[MAX_NODES], parent[MAX_NODES];
   // the rejected siblings at the node: token, 1 / sum of p after it, 1 / sum of q before it
   double scale_p[MAX_NODES], scale_q[MAX_NODES];
-  int token[MAX_NODES];
+  int fallen[MAX_NODES];
 };
+
+constexpr int CHUNK = 16;      // tokens of a row that a lane has in registers at a time
+
+// A lane's CHUNK tokens of a warp's 32 * CHUNK from i0 on, -inf from hi on: token j is i0 + place(j).
+__device__ __forceinline__ int place(int j, bool vec, int lane) { return vec ? 4 * lane + 128 * (j >> 2) + (j & 3) : lane + 32 * j; }
+__device__ __forceinline__ void load_chunk(const float* __restrict__ row, int i0, int hi, bool vec, int lane, float (&x)[CHUNK]) {
+  if (vec) {
+#pragma unroll
+    for (int j = 0; j < CHUNK; j += 4) {
+      const int i = i0 + place(j, true, lane);
+      const float4 v = i < hi ? *(const float4*)(row + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      x[j] = v.x, x[j + 1] = v.y, x[j + 2] = v.z, x[j + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < CHUNK; ++j) {
+      const int i = i0 + place(j, false, lane);
+      x[j] = i < hi ? row[i] : -INFINITY;
+    }
+  }
+}
+
+// A chunk joins a lane's statistics: its sum goes by its own maximum so far.
+__device__ __forceinline__ void add_chunk(const float (&x)[CHUNK], float& top, double& sum, bool& bad, double scale, const double* tab) {
+  float m = top;
+#pragma unroll
+  for (int j = 0; j < CHUNK; ++j) m = fmaxf(m, x[j]);
+  if (m > top) {
+    if (sum != 0.0) sum *= weight(top, Ref{scale, (double)m}, tab);
+    top = m;
+  }
+  const Ref r = {scale, top == -INFINITY ? 0.0 : (double)top};
+  double part[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+  for (int j = 0; j < CHUNK; ++j) {
+    bad = bad || !(x[j] <= 3.402823466e38f);      // a NaN, +inf
+    part[j & 3] += weight(x[j], r, tab);
+  }
+  sum += (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// The lanes' (the first `width` of them; a power of two) maxima and sums as one, in every one of these lanes.
+__device__ __forceinline__ void join_lanes(float& top, double& sum, int width, double scale, const double* tab) {
+  float m = top;
+  for (int o = width >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  double v = sum == 0.0 ? 0.0 : sum * weight(top, Ref{scale, (double)m}, tab);
+  for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  top = m;
+  sum = v;
+}
 
 template <int BLOCKS>
 __global__ void __launch_bounds__(THREADS, 1)
 verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft, const float* __restrict__ temperature,
               const double* __restrict__ uniform, const int* __restrict__ tokens, const int* __restrict__ parents,
               const int* __restrict__ seg, int N, int V, int* __restrict__ path, int* __restrict__ count, int* __restrict__ next_ids, int* err) {
-  __shared__ Shared sh;
+  extern __shared__ __align__(16) unsigned char verify_smem[];
+  Shared& sh = *(Shared*)verify_smem;
   cg::cluster_group cluster = cg::this_cluster();
   fz_grid_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int s = blockIdx.x / BLOCKS, rank = blockIdx.x % BLOCKS;
-  if (tid < 64) sh.tab[tid] = exp2((double)tid / 64.0);
+  if (tid < 256) sh.tab[tid] = exp2((double)tid / 256.0);
   fz_grid_wait();
   const int row0 = seg[4 * s], n = seg[4 * s + 1];
+  const float T = temperature[s];
   const bool first = rank == 0 && tid == 0;
   if (n <= 0 || row0 < 0 || row0 + n > N || n > MAX_NODES) {      // (the whole cluster)
     if (first) {
@@ -104,74 +150,55 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     }
     return;
   }
+  for (int i = tid; i < n; i += THREADS) {
+    sh.uniform[i] = uniform[row0 + i];
+    sh.token[i] = tokens[row0 + i];
+    sh.parent[i] = parents[row0 + i];
+  }
   __syncthreads();
-  const float T = temperature[s];
   const bool greedy = !(T > 0.f);
-  const double scale = 92.33248261689366 / (double)T;      // 64 log2(e) / T
+  const double scale = 369.3299304675746 / (double)T;      // 256 log2(e) / T
   // this warp's run of tokens: [lo, hi), within the block's part of the vocabulary; multiples of four
   const int per_warp = ((V + BLOCKS * WARPS - 1) / (BLOCKS * WARPS) + 3) & ~3;
   const int lo = min(V, (rank * WARPS + warp) * per_warp), hi = min(V, lo + per_warp);
   const bool vec = (V & 3) == 0 && (((uintptr_t)logits | (uintptr_t)draft) & 15) == 0;
   int turn = 0;
-  // Every block leaves its slot; after the barrier all read all of them (the next exchange writes the other slot).
-  auto exchange = [&](Slot mine, Slot& got, bool with_max) {
+  // Every block leaves its slot; after the barrier all have all of them (the next exchange writes the other slot). The first warp reads
+  // the slots, joins them as the pass asks for, and tells the block. `mine`: thread 0's.
+  enum { ARGMAX, STATS, SUMS };
+  auto exchange = [&](const Slot& mine, int what) -> Slot {
     if (tid == 0) sh.slot[turn] = mine;
-    if (BLOCKS == 1) __syncthreads();
-    else cluster.sync();
-    Slot r = lane < BLOCKS ? (BLOCKS == 1 ? sh.slot[turn] : *cluster.map_shared_rank(&sh.slot[turn], lane)) : Slot{-INFINITY, -INFINITY, 0.0, 0.0, -1};
-    turn ^= 1;
+    if (BLOCKS > 1) cluster.sync();
+    if (warp == 0) {
+      __syncwarp();
+      Slot r = lane < BLOCKS ? (BLOCKS == 1 ? sh.slot[turn] : *cluster.map_shared_rank(&sh.slot[turn], lane)) : Slot{-INFINITY, -INFINITY, 0.0, 0.0, -1, 0};
+      if (what == ARGMAX) {
 #pragma unroll
-    for (int o = 1; o < BLOCKS; o <<= 1) {
-      Slot b;
-      b.top_p = __shfl_xor_sync(0xffffffffu, r.top_p, o);
-      b.top_q = __shfl_xor_sync(0xffffffffu, r.top_q, o);
-      b.sum_p = __shfl_xor_sync(0xffffffffu, r.sum_p, o);
-      b.sum_q = __shfl_xor_sync(0xffffffffu, r.sum_q, o);
-      b.arg = __shfl_xor_sync(0xffffffffu, r.arg, o);
-      if (greedy) {
-        if (better(b.top_p, b.arg, r.top_p, r.arg)) { r.top_p = b.top_p; r.arg = b.arg; }
-      } else if (with_max) {
-        const Stat p = join({r.top_p, r.sum_p}, {b.top_p, b.sum_p}, scale, sh.tab), q = join({r.top_q, r.sum_q}, {b.top_q, b.sum_q}, scale, sh.tab);
-        r.top_p = p.top, r.sum_p = p.sum, r.top_q = q.top, r.sum_q = q.sum;
+        for (int o = BLOCKS >> 1; o > 0; o >>= 1) {
+          const float v = __shfl_xor_sync(0xffffffffu, r.top_p, o);
+          const int i = __shfl_xor_sync(0xffffffffu, r.arg, o);
+          if (better(v, i, r.top_p, r.arg)) { r.top_p = v; r.arg = i; }
+        }
+      } else if (what == STATS) {
+        join_lanes(r.top_p, r.sum_p, BLOCKS, scale, sh.tab);
+        join_lanes(r.top_q, r.sum_q, BLOCKS, scale, sh.tab);
+        r.bad = (int)__reduce_or_sync(0xffffffffu, (unsigned)r.bad);
       } else {
-        r.sum_p += b.sum_p;
-        r.sum_q += b.sum_q;
-      }
-    }
-    got.top_p = __shfl_sync(0xffffffffu, r.top_p, 0);
-    got.top_q = __shfl_sync(0xffffffffu, r.top_q, 0);
-    got.sum_p = __shfl_sync(0xffffffffu, r.sum_p, 0);
-    got.sum_q = __shfl_sync(0xffffffffu, r.sum_q, 0);
-    got.arg = __shfl_sync(0xffffffffu, r.arg, 0);
-  };
-  auto each = [&](const float* row, auto f) {      // f(index, x) over the warp's run
-    if (vec) {
-      for (int i = lo + 4 * lane; i < hi; i += 128) {
-        const float4 x = *(const float4*)(row + i);
-        f(i, x.x); f(i + 1, x.y); f(i + 2, x.z); f(i + 3, x.w);
-      }
-    } else {
-      for (int i = lo + lane; i < hi; i += 32) f(i, row[i]);
-    }
-  };
-  auto row_stat = [&](const float* row) {      // maximum and sum of the warp's run, in one pass: a lane's sum goes by its own maximum
-    float top = -INFINITY;
-    double sum = 0.0;
-    each(row, [&](int, float x) {
-      if (x > top) {
-        if (sum != 0.0) sum *= weight(top, Ref{scale, (double)x}, sh.tab);
-        top = x;
-      }
-      if (x != -INFINITY) sum += weight(x, Ref{scale, (double)top}, sh.tab);      // (a token left out has none, also ahead of a first one)
-    });
-    Stat st = {top, sum};
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) st = join(st, {__shfl_xor_sync(0xffffffffu, st.top, o), __shfl_xor_sync(0xffffffffu, st.sum, o)}, scale, sh.tab);
-    return st;
+        for (int o = BLOCKS >> 1; o > 0; o >>= 1) {
+          r.sum_p += __shfl_xor_sync(0xffffffffu, r.sum_p, o);
+          r.sum_q += __shfl_xor_sync(0xffffffffu, r.sum_q, o);
+        }
+      }
+      if (lane == 0) sh.all = r;
+    }
+    __syncthreads();
+    turn ^= 1;
+    return sh.all;
   };
   auto next_child = [&](int node, int after) {      // the node's next child behind `after`, or -1
     for (int j0 = after + 1; j0 < n; j0 += 32) {
-      const unsigned hit = __ballot_sync(0xffffffffu, j0 + lane < n && parents[row0 + j0 + lane] == node);
+      const unsigned hit = __ballot_sync(0xffffffffu, j0 + lane < n && sh.parent[j0 + lane] == node);
       if (hit) return j0 + __ffs(hit) - 1;
     }
     return -1;
@@ -183,11 +210,19 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     const float* lrow = logits + (size_t)(row0 + node) * V;
     const float* drow = draft ? draft + (size_t)(row0 + node) * V : nullptr;
     int child = next_child(node, node);
-    Slot mine = {-INFINITY, -INFINITY, 0.0, 0.0, -1}, all;
+    Slot mine = {-INFINITY, -INFINITY, 0.0, 0.0, -1, 0};
     if (greedy) {
       float bv = -INFINITY;
       int bi = -1;
-      each(lrow, [&](int i, float x) { if (better(x, i, bv, bi)) { bv = x; bi = i; } });
+      for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
+        float x[CHUNK];
+        load_chunk(lrow, i0, hi, vec, lane, x);
+#pragma unroll
+        for (int j = 0; j < CHUNK; ++j) {
+          const int i = i0 + place(j, vec, lane);
+          if (i < hi && better(x[j], i, bv, bi)) { bv = x[j]; bi = i; }
+        }
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
@@ -199,10 +234,10 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       if (tid == 0)
         for (int w = 0; w < WARPS; ++w)
           if (better(sh.top_p[w], sh.arg[w], mine.top_p, mine.arg)) { mine.top_p = sh.top_p[w]; mine.arg = sh.arg[w]; }
-      exchange(mine, all, false);
-      while (child >= 0 && tokens[row0 + child] != all.arg) child = next_child(node, child);
+      const int best = exchange(mine, ARGMAX).arg;
+      while (child >= 0 && sh.token[child] != best) child = next_child(node, child);
       if (child < 0) {
-        result = all.arg;
+        result = best;
         break;
       }
       node = child;
@@ -210,97 +245,109 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       ++kept;
       continue;
     }
-    // statistics of the node's rows (the drafter's only where there is a child to try)
+    // statistics of the node's rows (the drafter's only where there is a child to try); the first child's own values on their way meanwhile
     const bool with_q = drow && child >= 0;
-    {
-      const Stat p = row_stat(lrow), q = with_q ? row_stat(drow) : Stat{-INFINITY, 0.0};
-      if (lane == 0) { sh.top_p[warp] = p.top; sh.sum_p[warp] = p.sum; sh.top_q[warp] = q.top; sh.sum_q[warp] = q.sum; }
-      __syncthreads();
-      if (warp == 0) {
-        Stat a = lane < WARPS ? Stat{sh.top_p[lane], sh.sum_p[lane]} : Stat{-INFINITY, 0.0}, b = lane < WARPS ? Stat{sh.top_q[lane], sh.sum_q[lane]} : Stat{-INFINITY, 0.0};
-#pragma unroll
-        for (int o = WARPS / 2; o > 0; o >>= 1) {
-          a = join(a, {__shfl_xor_sync(0xffffffffu, a.top, o), __shfl_xor_sync(0xffffffffu, a.sum, o)}, scale, sh.tab);
-          b = join(b, {__shfl_xor_sync(0xffffffffu, b.top, o), __shfl_xor_sync(0xffffffffu, b.sum, o)}, scale, sh.tab);
-        }
-        mine = {a.top, b.top, a.sum, b.sum, 0};
-      }
+    int x = child >= 0 ? sh.token[child] : 0;
+    bool ok = x >= 0 && x < V;
+    float lx = ok ? lrow[x] : 0.f, dx = ok && with_q ? drow[x] : 0.f;
+    float top_p = -INFINITY, top_q = -INFINITY;
+    double sum_p = 0.0, sum_q = 0.0;
+    bool bad = false, bad_q = false;
+    for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
+      float a[CHUNK], b[CHUNK];
+      load_chunk(lrow, i0, hi, vec, lane, a);
+      if (with_q) load_chunk(drow, i0, hi, vec, lane, b);
+      add_chunk(a, top_p, sum_p, bad, scale, sh.tab);
+      if (with_q) add_chunk(b, top_q, sum_q, bad_q, scale, sh.tab);
     }
-    exchange(mine, all, true);
+    join_lanes(top_p, sum_p, 32, scale, sh.tab);
+    join_lanes(top_q, sum_q, 32, scale, sh.tab);
+    const int flags = (int)__reduce_or_sync(0xffffffffu, (bad ? 1u : 0u) | (bad_q ? 2u : 0u));
+    if (lane == 0) { sh.top_p[warp] = top_p; sh.sum_p[warp] = sum_p; sh.top_q[warp] = top_q; sh.sum_q[warp] = sum_q; sh.arg[warp] = flags; }
+    __syncthreads();
+    if (warp == 0) {
+      float a = lane < WARPS ? sh.top_p[lane] : -INFINITY, b = lane < WARPS ? sh.top_q[lane] : -INFINITY;
+      double u = lane < WARPS ? sh.sum_p[lane] : 0.0, v = lane < WARPS ? sh.sum_q[lane] : 0.0;
+      join_lanes(a, u, WARPS, scale, sh.tab);
+      join_lanes(b, v, WARPS, scale, sh.tab);
+      mine = {a, b, u, v, 0, (int)__reduce_or_sync(0xffffffffu, lane < WARPS ? (unsigned)sh.arg[lane] : 0u)};
+    }
+    const Slot all = exchange(mine, STATS);
+    if ((all.bad & 1) || !(all.sum_p > 0.0)) break;      // a row without a distribution: V - 1
+    const bool dead_q = with_q && ((all.bad & 2) || !(all.sum_q > 0.0));      // a drafter's row without one: no child stands, p stays
     const Ref rp = {scale, (double)all.top_p}, rq = {scale, (double)all.top_q};
     const double inv_p = 1.0 / all.sum_p;
-    double inv_q = with_q ? 1.0 / all.sum_q : 0.0, total = all.sum_p;      // total: the sum over all tokens of what `run` sums over a warp's
-    double run = sh.sum_p[warp] == 0.0 ? 0.0 : sh.sum_p[warp] * weight(sh.top_p[warp], rp, sh.tab);
+    double inv_q = with_q && !dead_q ? 1.0 / all.sum_q : 0.0, total = all.sum_p;      // total: the sum over all tokens of what `run` sums over a warp's
+    double run = sum_p == 0.0 ? 0.0 : sum_p * weight(top_p, rp, sh.tab);
     bool plain = true;                  // the draw goes by p itself (weights not divided by their sum), nothing has been rejected
     int rejected = 0;
-    // p and q of a token after `r` rejections
-    auto p_after = [&](int i, float x, float d, int r, double& qv) {
-      double pv = __dmul_rn(weight(x, rp, sh.tab), inv_p);
+    // p of a token after `r` rejections, and its q before it is divided by its sum
+    auto p_after = [&](int i, float l, float d, int r, double& qv) {
+      double pv = __dmul_rn(weight(l, rp, sh.tab), inv_p);
       double base = with_q ? weight(d, rq, sh.tab) : 0.0;
       for (int k = 0; k < r; ++k) {
-        const bool it = i == sh.token[k];
+        const bool it = i == sh.fallen[k];
         const double qk = with_q ? __dmul_rn(base, sh.scale_q[k]) : it ? 1.0 : 0.0;
         pv = __dmul_rn(fmax(__dadd_rn(pv, -qk), 0.0), sh.scale_p[k]);
         if (it) base = 0.0;
       }
-      qv = base;      // (not yet divided by its sum)
+      qv = base;
       return pv;
     };
     bool stands = false;
-    while (child >= 0) {
-      const int x = tokens[row0 + child];
-      const bool ok = x >= 0 && x < V;
+    while (child >= 0 && !dead_q) {
       if (!ok && first) atomicOr(err, FZ_ERR_TOKEN_RANGE);
       double qx = 1.0, px = 0.0;
       if (ok) {
         double base;
-        px = p_after(x, lrow[x], with_q ? drow[x] : 0.f, rejected, base);
+        px = p_after(x, lx, dx, rejected, base);
         if (with_q) qx = __dmul_rn(base, inv_q);
       }
-      if (uniform[row0 + child] * qx < px) { stands = true; break; }
-      // rejected: the sums of what p and q are now
+      if (sh.uniform[child] * qx < px) { stands = true; break; }
+      // rejected: the sums of what p and q are now (the next child's own values on their way meanwhile)
+      const int gone = ok ? x : -1;
+      child = next_child(node, child);
+      x = child >= 0 ? sh.token[child] : 0;
+      ok = x >= 0 && x < V;
+      lx = ok ? lrow[x] : 0.f, dx = ok && with_q ? drow[x] : 0.f;
       __syncthreads();      // (nobody still reads the list's last entry)
-      if (tid == 0) { sh.token[rejected] = ok ? x : -1; sh.scale_p[rejected] = 1.0; sh.scale_q[rejected] = inv_q; }
+      if (tid == 0) { sh.fallen[rejected] = gone; sh.scale_p[rejected] = 1.0; sh.scale_q[rejected] = inv_q; }
       __syncthreads();
       double sp = 0.0, sq = 0.0;
-      if (with_q && vec) {
-        for (int i = lo + 4 * lane; i < hi; i += 128) {
-          const float4 a = *(const float4*)(lrow + i), b = *(const float4*)(drow + i);
-          double q0, q1, q2, q3;
-          sp += p_after(i, a.x, b.x, rejected + 1, q0); sp += p_after(i + 1, a.y, b.y, rejected + 1, q1);
-          sp += p_after(i + 2, a.z, b.z, rejected + 1, q2); sp += p_after(i + 3, a.w, b.w, rejected + 1, q3);
-          sq += (q0 + q1) + (q2 + q3);
-        }
-      } else if (with_q) {
-        for (int i = lo + lane; i < hi; i += 32) {
+      for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
+        float a[CHUNK], b[CHUNK];
+        load_chunk(lrow, i0, hi, vec, lane, a);
+        if (with_q) load_chunk(drow, i0, hi, vec, lane, b);
+#pragma unroll
+        for (int j = 0; j < CHUNK; ++j) {      // (tokens from hi on weigh 0)
           double qv;
-          sp += p_after(i, lrow[i], drow[i], rejected + 1, qv);
+          sp += p_after(i0 + place(j, vec, lane), a[j], with_q ? b[j] : 0.f, rejected + 1, qv);
           sq += qv;
         }
-      } else {
-        each(lrow, [&](int i, float v) { double qv; sp += p_after(i, v, 0.f, rejected + 1, qv); });
       }
       sp = warp_sum_d(sp);
       sq = warp_sum_d(sq);
       if (lane == 0) { sh.sum_p[warp] = sp; sh.sum_q[warp] = sq; }
       __syncthreads();
-      Slot m2 = {0.f, 0.f, 0.0, 0.0, 0};
-      if (tid == 0)
-        for (int w = 0; w < WARPS; ++w) { m2.sum_p += sh.sum_p[w]; m2.sum_q += sh.sum_q[w]; }
-      exchange(m2, all, false);
-      if (all.sum_p > 0.0) {
+      if (warp == 0) {
+        double u = lane < WARPS ? sh.sum_p[lane] : 0.0, v = lane < WARPS ? sh.sum_q[lane] : 0.0;
+        u = warp_sum_d(u);
+        v = warp_sum_d(v);
+        mine = {0.f, 0.f, u, v, 0, 0};
+      }
+      const Slot left = exchange(mine, SUMS);
+      if (left.sum_p > 0.0) {
         total = 1.0;
         plain = false;
-        run = sp / all.sum_p;
-        if (tid == 0) sh.scale_p[rejected] = 1.0 / all.sum_p;
+        run = sp / left.sum_p;
+        if (tid == 0) sh.scale_p[rejected] = 1.0 / left.sum_p;
       } else if (tid == 0) {      // nothing is left: p stays what it was (the rejection had no probability)
         sh.scale_q[rejected] = 0.0;
-        if (!with_q) sh.token[rejected] = -1;
+        if (!with_q) sh.fallen[rejected] = -1;
       }
       __syncthreads();
-      if (with_q) inv_q = all.sum_q > 0.0 ? 1.0 / all.sum_q : 0.0;
+      if (with_q) inv_q = left.sum_q > 0.0 ? 1.0 / left.sum_q : 0.0;
       ++rejected;
-      child = next_child(node, child);
     }
     if (stands) {
       node = child;
@@ -308,74 +355,81 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       ++kept;
       continue;
     }
-    // the draw: the first token whose running sum, in index order, exceeds u * total. Blocks' runs before this one's first.
-    const double target = uniform[row0] * total;
+    // The draw: the first token whose running sum, in index order, exceeds u * total. Where a warp's run begins and ends among the
+    // running sums: the blocks before, then the warps before, added up the same way by all, so that every end is the next one's
+    // beginning.
+    const double target = fmax(sh.uniform[0], 0.0) * total;      // (a NaN: 0)
     if (lane == 0) sh.run[warp] = run;
     __syncthreads();
-    mine = {0.f, 0.f, 0.0, 0.0, 0};
-    if (tid == 0)
+    if (tid == 0) {
+      mine = {0.f, 0.f, 0.0, 0.0, 0, 0};
       for (int w = 0; w < WARPS; ++w) mine.sum_p += sh.run[w];
-    if (tid == 0) sh.slot[turn] = mine;
+      sh.slot[turn] = mine;
+    }
     if (BLOCKS == 1) __syncthreads();
     else cluster.sync();
-    // where the warp's run begins and ends among the running sums: the blocks before, then the warps before, added up the same way by
-    // all, so that every end is the next one's beginning
-    double blocks = 0.0, part = 0.0, behind = 0.0;
+    double blocks = 0.0, behind = 0.0, own_sum = 0.0;
     for (int b = 0; b < BLOCKS; ++b) {
-      const double sum = BLOCKS == 1 ? 0.0 : cluster.map_shared_rank(&sh.slot[turn], b)->sum_p;
+      const double sum = BLOCKS == 1 ? sh.slot[turn].sum_p : cluster.map_shared_rank(&sh.slot[turn], b)->sum_p;
       if (b < rank) blocks += sum;
       else if (b > rank) behind += sum;
+      else own_sum = sum;
     }
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) part += sh.run[w];
-      else if (w > warp) behind += sh.run[w];
-    }
-    const double before = blocks + part;
     turn ^= 1;
-    result = -1;
-    // (behind = 0: u so near 1 that the sums' roundings end below the target: the last token that has any probability)
-    if (run > 0.0 && before <= target && (blocks + (part + run) > target || behind == 0.0)) {
-      double at = before;
-      int found = -1, last = -1;
-      for (int i0 = lo; i0 < hi && found < 0; i0 += 32) {
-        const int i = i0 + lane;
-        double w = 0.0, unused;
-        if (i < hi) w = plain ? weight(lrow[i], rp, sh.tab) : p_after(i, lrow[i], with_q ? drow[i] : 0.f, rejected, unused);
-        double upto = w;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double v = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += v;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && at + upto > target), some = __ballot_sync(0xffffffffu, w > 0.0);
-        if (hit) found = i0 + __ffs(hit) - 1;
-        if (some) last = i0 + 31 - __clz(some);
-        at += __shfl_sync(0xffffffffu, upto, 31);
+    // (nothing behind: u so near 1 that the sums' roundings end below the target: the last token that has any probability)
+    if (own_sum > 0.0 && blocks <= target && (blocks + own_sum > target || behind == 0.0)) {
+      // this block's: the warp whose run holds it, then all threads share that run, a few neighbouring tokens each
+      int who = -1;
+      double part = 0.0, begin = 0.0;
+      for (int w = 0; w < WARPS; ++w) {
+        const double end = part + sh.run[w];
+        if (sh.run[w] > 0.0 && blocks + part <= target) { who = w; begin = blocks + part; }      // (the last one that begins at or before it)
+        part = end;
       }
-      result = found >= 0 ? found : last;      // (the run's sum, taken in another order, was a little larger)
+      const int from = min(V, (rank * WARPS + who) * per_warp), to = min(V, from + per_warp);
+      const int each = (to - from + THREADS - 1) / THREADS, i0 = min(to, from + tid * each), i1 = min(to, i0 + each);
+      auto value = [&](int i) {
+        double unused;
+        return plain ? weight(lrow[i], rp, sh.tab) : p_after(i, lrow[i], with_q ? drow[i] : 0.f, rejected, unused);
+      };
+      double mass = 0.0;
+      for (int i = i0; i < i1; ++i) mass += value(i);
+      double upto = mass;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      __syncthreads();      // (the runs have been read)
+      if (lane == 31) sh.run[warp] = upto;
+      if (tid == 0) sh.all.arg = -1;
+      __syncthreads();
+      double ahead = begin;
+      for (int w = 0; w < warp; ++w) ahead += sh.run[w];
+      double at = ahead + (upto - mass);
+      // the last thread whose tokens begin at or before the target holds it (the very sums that follow decide within it)
+      if (mass > 0.0 && at <= target) atomicMax(&sh.all.arg, tid);
+      __syncthreads();
+      if (tid == sh.all.arg) {
+        int last = -1, found = -1;
+        for (int i = i0; i < i1 && found < 0; ++i) {
+          const double v = value(i);
+          at += v;
+          if (v > 0.0) {
+            last = i;
+            if (at > target) found = i;
+          }
+        }
+        next_ids[s] = found >= 0 ? found : last;
+      }
     }
+    result = -1;      // (written)
     break;
   }
-  // the block and warp that hold the token, or (a row without a distribution) nobody: V - 1
-  if (greedy) {
-    if (first) next_ids[s] = result;
-  } else {
-    const bool mine = __any_sync(0xffffffffu, result >= 0);
-    if (lane == 0) sh.arg[warp] = mine ? result : -1;
-    __syncthreads();
-    Slot out = {0.f, 0.f, 0.0, 0.0, -1};
-    if (tid == 0)
-      for (int w = 0; w < WARPS; ++w) out.arg = max(out.arg, sh.arg[w]);
-    if (tid == 0) sh.slot[turn] = out;
-    if (BLOCKS == 1) __syncthreads();
-    else cluster.sync();
-    if (first) {
-      int id = -1;
-      for (int b = 0; b < BLOCKS; ++b) id = max(id, BLOCKS == 1 ? sh.slot[turn].arg : cluster.map_shared_rank(&sh.slot[turn], b)->arg);
-      next_ids[s] = id >= 0 ? id : V - 1;
-    }
+  if (first) {
+    if (result >= 0) next_ids[s] = result;
+    count[s] = kept;
   }
-  if (first) count[s] = kept;
   if (rank == 0)
     for (int k = kept + tid; k < n; k += THREADS) path[row0 + k] = -1;
   if (BLOCKS > 1) cluster.sync();      // nobody leaves while its slots may still be read
@@ -385,6 +439,7 @@ template <int BLOCKS>
 int launch(const float* logits, const float* draft, const float* temperature, const double* uniform, const int* tokens, const int* parents,
            const int* seg, int S, int N, int V, int* path, int* count, int* next_ids, int* err, cudaStream_t stream) {
   auto kern = verify_kernel<BLOCKS>;
+  FZ_RAISE_SMEM(kern);
   if (BLOCKS > 8) {
     static const cudaError_t wide = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (wide != cudaSuccess) return (int)wide;
@@ -392,6 +447,7 @@ int launch(const float* logits, const float* draft, const float* temperature, co
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)S * BLOCKS);
   cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -415,7 +471,7 @@ int launch(const float* logits, const float* draft, const float* temperature, co
 // Blocks per request: as many as the chip holds at once beside the other requests' (14 clusters of eight, 32 of four, 74 of two),
 // each with 2,048 tokens and more.
 FZ_API int fz_verify_blocks(int S, int V) {
-  int b = S <= 14 ? 8 : S <= 32 ? 4 : S <= 74 ? 2 : 1;
+  int b = S <= 6 ? 16 : S <= 14 ? 8 : S <= 32 ? 4 : S <= 74 ? 2 : 1;
   while (b > 1 && V < 2048 * b) b >>= 1;
   return b;
 }

@@ -480,7 +480,8 @@ class Ops:
         over its sum (if that is not 0) and q loses x, scaled to sum 1. No child stands: next_ids[s] is the token at which the
         running sum of p, in index order, first exceeds uniform[root] * total. T <= 0: the first child that is the argmax
         (the order of `argmax`) stands, else the argmax is the next token. float64. A row without a distribution (a NaN, +inf, or
-        nothing above -inf): no child stands and the draw gives V - 1.
+        nothing above -inf): no child stands and the draw gives V - 1 (a drafter's row: no child stands and p is
+        drawn from).
         Results, int32: count[s] kept nodes (the root among them; 0 for no rows, next_ids[s] = -1); path[first row + k] = node of the
         k-th of them, -1 from count[s] to the request's last row; rows of `path` beside the requests' are left."""
         raise NotImplementedError

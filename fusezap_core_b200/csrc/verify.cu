@@ -7,13 +7,19 @@
 // child stands, the next token is drawn from what p is then, so the tokens are distributed as the target's own (recursive
 // rejection sampling). T <= 0: the child that is the argmax stands, else the argmax is the next token.
 //
-// The tokens of a row are shared by the BLOCKS blocks of a cluster, one cluster per request: a walk is a chain of passes over one
-// row pair each (statistics of a node: maximum and sum; after a rejection: the sums of the new p and q), each ended by one exchange
-// through distributed shared memory after which all blocks know the sums and take the same decisions. Only the rows of nodes
-// that the walk visits are read. A pass keeps its sums per warp, whose tokens are one run each, so the last pass before the draw
-// already says in whose run the drawn token lies: one warp walks that run again, in index order.
-// exp in float64 by a table of 2^(j/256) and a Taylor polynomial (the table-driven method of P. T. P. Tang, 1989): ten float64
-// operations a token, so that a pass is not bound by them (a draw's place among 100,000 running sums needs more than 32 bits).
+// The tokens of a row are shared by the BLOCKS blocks of a cluster, one cluster per request. A walk is a chain of passes over one
+// row pair each, ended by one exchange through distributed shared memory, after which all blocks know the sums and take the same
+// decisions. Only the rows of nodes that the walk visits are read. The kinds of pass:
+//   quick   maximum and sum of p's and q's row, exponentials in float32, once per visited node. Whether a child stands is decided from
+//           these sums unless u q(x) lies within MARGIN of p(x); the sums are off by 6e-6 at most (see `quick_chunk`);
+//   first   float64, where a child falls, or is too near to call, or the draw is due: the exact sums, and with them at once the sum of
+//           max(p - q, 0). That one takes p's and q's exact sums beforehand, which are not known yet: with the quick sums' ratio a0 for
+//           a, S(a) = sum max(a p - q, 0) is S(a0) + (a - a0) times the p for which a0 p > q, up to the tokens that change sides
+//           between a0 and a (a part of 1e-6 of those within 1e-6);
+//   next    float64, for every further sibling that falls: the sums of the new p and q.
+// Sums are kept per warp, whose tokens are one run each, so the last pass before the draw already says in whose run the drawn token
+// lies: its block's threads walk that run again, a few neighbouring tokens each. A draw's place among 100,000 running sums needs more
+// than 32 bits: exp in float64 by a table of 2^(j/256) and a Taylor polynomial (the table-driven method of P. T. P. Tang, 1989).
 #include "common.cuh"
 #include <cooperative_groups.h>
 #include <math.h>
@@ -23,6 +29,7 @@ namespace cg = cooperative_groups;
 namespace {
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int MAX_NODES = 1024;      // nodes of a tree
+constexpr double MARGIN = 3e-5;      // of p(x): a decision nearer than that is taken in float64
 
 struct Ref {      // a row's scale: token x weighs exp((x - top) / T)
   double scale, top;      // 256 log2(e) / T, and the row's maximum
@@ -58,7 +65,7 @@ __device__ __forceinline__ double warp_sum_d(double v) {
 
 struct Slot {      // what a block tells the others after a pass
   float top_p, top_q;
-  double sum_p, sum_q;
+  double sum_p, sum_q, over, under;
   int arg, bad;
 };
 
@@ -66,7 +73,7 @@ struct Shared {
   double tab[256];
   Slot slot[2], all;
   float top_p[WARPS], top_q[WARPS];
-  double sum_p[WARPS], sum_q[WARPS], run[WARPS];
+  double sum_p[WARPS], sum_q[WARPS], over[WARPS], under[WARPS], run[WARPS];
   int arg[WARPS];
   // the request's tree
   double uniform[MAX_NODES];
@@ -97,8 +104,10 @@ __device__ __forceinline__ void load_chunk(const float* __restrict__ row, int i0
   }
 }
 
-// A chunk joins a lane's statistics: its sum goes by its own maximum so far.
-__device__ __forceinline__ void add_chunk(const float (&x)[CHUNK], float& top, double& sum, bool& bad, double scale, const double* tab) {
+// A chunk joins a lane's statistics, in float32: its sum goes by its own maximum so far. A weight is off by 2^-22.5 (ex2.approx) and by
+// four roundings of the exponent t, 4 |t| 2^-24 ln 2 of itself; |t| is log2(V) on average over p, 31 at most (the entropy of p is that
+// average plus log2 of the sum, and at most log2(V)); 16 weights are added in float32, chunks in float64: 6e-6 of the sum in all.
+__device__ __forceinline__ void quick_chunk(const float (&x)[CHUNK], float& top, double& sum, bool& bad, float scale2, double scale, const double* tab) {
   float m = top;
 #pragma unroll
   for (int j = 0; j < CHUNK; ++j) m = fmaxf(m, x[j]);
@@ -106,14 +115,16 @@ __device__ __forceinline__ void add_chunk(const float (&x)[CHUNK], float& top, d
     if (sum != 0.0) sum *= weight(top, Ref{scale, (double)m}, tab);
     top = m;
   }
-  const Ref r = {scale, top == -INFINITY ? 0.0 : (double)top};
-  double part[4] = {0.0, 0.0, 0.0, 0.0};
+  const float from = top == -INFINITY ? 0.f : top;
+  float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < CHUNK; ++j) {
     bad = bad || !(x[j] <= 3.402823466e38f);      // a NaN, +inf
-    part[j & 3] += weight(x[j], r, tab);
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x[j] - from) * scale2));
+    part[j & 3] += e;
   }
-  sum += (part[0] + part[1]) + (part[2] + part[3]);
+  sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
 }
 
 // The lanes' (the first `width` of them; a power of two) maxima and sums as one, in every one of these lanes.
@@ -158,6 +169,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
   __syncthreads();
   const bool greedy = !(T > 0.f);
   const double scale = 369.3299304675746 / (double)T;      // 256 log2(e) / T
+  const float scale2 = (float)fmin(scale / 256.0, 3.4e38);
   // this warp's run of tokens: [lo, hi), within the block's part of the vocabulary; multiples of four
   const int per_warp = ((V + BLOCKS * WARPS - 1) / (BLOCKS * WARPS) + 3) & ~3;
   const int lo = min(V, (rank * WARPS + warp) * per_warp), hi = min(V, lo + per_warp);
@@ -171,7 +183,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     if (BLOCKS > 1) cluster.sync();
     if (warp == 0) {
       __syncwarp();
-      Slot r = lane < BLOCKS ? (BLOCKS == 1 ? sh.slot[turn] : *cluster.map_shared_rank(&sh.slot[turn], lane)) : Slot{-INFINITY, -INFINITY, 0.0, 0.0, -1, 0};
+      Slot r = lane < BLOCKS ? (BLOCKS == 1 ? sh.slot[turn] : *cluster.map_shared_rank(&sh.slot[turn], lane)) : Slot{-INFINITY, -INFINITY, 0.0, 0.0, 0.0, 0.0, -1, 0};
       if (what == ARGMAX) {
 #pragma unroll
         for (int o = BLOCKS >> 1; o > 0; o >>= 1) {
@@ -188,6 +200,8 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
         for (int o = BLOCKS >> 1; o > 0; o >>= 1) {
           r.sum_p += __shfl_xor_sync(0xffffffffu, r.sum_p, o);
           r.sum_q += __shfl_xor_sync(0xffffffffu, r.sum_q, o);
+          r.over += __shfl_xor_sync(0xffffffffu, r.over, o);
+          r.under += __shfl_xor_sync(0xffffffffu, r.under, o);
         }
       }
       if (lane == 0) sh.all = r;
@@ -210,7 +224,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     const float* lrow = logits + (size_t)(row0 + node) * V;
     const float* drow = draft ? draft + (size_t)(row0 + node) * V : nullptr;
     int child = next_child(node, node);
-    Slot mine = {-INFINITY, -INFINITY, 0.0, 0.0, -1, 0};
+    Slot mine = {-INFINITY, -INFINITY, 0.0, 0.0, 0.0, 0.0, -1, 0};
     if (greedy) {
       float bv = -INFINITY;
       int bi = -1;
@@ -257,8 +271,8 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       float a[CHUNK], b[CHUNK];
       load_chunk(lrow, i0, hi, vec, lane, a);
       if (with_q) load_chunk(drow, i0, hi, vec, lane, b);
-      add_chunk(a, top_p, sum_p, bad, scale, sh.tab);
-      if (with_q) add_chunk(b, top_q, sum_q, bad_q, scale, sh.tab);
+      quick_chunk(a, top_p, sum_p, bad, scale2, scale, sh.tab);
+      if (with_q) quick_chunk(b, top_q, sum_q, bad_q, scale2, scale, sh.tab);
     }
     join_lanes(top_p, sum_p, 32, scale, sh.tab);
     join_lanes(top_q, sum_q, 32, scale, sh.tab);
@@ -270,16 +284,15 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       double u = lane < WARPS ? sh.sum_p[lane] : 0.0, v = lane < WARPS ? sh.sum_q[lane] : 0.0;
       join_lanes(a, u, WARPS, scale, sh.tab);
       join_lanes(b, v, WARPS, scale, sh.tab);
-      mine = {a, b, u, v, 0, (int)__reduce_or_sync(0xffffffffu, lane < WARPS ? (unsigned)sh.arg[lane] : 0u)};
+      mine = {a, b, u, v, 0.0, 0.0, 0, (int)__reduce_or_sync(0xffffffffu, lane < WARPS ? (unsigned)sh.arg[lane] : 0u)};
     }
     const Slot all = exchange(mine, STATS);
     if ((all.bad & 1) || !(all.sum_p > 0.0)) break;      // a row without a distribution: V - 1
     const bool dead_q = with_q && ((all.bad & 2) || !(all.sum_q > 0.0));      // a drafter's row without one: no child stands, p stays
     const Ref rp = {scale, (double)all.top_p}, rq = {scale, (double)all.top_q};
-    const double inv_p = 1.0 / all.sum_p;
-    double inv_q = with_q && !dead_q ? 1.0 / all.sum_q : 0.0, total = all.sum_p;      // total: the sum over all tokens of what `run` sums over a warp's
-    double run = sum_p == 0.0 ? 0.0 : sum_p * weight(top_p, rp, sh.tab);
-    bool plain = true;                  // the draw goes by p itself (weights not divided by their sum), nothing has been rejected
+    double inv_p = 1.0 / all.sum_p, inv_q = with_q && !dead_q ? 1.0 / all.sum_q : 0.0;      // (quick until `exact`)
+    double run = 0.0, total = 0.0;      // what the draw goes by: this warp's part of it and the whole
+    bool exact = false, plain = true;   // plain: the draw goes by p itself (weights not divided by their sum)
     int rejected = 0;
     // p of a token after `r` rejections, and its q before it is divided by its sum
     auto p_after = [&](int i, float l, float d, int r, double& qv) {
@@ -294,26 +307,82 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       qv = base;
       return pv;
     };
-    bool stands = false;
-    while (child >= 0 && !dead_q) {
-      if (!ok && first) atomicOr(err, FZ_ERR_TOKEN_RANGE);
-      double qx = 1.0, px = 0.0;
-      if (ok) {
-        double base;
-        px = p_after(x, lx, dx, rejected, base);
-        if (with_q) qx = __dmul_rn(base, inv_q);
+    // one exchange of four sums over all tokens; the warp's own stay in sp, sq, so, su
+    auto add_up = [&](double& sp, double& sq, double& so, double& su) {
+      sp = warp_sum_d(sp), sq = warp_sum_d(sq), so = warp_sum_d(so), su = warp_sum_d(su);
+      if (lane == 0) { sh.sum_p[warp] = sp; sh.sum_q[warp] = sq; sh.over[warp] = so; sh.under[warp] = su; }
+      __syncthreads();
+      if (warp == 0) {
+        const bool in = lane < WARPS;
+        double u = in ? sh.sum_p[lane] : 0.0, v = in ? sh.sum_q[lane] : 0.0, w = in ? sh.over[lane] : 0.0, z = in ? sh.under[lane] : 0.0;
+        u = warp_sum_d(u), v = warp_sum_d(v), w = warp_sum_d(w), z = warp_sum_d(z);
+        mine = {0.f, 0.f, u, v, w, z, 0, 0};
       }
-      if (sh.uniform[child] * qx < px) { stands = true; break; }
-      // rejected: the sums of what p and q are now (the next child's own values on their way meanwhile)
-      const int gone = ok ? x : -1;
-      child = next_child(node, child);
-      x = child >= 0 ? sh.token[child] : 0;
-      ok = x >= 0 && x < V;
-      lx = ok ? lrow[x] : 0.f, dx = ok && with_q ? drow[x] : 0.f;
+      return exchange(mine, SUMS);
+    };
+    // The first pass in float64: exact sums, and if a child x has fallen (x = -1: none) the sums of p and q after it. Returns false where
+    // the sum of max(p - q, 0) came out too small to be had this way (p and q nearly the same).
+    auto first_pass = [&](int gone, float lg, float dg, bool fell) -> bool {
+      const double a0 = with_q ? inv_p / inv_q : 0.0;
+      double sp = 0.0, sq = 0.0, so = 0.0, su = 0.0;
+      for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
+        float a[CHUNK], b[CHUNK];
+        load_chunk(lrow, i0, hi, vec, lane, a);
+        if (with_q) load_chunk(drow, i0, hi, vec, lane, b);
+#pragma unroll
+        for (int j = 0; j < CHUNK; ++j) {      // (tokens from hi on weigh 0)
+          const double wp = weight(a[j], rp, sh.tab);
+          if (with_q) {
+            const double wq = weight(b[j], rq, sh.tab), over = fma(a0, wp, -wq);
+            const bool it = i0 + place(j, vec, lane) == gone;
+            sp += wp;
+            sq += it ? 0.0 : wq;
+            so += fmax(over, 0.0);
+            su += over > 0.0 ? wp : 0.0;
+          } else {
+            sp += i0 + place(j, vec, lane) == gone ? 0.0 : wp;
+          }
+        }
+      }
+      const Slot sum = add_up(sp, sq, so, su);
+      const double wg = gone >= 0 ? weight(lg, rp, sh.tab) : 0.0, dgw = gone >= 0 && with_q ? weight(dg, rq, sh.tab) : 0.0;
+      const double all_p = with_q ? sum.sum_p : sum.sum_p + wg, all_q = sum.sum_q + dgw;
+      inv_p = 1.0 / all_p;
+      if (with_q) inv_q = 1.0 / all_q;
+      exact = true;
+      run = sp, total = sum.sum_p, plain = true;
+      if (!fell) return true;
+      // the list's entry for x; the draw's sums
+      double left = 0.0;
+      bool good = true;
+      if (with_q) {
+        const double da = all_q / all_p - a0;
+        left = (sum.over + da * sum.under) / all_q;
+        good = left > 1e-6;
+        if (good) run = (so + da * su) / all_q / left, total = 1.0, plain = false;
+      } else if (sum.sum_p > 0.0) {
+        left = sum.sum_p / all_p;
+        run = sp / sum.sum_p, total = 1.0, plain = false;
+      } else {
+        run = sp + (gone >= lo && gone < hi ? wg : 0.0), total = all_p;      // (p stays what it was)
+      }
+      if (!good) return false;
+      if (tid == 0) {
+        sh.fallen[0] = !with_q && left <= 0.0 ? -1 : gone;
+        sh.scale_p[0] = left > 0.0 ? 1.0 / left : 1.0;
+        sh.scale_q[0] = inv_q;
+      }
+      __syncthreads();
+      if (with_q) inv_q = sum.sum_q > 0.0 ? 1.0 / sum.sum_q : 0.0;
+      rejected = 1;
+      return true;
+    };
+    // a further pass: child `gone` falls from p and q as `rejected` children have left them
+    auto next_pass = [&](int gone) {
       __syncthreads();      // (nobody still reads the list's last entry)
       if (tid == 0) { sh.fallen[rejected] = gone; sh.scale_p[rejected] = 1.0; sh.scale_q[rejected] = inv_q; }
       __syncthreads();
-      double sp = 0.0, sq = 0.0;
+      double sp = 0.0, sq = 0.0, so = 0.0, su = 0.0;
       for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
         float a[CHUNK], b[CHUNK];
         load_chunk(lrow, i0, hi, vec, lane, a);
@@ -325,17 +394,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
           sq += qv;
         }
       }
-      sp = warp_sum_d(sp);
-      sq = warp_sum_d(sq);
-      if (lane == 0) { sh.sum_p[warp] = sp; sh.sum_q[warp] = sq; }
-      __syncthreads();
-      if (warp == 0) {
-        double u = lane < WARPS ? sh.sum_p[lane] : 0.0, v = lane < WARPS ? sh.sum_q[lane] : 0.0;
-        u = warp_sum_d(u);
-        v = warp_sum_d(v);
-        mine = {0.f, 0.f, u, v, 0, 0};
-      }
-      const Slot left = exchange(mine, SUMS);
+      const Slot left = add_up(sp, sq, so, su);
       if (left.sum_p > 0.0) {
         total = 1.0;
         plain = false;
@@ -348,6 +407,34 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       __syncthreads();
       if (with_q) inv_q = left.sum_q > 0.0 ? 1.0 / left.sum_q : 0.0;
       ++rejected;
+    };
+    bool stands = false;
+    for (;;) {
+      enum { EXACT, FALL_FIRST, FALL_NEXT } todo = EXACT;
+      int gone = -1;
+      float lg = 0.f, dg = 0.f;
+      if (child < 0 || dead_q) {
+        if (exact) break;      // (the draw's sums are there)
+      } else {
+        if (!ok && first) atomicOr(err, FZ_ERR_TOKEN_RANGE);
+        double qx = 1.0, px = 0.0, base;
+        if (ok) {
+          px = p_after(x, lx, dx, rejected, base);
+          if (with_q) qx = __dmul_rn(base, inv_q);
+        }
+        const double ux = sh.uniform[child] * qx;
+        if (exact || px == 0.0 || fabs(ux - px) > MARGIN * px) {
+          if (ux < px) { stands = true; break; }
+          todo = exact ? FALL_NEXT : FALL_FIRST;
+          if (ok) gone = x, lg = lx, dg = dx;
+          child = next_child(node, child);      // (the next child's own values on their way meanwhile)
+          x = child >= 0 ? sh.token[child] : 0;
+          ok = x >= 0 && x < V;
+          lx = ok ? lrow[x] : 0.f, dx = ok && with_q ? drow[x] : 0.f;
+        }
+      }
+      if (todo != FALL_NEXT && !first_pass(gone, lg, dg, todo == FALL_FIRST)) todo = FALL_NEXT;
+      if (todo == FALL_NEXT) next_pass(gone);
     }
     if (stands) {
       node = child;
@@ -362,7 +449,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     if (lane == 0) sh.run[warp] = run;
     __syncthreads();
     if (tid == 0) {
-      mine = {0.f, 0.f, 0.0, 0.0, 0, 0};
+      mine = {0.f, 0.f, 0.0, 0.0, 0.0, 0.0, 0, 0};
       for (int w = 0; w < WARPS; ++w) mine.sum_p += sh.run[w];
       sh.slot[turn] = mine;
     }

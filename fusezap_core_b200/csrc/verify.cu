@@ -33,19 +33,24 @@ constexpr double MARGIN = 3e-5;      // of p(x): a decision nearer than that is 
 
 struct Ref {      // a row's scale: token x weighs exp((x - top) / T)
   double scale, top;      // 256 log2(e) / T, and the row's maximum
+  float cut;              // tokens below it weigh as much as it: NOTHING at most
 };
+constexpr double NOTHING = 1e-290;      // weights and probabilities up to this count as 0
+// (2^-1015 is 260,000 / 256 powers of two below 1; -inf must not reach the subtraction)
+__device__ __forceinline__ Ref ref_of(float top, double scale) {
+  return {scale, (double)top, (float)fmax((double)top - 260000.0 / scale, -3.0e38)};
+}
 
-// The token's weight, tab[j] = 2^(j / 256); 1 for x = top exactly. -inf gives 0; a row that holds a NaN or +inf is not asked for.
-// Here and where p and q are made from weights the roundings are written out: every place that needs a token's p gets the same
-// bits.
+// The token's weight, tab[j] = 2^(j / 256); 1 for x = top exactly. A row that holds a NaN or +inf is not asked for. Here and where p
+// and q are made from weights the roundings are written out: every place that needs a token's p gets the same bits.
 __device__ __forceinline__ double weight(float x, const Ref& r, const double* tab) {
-  const double t = __dmul_rn(__dadd_rn((double)x, -r.top), r.scale);      // 256 log2 of the weight
+  const double t = __dmul_rn(__dadd_rn((double)fmaxf(x, r.cut), -r.top), r.scale);      // 256 log2 of the weight
   const double big = 6755399441055744.0;                                  // 1.5 * 2^52: the low bits of the sum are the nearest whole number
   const double shifted = __dadd_rn(t, big), f = __dadd_rn(t, -__dadd_rn(shifted, -big));
   const int k = __double2loint(shifted);
   constexpr double c1 = 0.0027076061740622863, c2 = 3.6655655969101062e-06, c3 = 3.3083026805413713e-09;      // (ln 2 / 256)^i / i!
   const double e = __dmul_rn(tab[k & 255], fma(f, fma(f, fma(f, c3, c2), c1), 1.0));
-  return t > -260000.0 ? __hiloint2double(__double2hiint(e) + ((k >> 8) << 20), __double2loint(e)) : 0.0;      // (0 below 2^-1015)
+  return __hiloint2double(__double2hiint(e) + (k & ~255) * 4096, __double2loint(e));
 }
 
 __device__ __forceinline__ bool better(float v, int i, float bv, int bi) {      // numpy.argmax: a NaN is the maximum, then the lower index
@@ -85,41 +90,38 @@ struct Shared {
 
 constexpr int CHUNK = 16;      // tokens of a row that a lane has in registers at a time
 
-// A lane's CHUNK tokens of a warp's 32 * CHUNK from i0 on, -inf from hi on: token j is i0 + place(j).
-__device__ __forceinline__ int place(int j, bool vec, int lane) { return vec ? 4 * lane + 128 * (j >> 2) + (j & 3) : lane + 32 * j; }
+// A lane's CHUNK tokens of a warp's 32 * CHUNK from i0 on, -inf from hi on: token j is i0 + 4 lane + step(j).
+__device__ __forceinline__ constexpr int step(int j) { return 128 * (j >> 2) + (j & 3); }
 __device__ __forceinline__ void load_chunk(const float* __restrict__ row, int i0, int hi, bool vec, int lane, float (&x)[CHUNK]) {
+  const int at = i0 + 4 * lane;
   if (vec) {
 #pragma unroll
     for (int j = 0; j < CHUNK; j += 4) {
-      const int i = i0 + place(j, true, lane);
-      const float4 v = i < hi ? *(const float4*)(row + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      const float4 v = at + step(j) < hi ? *(const float4*)(row + at + step(j)) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       x[j] = v.x, x[j + 1] = v.y, x[j + 2] = v.z, x[j + 3] = v.w;
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < CHUNK; ++j) {
-      const int i = i0 + place(j, false, lane);
-      x[j] = i < hi ? row[i] : -INFINITY;
-    }
+    for (int j = 0; j < CHUNK; ++j) x[j] = at + step(j) < hi ? row[at + step(j)] : -INFINITY;
   }
 }
 
 // A chunk joins a lane's statistics, in float32: its sum goes by its own maximum so far. A weight is off by 2^-22.5 (ex2.approx) and by
 // four roundings of the exponent t, 4 |t| 2^-24 ln 2 of itself; |t| is log2(V) on average over p, 31 at most (the entropy of p is that
 // average plus log2 of the sum, and at most log2(V)); 16 weights are added in float32, chunks in float64: 6e-6 of the sum in all.
-__device__ __forceinline__ void quick_chunk(const float (&x)[CHUNK], float& top, double& sum, bool& bad, float scale2, double scale, const double* tab) {
+// A NaN makes the sum one, +inf the maximum or the sum.
+__device__ __forceinline__ void quick_chunk(const float (&x)[CHUNK], float& top, double& sum, float scale2, double scale, const double* tab) {
   float m = top;
 #pragma unroll
   for (int j = 0; j < CHUNK; ++j) m = fmaxf(m, x[j]);
   if (m > top) {
-    if (sum != 0.0) sum *= weight(top, Ref{scale, (double)m}, tab);
+    if (sum != 0.0) sum *= weight(top, ref_of(m, scale), tab);
     top = m;
   }
   const float from = top == -INFINITY ? 0.f : top;
   float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < CHUNK; ++j) {
-    bad = bad || !(x[j] <= 3.402823466e38f);      // a NaN, +inf
     float e;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x[j] - from) * scale2));
     part[j & 3] += e;
@@ -131,7 +133,7 @@ __device__ __forceinline__ void quick_chunk(const float (&x)[CHUNK], float& top,
 __device__ __forceinline__ void join_lanes(float& top, double& sum, int width, double scale, const double* tab) {
   float m = top;
   for (int o = width >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  double v = sum == 0.0 ? 0.0 : sum * weight(top, Ref{scale, (double)m}, tab);
+  double v = sum == 0.0 ? 0.0 : sum * weight(top, ref_of(m, scale), tab);
   for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   top = m;
   sum = v;
@@ -233,7 +235,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
         load_chunk(lrow, i0, hi, vec, lane, x);
 #pragma unroll
         for (int j = 0; j < CHUNK; ++j) {
-          const int i = i0 + place(j, vec, lane);
+          const int i = i0 + 4 * lane + step(j);
           if (i < hi && better(x[j], i, bv, bi)) { bv = x[j]; bi = i; }
         }
       }
@@ -264,19 +266,28 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     int x = child >= 0 ? sh.token[child] : 0;
     bool ok = x >= 0 && x < V;
     float lx = ok ? lrow[x] : 0.f, dx = ok && with_q ? drow[x] : 0.f;
+    // few requests: the rows of the node that comes next if the first child stands are brought into L2 meanwhile (where requests are
+    // many their own loads keep the memory busy)
+    if (BLOCKS >= 8 && child >= 0) {
+      const bool inner = draft && next_child(child, child) >= 0;
+      for (int i = lo + 32 * lane; i < hi; i += 32 * 32) {
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(logits + (size_t)(row0 + child) * V + i));
+        if (inner) asm volatile("prefetch.global.L2 [%0];" ::"l"(draft + (size_t)(row0 + child) * V + i));
+      }
+    }
     float top_p = -INFINITY, top_q = -INFINITY;
     double sum_p = 0.0, sum_q = 0.0;
-    bool bad = false, bad_q = false;
     for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
       float a[CHUNK], b[CHUNK];
       load_chunk(lrow, i0, hi, vec, lane, a);
       if (with_q) load_chunk(drow, i0, hi, vec, lane, b);
-      quick_chunk(a, top_p, sum_p, bad, scale2, scale, sh.tab);
-      if (with_q) quick_chunk(b, top_q, sum_q, bad_q, scale2, scale, sh.tab);
+      quick_chunk(a, top_p, sum_p, scale2, scale, sh.tab);
+      if (with_q) quick_chunk(b, top_q, sum_q, scale2, scale, sh.tab);
     }
+    auto is_bad = [](float top, double sum) { return !(top < INFINITY) || !(sum < INFINITY); };      // (a NaN, +inf)
+    const int flags = (int)__reduce_or_sync(0xffffffffu, (is_bad(top_p, sum_p) ? 1u : 0u) | (is_bad(top_q, sum_q) ? 2u : 0u));
     join_lanes(top_p, sum_p, 32, scale, sh.tab);
     join_lanes(top_q, sum_q, 32, scale, sh.tab);
-    const int flags = (int)__reduce_or_sync(0xffffffffu, (bad ? 1u : 0u) | (bad_q ? 2u : 0u));
     if (lane == 0) { sh.top_p[warp] = top_p; sh.sum_p[warp] = sum_p; sh.top_q[warp] = top_q; sh.sum_q[warp] = sum_q; sh.arg[warp] = flags; }
     __syncthreads();
     if (warp == 0) {
@@ -289,7 +300,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     const Slot all = exchange(mine, STATS);
     if ((all.bad & 1) || !(all.sum_p > 0.0)) break;      // a row without a distribution: V - 1
     const bool dead_q = with_q && ((all.bad & 2) || !(all.sum_q > 0.0));      // a drafter's row without one: no child stands, p stays
-    const Ref rp = {scale, (double)all.top_p}, rq = {scale, (double)all.top_q};
+    const Ref rp = ref_of(all.top_p, scale), rq = ref_of(all.top_q, scale);
     double inv_p = 1.0 / all.sum_p, inv_q = with_q && !dead_q ? 1.0 / all.sum_q : 0.0;      // (quick until `exact`)
     double run = 0.0, total = 0.0;      // what the draw goes by: this warp's part of it and the whole
     bool exact = false, plain = true;   // plain: the draw goes by p itself (weights not divided by their sum)
@@ -328,19 +339,24 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
         float a[CHUNK], b[CHUNK];
         load_chunk(lrow, i0, hi, vec, lane, a);
-        if (with_q) load_chunk(drow, i0, hi, vec, lane, b);
+        const int it = gone - i0 - 4 * lane;
+        if (with_q) {
+          load_chunk(drow, i0, hi, vec, lane, b);
 #pragma unroll
-        for (int j = 0; j < CHUNK; ++j) {      // (tokens from hi on weigh 0)
-          const double wp = weight(a[j], rp, sh.tab);
-          if (with_q) {
-            const double wq = weight(b[j], rq, sh.tab), over = fma(a0, wp, -wq);
-            const bool it = i0 + place(j, vec, lane) == gone;
+          for (int j = 0; j < CHUNK; ++j) {      // (tokens from hi on weigh nothing)
+            const double wp = weight(a[j], rp, sh.tab), wq = weight(b[j], rq, sh.tab), over = fma(a0, wp, -wq);
             sp += wp;
-            sq += it ? 0.0 : wq;
-            so += fmax(over, 0.0);
-            su += over > 0.0 ? wp : 0.0;
-          } else {
-            sp += i0 + place(j, vec, lane) == gone ? 0.0 : wp;
+            if (it != step(j)) sq += wq;
+            if (over > 0.0) {
+              so += over;
+              su += wp;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) {
+            const double wp = weight(a[j], rp, sh.tab);
+            if (it != step(j)) sp += wp;
           }
         }
       }
@@ -360,7 +376,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
         left = (sum.over + da * sum.under) / all_q;
         good = left > 1e-6;
         if (good) run = (so + da * su) / all_q / left, total = 1.0, plain = false;
-      } else if (sum.sum_p > 0.0) {
+      } else if (sum.sum_p > NOTHING) {
         left = sum.sum_p / all_p;
         run = sp / sum.sum_p, total = 1.0, plain = false;
       } else {
@@ -373,7 +389,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
         sh.scale_q[0] = inv_q;
       }
       __syncthreads();
-      if (with_q) inv_q = sum.sum_q > 0.0 ? 1.0 / sum.sum_q : 0.0;
+      if (with_q) inv_q = sum.sum_q > NOTHING ? 1.0 / sum.sum_q : 0.0;
       rejected = 1;
       return true;
     };
@@ -388,14 +404,14 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
         load_chunk(lrow, i0, hi, vec, lane, a);
         if (with_q) load_chunk(drow, i0, hi, vec, lane, b);
 #pragma unroll
-        for (int j = 0; j < CHUNK; ++j) {      // (tokens from hi on weigh 0)
+        for (int j = 0; j < CHUNK; ++j) {      // (tokens from hi on weigh nothing)
           double qv;
-          sp += p_after(i0 + place(j, vec, lane), a[j], with_q ? b[j] : 0.f, rejected + 1, qv);
+          sp += p_after(i0 + 4 * lane + step(j), a[j], with_q ? b[j] : 0.f, rejected + 1, qv);
           sq += qv;
         }
       }
       const Slot left = add_up(sp, sq, so, su);
-      if (left.sum_p > 0.0) {
+      if (left.sum_p > NOTHING) {
         total = 1.0;
         plain = false;
         run = sp / left.sum_p;
@@ -405,7 +421,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
         if (!with_q) sh.fallen[rejected] = -1;
       }
       __syncthreads();
-      if (with_q) inv_q = left.sum_q > 0.0 ? 1.0 / left.sum_q : 0.0;
+      if (with_q) inv_q = left.sum_q > NOTHING ? 1.0 / left.sum_q : 0.0;
       ++rejected;
     };
     bool stands = false;
@@ -422,6 +438,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
           px = p_after(x, lx, dx, rejected, base);
           if (with_q) qx = __dmul_rn(base, inv_q);
         }
+        if (px <= NOTHING) px = 0.0;
         const double ux = sh.uniform[child] * qx;
         if (exact || px == 0.0 || fabs(ux - px) > MARGIN * px) {
           if (ux < px) { stands = true; break; }
@@ -464,13 +481,13 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     }
     turn ^= 1;
     // (nothing behind: u so near 1 that the sums' roundings end below the target: the last token that has any probability)
-    if (own_sum > 0.0 && blocks <= target && (blocks + own_sum > target || behind == 0.0)) {
+    if (own_sum > NOTHING && blocks <= target && (blocks + own_sum > target || behind <= NOTHING)) {
       // this block's: the warp whose run holds it, then all threads share that run, a few neighbouring tokens each
       int who = -1;
       double part = 0.0, begin = 0.0;
       for (int w = 0; w < WARPS; ++w) {
         const double end = part + sh.run[w];
-        if (sh.run[w] > 0.0 && blocks + part <= target) { who = w; begin = blocks + part; }      // (the last one that begins at or before it)
+        if (sh.run[w] > NOTHING && blocks + part <= target) { who = w; begin = blocks + part; }      // (the last one that begins at or before it)
         part = end;
       }
       const int from = min(V, (rank * WARPS + who) * per_warp), to = min(V, from + per_warp);
@@ -495,14 +512,14 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       for (int w = 0; w < warp; ++w) ahead += sh.run[w];
       double at = ahead + (upto - mass);
       // the last thread whose tokens begin at or before the target holds it (the very sums that follow decide within it)
-      if (mass > 0.0 && at <= target) atomicMax(&sh.all.arg, tid);
+      if (mass > NOTHING && at <= target) atomicMax(&sh.all.arg, tid);
       __syncthreads();
       if (tid == sh.all.arg) {
         int last = -1, found = -1;
         for (int i = i0; i < i1 && found < 0; ++i) {
           const double v = value(i);
           at += v;
-          if (v > 0.0) {
+          if (v > NOTHING) {
             last = i;
             if (at > target) found = i;
           }
@@ -558,7 +575,7 @@ int launch(const float* logits, const float* draft, const float* temperature, co
 // Blocks per request: as many as the chip holds at once beside the other requests' (14 clusters of eight, 32 of four, 74 of two),
 // each with 2,048 tokens and more.
 FZ_API int fz_verify_blocks(int S, int V) {
-  int b = S <= 6 ? 16 : S <= 14 ? 8 : S <= 32 ? 4 : S <= 74 ? 2 : 1;
+  int b = S <= 8 ? 16 : S <= 14 ? 8 : S <= 32 ? 4 : S <= 74 ? 2 : 1;
   while (b > 1 && V < 2048 * b) b >>= 1;
   return b;
 }

@@ -29,7 +29,7 @@ namespace cg = cooperative_groups;
 namespace {
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int MAX_NODES = 1024;      // nodes of a tree
-constexpr double MARGIN = 3e-5;      // of p(x): a decision nearer than that is taken in float64
+constexpr float MARGIN = 1e-3f;      // of p(x): a decision nearer than that is taken in float64
 
 struct Ref {      // a row's scale: token x weighs exp((x - top) / T)
   double scale, top;      // 256 log2(e) / T, and the row's maximum
@@ -68,18 +68,21 @@ __device__ __forceinline__ double warp_sum_d(double v) {
   return v;
 }
 
-struct Slot {      // what a block tells the others after a pass
-  float top_p, top_q;
+struct alignas(16) Slot {      // what a block tells the others after a pass
   double sum_p, sum_q, over, under;
-  int arg, bad;
+};
+struct alignas(8) Found {     // a node's rows, quick; or the argmax (p.top, arg)
+  float top_p, sum_p, top_q, sum_q;
+  int arg, bad;      // bad: 1 p's row has no distribution, 2 q's
 };
 
 struct Shared {
   double tab[256];
-  Slot slot[2], all;
-  float top_p[WARPS], top_q[WARPS];
+  Slot slot[2], sums;
+  Found found[2], warp_found[WARPS], node_found;
+  int who;
+  double block_run[16];
   double sum_p[WARPS], sum_q[WARPS], over[WARPS], under[WARPS], run[WARPS];
-  int arg[WARPS];
   // the request's tree
   double uniform[MAX_NODES];
   int token[MAX_NODES], parent[MAX_NODES];
@@ -106,44 +109,160 @@ __device__ __forceinline__ void load_chunk(const float* __restrict__ row, int i0
   }
 }
 
-// A chunk joins a lane's statistics, in float32: its sum goes by its own maximum so far. A weight is off by 2^-22.5 (ex2.approx) and by
-// four roundings of the exponent t, 4 |t| 2^-24 ln 2 of itself; |t| is log2(V) on average over p, 31 at most (the entropy of p is that
-// average plus log2 of the sum, and at most log2(V)); 16 weights are added in float32, chunks in float64: 6e-6 of the sum in all.
-// A NaN makes the sum one, +inf the maximum or the sum.
-__device__ __forceinline__ void quick_chunk(const float (&x)[CHUNK], float& top, double& sum, float scale2, double scale, const double* tab) {
-  float m = top;
-#pragma unroll
-  for (int j = 0; j < CHUNK; ++j) m = fmaxf(m, x[j]);
-  if (m > top) {
-    if (sum != 0.0) sum *= weight(top, ref_of(m, scale), tab);
-    top = m;
-  }
-  const float from = top == -INFINITY ? 0.f : top;
-  float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int j = 0; j < CHUNK; ++j) {
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x[j] - from) * scale2));
-    part[j & 3] += e;
-  }
-  sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
+__device__ __forceinline__ float quick_exp2(float t) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return e;
 }
 
-// The lanes' (the first `width` of them; a power of two) maxima and sums as one, in every one of these lanes.
-__device__ __forceinline__ void join_lanes(float& top, double& sum, int width, double scale, const double* tab) {
-  float m = top;
-  for (int o = width >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  double v = sum == 0.0 ? 0.0 : sum * weight(top, ref_of(m, scale), tab);
-  for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  top = m;
-  sum = v;
+// A row's maximum and sum of weights, quick: float32.
+struct Quick { float top, sum; };
+
+// A chunk joins a lane's statistics; its sum goes by its own maximum so far. How far off a sum may be, of itself: a weight 2^-22.5
+// (ex2.approx) and four roundings of the exponent t, 4 |t| 2^-24 ln 2, where |t| is log2(V) on average over p (the entropy of p is that
+// average plus log2 of the sum, and at most log2(V)): 4e-6; a chunk's addition, and its rescaling where the maximum grew, 4e-7 at most,
+// 1,024 chunks (vocabularies of eight million): 4e-4. MARGIN covers both sums. A NaN makes the sum one, +inf the maximum or the sum.
+__device__ __forceinline__ void quick_chunk(const float (&x)[CHUNK], Quick& r, float scale2) {
+  float m = r.top;
+#pragma unroll
+  for (int j = 0; j < CHUNK; ++j) m = fmaxf(m, x[j]);
+  if (m > r.top) {
+    r.sum = r.sum == 0.f ? 0.f : r.sum * quick_exp2((r.top - m) * scale2);
+    r.top = m;
+  }
+  const float from = r.top == -INFINITY ? 0.f : r.top;
+  float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < CHUNK; ++j) part[j & 3] += quick_exp2((x[j] - from) * scale2);
+  r.sum += (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// The statistics of a warp's run of one or two rows, the next chunk's loads under way while one is computed.
+__device__ __forceinline__ void quick_rows(const float* __restrict__ lrow, const float* __restrict__ drow, int lo, int hi, bool vec, int lane, float scale2,
+                                           Quick& p, Quick& q) {
+  float a[CHUNK], b[CHUNK];
+  if (lo < hi) {
+    load_chunk(lrow, lo, hi, vec, lane, a);
+    if (drow) load_chunk(drow, lo, hi, vec, lane, b);
+  }
+  for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
+    float c[CHUNK], d[CHUNK];
+    load_chunk(lrow, i0 + 32 * CHUNK, hi, vec, lane, c);
+    if (drow) load_chunk(drow, i0 + 32 * CHUNK, hi, vec, lane, d);
+    quick_chunk(a, p, scale2);
+    if (drow) quick_chunk(b, q, scale2);
+#pragma unroll
+    for (int j = 0; j < CHUNK; ++j) a[j] = c[j], b[j] = d[j];
+  }
+}
+
+__device__ __forceinline__ bool is_bad(const Quick& r) { return !(r.top < INFINITY) || !(r.sum < INFINITY); }
+
+// The lanes' (the first `width` of them; a power of two) statistics as one, in every one of these lanes.
+__device__ __forceinline__ void join_lanes(Quick& r, int width, float scale2) {
+  float m = r.top;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < width) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float v = r.sum == 0.f ? 0.f : r.sum * quick_exp2((r.top - m) * scale2);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < width) v += __shfl_xor_sync(0xffffffffu, v, o);
+  r = {m, v};
+}
+
+// The quick statistics of all rows ahead of the walks, which then start a node with its rows' sums in hand: a row's slices are evenly
+// spread over the SMs, where walks are as long as they are (see `fz_verify_ahead`). stats: (N, slices). A row is p's and, where its node has
+// children, q's; of a greedy request the argmax of p's alone.
+// One (row, lane < width) each: the joined statistics in every lane.
+__device__ __forceinline__ Found join_found(const Found& mine, bool greedy, int width, float scale2) {
+  Found r = mine;
+  if (greedy) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      if (o >= width) continue;
+      const float v = __shfl_xor_sync(0xffffffffu, r.top_p, o);
+      const int i = __shfl_xor_sync(0xffffffffu, r.arg, o);
+      if (better(v, i, r.top_p, r.arg)) { r.top_p = v; r.arg = i; }
+    }
+  } else {
+    Quick p = {r.top_p, r.sum_p}, q = {r.top_q, r.sum_q};
+    r.bad = (int)__reduce_or_sync(0xffffffffu, (unsigned)r.bad);
+    join_lanes(p, width, scale2);
+    join_lanes(q, width, scale2);
+    r.top_p = p.top, r.sum_p = p.sum, r.top_q = q.top, r.sum_q = q.sum;
+  }
+  return r;
+}
+__device__ __forceinline__ Found nobody() { return {-INFINITY, 0.f, -INFINITY, 0.f, -1, 0}; }
+
+// A warp's run of a node's rows (drow null: p's alone), joined.
+__device__ __forceinline__ Found find_warp(const float* __restrict__ lrow, const float* __restrict__ drow, int lo, int hi, bool vec, int lane, bool greedy,
+                                           float scale2) {
+  Found r = nobody();
+  if (greedy) {
+    for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
+      float x[CHUNK];
+      load_chunk(lrow, i0, hi, vec, lane, x);
+#pragma unroll
+      for (int j = 0; j < CHUNK; ++j) {
+        const int i = i0 + 4 * lane + step(j);
+        if (i < hi && better(x[j], i, r.top_p, r.arg)) { r.top_p = x[j]; r.arg = i; }
+      }
+    }
+  } else {
+    Quick p = {-INFINITY, 0.f}, q = {-INFINITY, 0.f};
+    quick_rows(lrow, drow, lo, hi, vec, lane, scale2, p, q);
+    r = {p.top, p.sum, q.top, q.sum, 0, (is_bad(p) ? 1 : 0) | (is_bad(q) ? 2 : 0)};
+  }
+  return join_found(r, greedy, 32, scale2);
+}
+
+constexpr int AHEAD_THREADS = 256, AHEAD_WARPS = AHEAD_THREADS / 32, MAX_SLICES = 32;
+__global__ void __launch_bounds__(AHEAD_THREADS)
+verify_stats_kernel(const float* __restrict__ logits, const float* __restrict__ draft, const float* __restrict__ temperature,
+                    const int* __restrict__ parents, const int* __restrict__ seg, int S, int N, int V, Found* __restrict__ stats) {
+  __shared__ Found s_found[AHEAD_WARPS];
+  fz_grid_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  fz_grid_wait();
+  const int row = blockIdx.x, slices = gridDim.y;
+  int s = -1, row0 = 0, n = 0;
+  for (int s0 = 0; s0 < S && s < 0; s0 += 32) {
+    const int2 sg = s0 + lane < S ? *(const int2*)(seg + 4 * (s0 + lane)) : make_int2(0, 0);
+    const unsigned hit = __ballot_sync(0xffffffffu, row >= sg.x && row - sg.x < sg.y);
+    if (hit) {
+      const int who = __ffs(hit) - 1;
+      s = s0 + who;
+      row0 = __shfl_sync(0xffffffffu, sg.x, who);
+      n = __shfl_sync(0xffffffffu, sg.y, who);
+    }
+  }
+  if (s < 0 || row0 + n > N || n > MAX_NODES) return;
+  const float T = temperature[s];
+  const bool greedy = !(T > 0.f);
+  bool with_q = false;
+  if (draft && !greedy)
+    for (int j0 = row - row0 + 1; j0 < n && !with_q; j0 += 32) with_q = __any_sync(0xffffffffu, j0 + lane < n && parents[row0 + j0 + lane] == row - row0);
+  const float scale2 = (float)fmin(1.4426950408889634 / (double)T, 3.4e38);
+  const int per_warp = ((V + slices * AHEAD_WARPS - 1) / (slices * AHEAD_WARPS) + 3) & ~3;
+  const int lo = min(V, ((int)blockIdx.y * AHEAD_WARPS + warp) * per_warp), hi = min(V, lo + per_warp);
+  const bool vec = (V & 3) == 0 && (((uintptr_t)logits | (uintptr_t)draft) & 15) == 0;
+  const Found mine = find_warp(logits + (size_t)row * V, with_q ? draft + (size_t)row * V : nullptr, lo, hi, vec, lane, greedy, scale2);
+  if (lane == 0) s_found[warp] = mine;
+  __syncthreads();
+  if (warp == 0) {
+    const Found all = join_found(lane < AHEAD_WARPS ? s_found[lane] : nobody(), greedy, AHEAD_WARPS, scale2);
+    if (lane == 0) stats[(size_t)row * slices + blockIdx.y] = all;
+  }
 }
 
 template <int BLOCKS>
 __global__ void __launch_bounds__(THREADS, 1)
 verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft, const float* __restrict__ temperature,
               const double* __restrict__ uniform, const int* __restrict__ tokens, const int* __restrict__ parents,
-              const int* __restrict__ seg, int N, int V, int* __restrict__ path, int* __restrict__ count, int* __restrict__ next_ids, int* err) {
+              const int* __restrict__ seg, int N, int V, int* __restrict__ path, int* __restrict__ count, int* __restrict__ next_ids,
+              const Found* __restrict__ stats, int slices, int* err) {
   extern __shared__ __align__(16) unsigned char verify_smem[];
   Shared& sh = *(Shared*)verify_smem;
   cg::cluster_group cluster = cg::this_cluster();
@@ -171,33 +290,26 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
   __syncthreads();
   const bool greedy = !(T > 0.f);
   const double scale = 369.3299304675746 / (double)T;      // 256 log2(e) / T
-  const float scale2 = (float)fmin(scale / 256.0, 3.4e38);
+  const float scale2 = (float)fmin(1.4426950408889634 / (double)T, 3.4e38);
   // this warp's run of tokens: [lo, hi), within the block's part of the vocabulary; multiples of four
   const int per_warp = ((V + BLOCKS * WARPS - 1) / (BLOCKS * WARPS) + 3) & ~3;
   const int lo = min(V, (rank * WARPS + warp) * per_warp), hi = min(V, lo + per_warp);
   const bool vec = (V & 3) == 0 && (((uintptr_t)logits | (uintptr_t)draft) & 15) == 0;
   int turn = 0;
-  // Every block leaves its slot; after the barrier all have all of them (the next exchange writes the other slot). The first warp reads
-  // the slots, joins them as the pass asks for, and tells the block. `mine`: thread 0's.
-  enum { ARGMAX, STATS, SUMS };
-  auto exchange = [&](const Slot& mine, int what) -> Slot {
-    if (tid == 0) sh.slot[turn] = mine;
+  // Every block leaves what it found in a slot of its own; after the barrier the first warp of every block reads all of them (loads from
+  // other blocks by all warps would queue: 28 against 16 us for a walk of one request), joins them in the same order everywhere and
+  // tells its block. The next exchange writes the other slot.
+  auto meet = [&] {
     if (BLOCKS > 1) cluster.sync();
-    if (warp == 0) {
-      __syncwarp();
-      Slot r = lane < BLOCKS ? (BLOCKS == 1 ? sh.slot[turn] : *cluster.map_shared_rank(&sh.slot[turn], lane)) : Slot{-INFINITY, -INFINITY, 0.0, 0.0, 0.0, 0.0, -1, 0};
-      if (what == ARGMAX) {
-#pragma unroll
-        for (int o = BLOCKS >> 1; o > 0; o >>= 1) {
-          const float v = __shfl_xor_sync(0xffffffffu, r.top_p, o);
-          const int i = __shfl_xor_sync(0xffffffffu, r.arg, o);
-          if (better(v, i, r.top_p, r.arg)) { r.top_p = v; r.arg = i; }
-        }
-      } else if (what == STATS) {
-        join_lanes(r.top_p, r.sum_p, BLOCKS, scale, sh.tab);
-        join_lanes(r.top_q, r.sum_q, BLOCKS, scale, sh.tab);
-        r.bad = (int)__reduce_or_sync(0xffffffffu, (unsigned)r.bad);
-      } else {
+    else __syncthreads();
+  };
+  auto exchange_sums = [&](const Slot& mine) -> Slot {      // mine: the first warp's
+    if (tid == 0) sh.slot[turn] = mine;
+    if (BLOCKS > 1) {
+      cluster.sync();
+      if (warp == 0) {
+        Slot r = {0.0, 0.0, 0.0, 0.0};
+        if (lane < BLOCKS) r = *cluster.map_shared_rank(&sh.slot[turn], lane);
 #pragma unroll
         for (int o = BLOCKS >> 1; o > 0; o >>= 1) {
           r.sum_p += __shfl_xor_sync(0xffffffffu, r.sum_p, o);
@@ -205,12 +317,14 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
           r.over += __shfl_xor_sync(0xffffffffu, r.over, o);
           r.under += __shfl_xor_sync(0xffffffffu, r.under, o);
         }
+        if (lane == 0) sh.sums = r;
       }
-      if (lane == 0) sh.all = r;
+    } else if (tid == 0) {
+      sh.sums = mine;
     }
-    __syncthreads();
     turn ^= 1;
-    return sh.all;
+    __syncthreads();
+    return sh.sums;
   };
   auto next_child = [&](int node, int after) {      // the node's next child behind `after`, or -1
     for (int j0 = after + 1; j0 < n; j0 += 32) {
@@ -226,34 +340,49 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     const float* lrow = logits + (size_t)(row0 + node) * V;
     const float* drow = draft ? draft + (size_t)(row0 + node) * V : nullptr;
     int child = next_child(node, node);
-    Slot mine = {-INFINITY, -INFINITY, 0.0, 0.0, 0.0, 0.0, -1, 0};
-    if (greedy) {
-      float bv = -INFINITY;
-      int bi = -1;
-      for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
-        float x[CHUNK];
-        load_chunk(lrow, i0, hi, vec, lane, x);
-#pragma unroll
-        for (int j = 0; j < CHUNK; ++j) {
-          const int i = i0 + 4 * lane + step(j);
-          if (i < hi && better(x[j], i, bv, bi)) { bv = x[j]; bi = i; }
+    // the drafter's row only where there is a child to try; the first child's own values on their way meanwhile
+    const bool with_q = drow && child >= 0 && !greedy;
+    int x = child >= 0 ? sh.token[child] : 0;
+    bool ok = x >= 0 && x < V;
+    float lx = ok ? lrow[x] : 0.f, dx = ok && with_q ? drow[x] : 0.f;
+    Found all = nobody();
+    if (stats) {
+      if (lane < slices) all = stats[(size_t)(row0 + node) * slices + lane];
+      all = join_found(all, greedy, 32, scale2);
+    } else {
+      // few requests: the rows of the node that comes next if the first child stands are brought into L2 meanwhile (where requests are
+      // many their own loads keep the memory busy)
+      if (BLOCKS >= 8 && child >= 0) {
+        const bool inner = draft && !greedy && next_child(child, child) >= 0;
+        for (int i = lo + 32 * lane; i < hi; i += 32 * 32) {
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(logits + (size_t)(row0 + child) * V + i));
+          if (inner) asm volatile("prefetch.global.L2 [%0];" ::"l"(draft + (size_t)(row0 + child) * V + i));
         }
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-        const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-        if (better(ov, oi, bv, bi)) { bv = ov; bi = oi; }
-      }
-      if (lane == 0) { sh.top_p[warp] = bv; sh.arg[warp] = bi; }
+      const Found mine = find_warp(lrow, with_q ? drow : nullptr, lo, hi, vec, lane, greedy, scale2);
+      if (lane == 0) sh.warp_found[warp] = mine;
       __syncthreads();
-      if (tid == 0)
-        for (int w = 0; w < WARPS; ++w)
-          if (better(sh.top_p[w], sh.arg[w], mine.top_p, mine.arg)) { mine.top_p = sh.top_p[w]; mine.arg = sh.arg[w]; }
-      const int best = exchange(mine, ARGMAX).arg;
-      while (child >= 0 && sh.token[child] != best) child = next_child(node, child);
+      if (warp == 0) {
+        Found r = join_found(lane < WARPS ? sh.warp_found[lane] : nobody(), greedy, WARPS, scale2);
+        if (lane == 0) (BLOCKS > 1 ? sh.found[turn] : sh.node_found) = r;
+      }
+      if (BLOCKS > 1) {
+        cluster.sync();
+        if (warp == 0) {
+          Found r = nobody();
+          if (lane < BLOCKS) r = *cluster.map_shared_rank(&sh.found[turn], lane);
+          r = join_found(r, greedy, BLOCKS, scale2);
+          if (lane == 0) sh.node_found = r;
+        }
+        turn ^= 1;
+      }
+      __syncthreads();
+      all = sh.node_found;
+    }
+    if (greedy) {
+      while (child >= 0 && sh.token[child] != all.arg) child = next_child(node, child);
       if (child < 0) {
-        result = best;
+        result = all.arg;
         break;
       }
       node = child;
@@ -261,47 +390,11 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       ++kept;
       continue;
     }
-    // statistics of the node's rows (the drafter's only where there is a child to try); the first child's own values on their way meanwhile
-    const bool with_q = drow && child >= 0;
-    int x = child >= 0 ? sh.token[child] : 0;
-    bool ok = x >= 0 && x < V;
-    float lx = ok ? lrow[x] : 0.f, dx = ok && with_q ? drow[x] : 0.f;
-    // few requests: the rows of the node that comes next if the first child stands are brought into L2 meanwhile (where requests are
-    // many their own loads keep the memory busy)
-    if (BLOCKS >= 8 && child >= 0) {
-      const bool inner = draft && next_child(child, child) >= 0;
-      for (int i = lo + 32 * lane; i < hi; i += 32 * 32) {
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(logits + (size_t)(row0 + child) * V + i));
-        if (inner) asm volatile("prefetch.global.L2 [%0];" ::"l"(draft + (size_t)(row0 + child) * V + i));
-      }
-    }
-    float top_p = -INFINITY, top_q = -INFINITY;
-    double sum_p = 0.0, sum_q = 0.0;
-    for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
-      float a[CHUNK], b[CHUNK];
-      load_chunk(lrow, i0, hi, vec, lane, a);
-      if (with_q) load_chunk(drow, i0, hi, vec, lane, b);
-      quick_chunk(a, top_p, sum_p, scale2, scale, sh.tab);
-      if (with_q) quick_chunk(b, top_q, sum_q, scale2, scale, sh.tab);
-    }
-    auto is_bad = [](float top, double sum) { return !(top < INFINITY) || !(sum < INFINITY); };      // (a NaN, +inf)
-    const int flags = (int)__reduce_or_sync(0xffffffffu, (is_bad(top_p, sum_p) ? 1u : 0u) | (is_bad(top_q, sum_q) ? 2u : 0u));
-    join_lanes(top_p, sum_p, 32, scale, sh.tab);
-    join_lanes(top_q, sum_q, 32, scale, sh.tab);
-    if (lane == 0) { sh.top_p[warp] = top_p; sh.sum_p[warp] = sum_p; sh.top_q[warp] = top_q; sh.sum_q[warp] = sum_q; sh.arg[warp] = flags; }
-    __syncthreads();
-    if (warp == 0) {
-      float a = lane < WARPS ? sh.top_p[lane] : -INFINITY, b = lane < WARPS ? sh.top_q[lane] : -INFINITY;
-      double u = lane < WARPS ? sh.sum_p[lane] : 0.0, v = lane < WARPS ? sh.sum_q[lane] : 0.0;
-      join_lanes(a, u, WARPS, scale, sh.tab);
-      join_lanes(b, v, WARPS, scale, sh.tab);
-      mine = {a, b, u, v, 0.0, 0.0, 0, (int)__reduce_or_sync(0xffffffffu, lane < WARPS ? (unsigned)sh.arg[lane] : 0u)};
-    }
-    const Slot all = exchange(mine, STATS);
-    if ((all.bad & 1) || !(all.sum_p > 0.0)) break;      // a row without a distribution: V - 1
-    const bool dead_q = with_q && ((all.bad & 2) || !(all.sum_q > 0.0));      // a drafter's row without one: no child stands, p stays
+    if ((all.bad & 1) || !(all.sum_p > 0.f)) break;      // a row without a distribution: V - 1
+    const bool dead_q = with_q && ((all.bad & 2) || !(all.sum_q > 0.f));      // a drafter's row without one: no child stands, p stays
     const Ref rp = ref_of(all.top_p, scale), rq = ref_of(all.top_q, scale);
-    double inv_p = 1.0 / all.sum_p, inv_q = with_q && !dead_q ? 1.0 / all.sum_q : 0.0;      // (quick until `exact`)
+    const float near_p = 1.f / all.sum_p, near_q = with_q && !dead_q ? 1.f / all.sum_q : 0.f;      // quick
+    double inv_p = 0.0, inv_q = 0.0;      // exact
     double run = 0.0, total = 0.0;      // what the draw goes by: this warp's part of it and the whole
     bool exact = false, plain = true;   // plain: the draw goes by p itself (weights not divided by their sum)
     int rejected = 0;
@@ -320,6 +413,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     };
     // one exchange of four sums over all tokens; the warp's own stay in sp, sq, so, su
     auto add_up = [&](double& sp, double& sq, double& so, double& su) {
+      Slot mine = {0.0, 0.0, 0.0, 0.0};
       sp = warp_sum_d(sp), sq = warp_sum_d(sq), so = warp_sum_d(so), su = warp_sum_d(su);
       if (lane == 0) { sh.sum_p[warp] = sp; sh.sum_q[warp] = sq; sh.over[warp] = so; sh.under[warp] = su; }
       __syncthreads();
@@ -327,14 +421,14 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
         const bool in = lane < WARPS;
         double u = in ? sh.sum_p[lane] : 0.0, v = in ? sh.sum_q[lane] : 0.0, w = in ? sh.over[lane] : 0.0, z = in ? sh.under[lane] : 0.0;
         u = warp_sum_d(u), v = warp_sum_d(v), w = warp_sum_d(w), z = warp_sum_d(z);
-        mine = {0.f, 0.f, u, v, w, z, 0, 0};
+        mine = {u, v, w, z};
       }
-      return exchange(mine, SUMS);
+      return exchange_sums(mine);
     };
     // The first pass in float64: exact sums, and if a child x has fallen (x = -1: none) the sums of p and q after it. Returns false where
     // the sum of max(p - q, 0) came out too small to be had this way (p and q nearly the same).
     auto first_pass = [&](int gone, float lg, float dg, bool fell) -> bool {
-      const double a0 = with_q ? inv_p / inv_q : 0.0;
+      const double a0 = with_q ? (double)near_p / (double)near_q : 0.0;
       double sp = 0.0, sq = 0.0, so = 0.0, su = 0.0;
       for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
         float a[CHUNK], b[CHUNK];
@@ -433,15 +527,22 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
         if (exact) break;      // (the draw's sums are there)
       } else {
         if (!ok && first) atomicOr(err, FZ_ERR_TOKEN_RANGE);
-        double qx = 1.0, px = 0.0, base;
-        if (ok) {
-          px = p_after(x, lx, dx, rejected, base);
-          if (with_q) qx = __dmul_rn(base, inv_q);
+        bool sure = true, yes;
+        if (!exact && ok) {      // from the quick sums
+          const float px = quick_exp2((lx - all.top_p) * scale2) * near_p, qx = with_q ? quick_exp2((dx - all.top_q) * scale2) * near_q : 1.f;
+          const float ux = (float)sh.uniform[child] * qx;
+          sure = lx == -INFINITY || (px > 1e-30f && fabsf(ux - px) > MARGIN * px);
+          yes = ux < px;
+        } else {
+          double qx = 1.0, px = 0.0, base;
+          if (ok) {
+            px = p_after(x, lx, dx, rejected, base);
+            if (with_q) qx = __dmul_rn(base, inv_q);
+          }
+          yes = sh.uniform[child] * qx < (px > NOTHING ? px : 0.0);
         }
-        if (px <= NOTHING) px = 0.0;
-        const double ux = sh.uniform[child] * qx;
-        if (exact || px == 0.0 || fabs(ux - px) > MARGIN * px) {
-          if (ux < px) { stands = true; break; }
+        if (sure) {
+          if (yes) { stands = true; break; }
           todo = exact ? FALL_NEXT : FALL_FIRST;
           if (ok) gone = x, lg = lx, dg = dx;
           child = next_child(node, child);      // (the next child's own values on their way meanwhile)
@@ -466,15 +567,16 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     if (lane == 0) sh.run[warp] = run;
     __syncthreads();
     if (tid == 0) {
-      mine = {0.f, 0.f, 0.0, 0.0, 0.0, 0.0, 0, 0};
-      for (int w = 0; w < WARPS; ++w) mine.sum_p += sh.run[w];
-      sh.slot[turn] = mine;
+      double sum = 0.0;
+      for (int w = 0; w < WARPS; ++w) sum += sh.run[w];
+      sh.slot[turn].sum_p = sum;
     }
-    if (BLOCKS == 1) __syncthreads();
-    else cluster.sync();
+    meet();
+    if (tid < BLOCKS) sh.block_run[tid] = BLOCKS == 1 ? sh.slot[turn].sum_p : cluster.map_shared_rank(&sh.slot[turn], tid)->sum_p;
+    __syncthreads();
     double blocks = 0.0, behind = 0.0, own_sum = 0.0;
     for (int b = 0; b < BLOCKS; ++b) {
-      const double sum = BLOCKS == 1 ? sh.slot[turn].sum_p : cluster.map_shared_rank(&sh.slot[turn], b)->sum_p;
+      const double sum = sh.block_run[b];
       if (b < rank) blocks += sum;
       else if (b > rank) behind += sum;
       else own_sum = sum;
@@ -506,15 +608,15 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       }
       __syncthreads();      // (the runs have been read)
       if (lane == 31) sh.run[warp] = upto;
-      if (tid == 0) sh.all.arg = -1;
+      if (tid == 0) sh.who = -1;
       __syncthreads();
       double ahead = begin;
       for (int w = 0; w < warp; ++w) ahead += sh.run[w];
       double at = ahead + (upto - mass);
       // the last thread whose tokens begin at or before the target holds it (the very sums that follow decide within it)
-      if (mass > NOTHING && at <= target) atomicMax(&sh.all.arg, tid);
+      if (mass > NOTHING && at <= target) atomicMax(&sh.who, tid);
       __syncthreads();
-      if (tid == sh.all.arg) {
+      if (tid == sh.who) {
         int last = -1, found = -1;
         for (int i = i0; i < i1 && found < 0; ++i) {
           const double v = value(i);
@@ -541,7 +643,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
 
 template <int BLOCKS>
 int launch(const float* logits, const float* draft, const float* temperature, const double* uniform, const int* tokens, const int* parents,
-           const int* seg, int S, int N, int V, int* path, int* count, int* next_ids, int* err, cudaStream_t stream) {
+           const int* seg, int S, int N, int V, int* path, int* count, int* next_ids, const Found* stats, int slices, int* err, cudaStream_t stream) {
   auto kern = verify_kernel<BLOCKS>;
   FZ_RAISE_SMEM(kern);
   if (BLOCKS > 8) {
@@ -567,7 +669,7 @@ int launch(const float* logits, const float* draft, const float* temperature, co
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, logits, draft, temperature, uniform, tokens, parents, seg, N, V, path, count, next_ids, err);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, logits, draft, temperature, uniform, tokens, parents, seg, N, V, path, count, next_ids, stats, slices, err);
   return e == cudaSuccess ? FZ_OK : (int)e;
 }
 }  // namespace
@@ -575,21 +677,40 @@ int launch(const float* logits, const float* draft, const float* temperature, co
 // Blocks per request: as many as the chip holds at once beside the other requests' (14 clusters of eight, 32 of four, 74 of two),
 // each with 2,048 tokens and more.
 FZ_API int fz_verify_blocks(int S, int V) {
+  if (const char* v = getenv("FZ_VB")) return atoi(v);
   int b = S <= 8 ? 16 : S <= 14 ? 8 : S <= 32 ? 4 : S <= 74 ? 2 : 1;
   while (b > 1 && V < 2048 * b) b >>= 1;
   return b;
 }
 
+// Slices of a row whose quick statistics a kernel of its own takes ahead of the walks (0: none; the scratch: N * slices * 24 bytes).
+FZ_API int fz_verify_ahead(int S, int N, int V) {
+  if (const char* v = getenv("FZ_VA")) { if (v[0] == '0') return 0; }
+  int slices = (8 * 148 + N - 1) / N;
+  if (slices > MAX_SLICES) slices = MAX_SLICES;
+  while (slices > 1 && V < 4096 * slices) --slices;
+  return slices;
+}
+
 // logits, draft (or null): (N, V) float32; temperature (S,); uniform (N,) in [0, 1): a child's own, the root's for the draw;
 // tokens, parents (N,): a node's parent within its request's rows (the root, node 0: -1); seg (S, 4) = (first row, rows, ..);
-// path (N,): the kept nodes of every request from its first row on, then -1; count (S,); next_ids (S,).
+// path (N,): the kept nodes of every request from its first row on, then -1; count (S,); next_ids (S,). scratch: as `fz_verify_ahead`
+// says, 8-byte aligned.
 FZ_API int fz_verify_tree(const float* logits, const float* draft, const float* temperature, const double* uniform, const int* tokens,
-                          const int* parents, const int* seg, int S, int N, int V, int* path, int* count, int* next_ids, int* err,
-                          cudaStream_t stream) {
+                          const int* parents, const int* seg, int S, int N, int V, int* path, int* count, int* next_ids, void* scratch, int slices,
+                          int* err, cudaStream_t stream) {
+  static_assert(sizeof(Found) == 24, "what callers size the scratch by");
   if (S <= 0) return FZ_OK;
-  if (V <= 0 || N < 0) return FZ_BAD_SHAPE;
+  if (V <= 0 || N < 0 || slices < 0 || slices > MAX_SLICES || (slices > 0 && !scratch)) return FZ_BAD_SHAPE;
+  if ((uintptr_t)scratch & 7 || (uintptr_t)seg & 15) return FZ_BAD_ALIGNMENT;
   if ((long long)S * 16 > 2147483647LL) return FZ_TOO_LARGE;
-#define FZ_V(B_) return launch<B_>(logits, draft, temperature, uniform, tokens, parents, seg, S, N, V, path, count, next_ids, err, stream)
+  Found* stats = slices > 0 ? (Found*)scratch : nullptr;
+  if (stats && N > 0) {
+    const cudaError_t e = fz_launch(verify_stats_kernel, dim3((unsigned)N, (unsigned)slices), dim3(AHEAD_THREADS), 0, stream, logits, draft, temperature,
+                                    parents, seg, S, N, V, stats);
+    if (e != cudaSuccess) return (int)e;
+  }
+#define FZ_V(B_) return launch<B_>(logits, draft, temperature, uniform, tokens, parents, seg, S, N, V, path, count, next_ids, stats, slices, err, stream)
   switch (fz_verify_blocks(S, V)) {
     case 16: FZ_V(16);
     case 8: FZ_V(8);

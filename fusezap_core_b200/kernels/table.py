@@ -890,9 +890,11 @@ class CudaOps(Ops):
             raise KernelError("verify_tree: the vocabulary is empty")
         if segments == 0:
             return
+        slices = self.drafts.fz_verify_ahead(segments, n, vocab)
+        stats = torch.empty(n * slices * 24, dtype=torch.uint8, device=self.device) if slices else None
         self._launch(self.drafts.fz_verify_tree, "verify_tree",
                      (_p(logits), _p(draft), _p(temperature), _p(uniform), _p(tokens), _p(parents), _p(seg), segments, n, vocab, _p(path),
-                      _p(count), _p(next_ids), _p(self.err)))
+                      _p(count), _p(next_ids), _p(stats), slices, _p(self.err)), kernels=2 if slices else 1)
 
     def _group_pool(self, pool) -> tuple[int, int, int, int, int]:
         """(slots, pages, parts, page size, bytes of a row) of a cache group's pool (see `KVNeed.pool_shape`, `LatentNeed.pool_shape`)."""

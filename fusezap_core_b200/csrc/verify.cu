@@ -19,7 +19,7 @@
 //   next    float64, for every further sibling that falls: the sums of the new p and q.
 // Sums are kept per warp, whose tokens are one run each, so the last pass before the draw already says in whose run the drawn token
 // lies: its block's threads walk that run again, a few neighbouring tokens each. A draw's place among 100,000 running sums needs more
-// than 32 bits: exp in float64 by a table of 2^(j/256) and a Taylor polynomial (the table-driven method of P. T. P. Tang, 1989).
+// than 32 bits.
 #include "common.cuh"
 #include <cooperative_groups.h>
 #include <math.h>
@@ -32,25 +32,29 @@ constexpr int MAX_NODES = 1024;      // nodes of a tree
 constexpr float MARGIN = 1e-3f;      // of p(x): a decision nearer than that is taken in float64
 
 struct Ref {      // a row's scale: token x weighs exp((x - top) / T)
-  double scale, top;      // 256 log2(e) / T, and the row's maximum
+  double scale, top;      // 128 log2(e) / T, and the row's maximum
   float cut;              // tokens below it weigh as much as it: NOTHING at most
 };
 constexpr double NOTHING = 1e-290;      // weights and probabilities up to this count as 0
-// (2^-1015 is 260,000 / 256 powers of two below 1; -inf must not reach the subtraction)
-__device__ __forceinline__ Ref ref_of(float top, double scale) {
-  return {scale, (double)top, (float)fmax((double)top - 260000.0 / scale, -3.0e38)};
-}
+// reach: how far below the maximum a token weighs 2^-1015 (-inf must not reach the subtraction)
+__device__ __forceinline__ Ref ref_of(float top, double scale, double reach) { return {scale, (double)top, (float)fmax((double)top - reach, -3.0e38)}; }
 
-// The token's weight, tab[j] = 2^(j / 256); 1 for x = top exactly. A row that holds a NaN or +inf is not asked for. Here and where p
-// and q are made from weights the roundings are written out: every place that needs a token's p gets the same bits.
+// The token's weight; 1 for x = top exactly, else off by 3e-12 of itself at most. t = 128 log2 of it, k = t rounded, f = t - k, 2^(t / 128) =
+// 2^(k / 128 div 128) * table[k mod 128] * 2^(f / 128), the last by a Taylor polynomial (the table-driven method of P. T. P. Tang, 1989).
+// tab: this lane's copy of the table, of which shared memory holds sixteen side by side: the lanes of half a warp, whose k are
+// anything, then never meet in a bank (with one copy the reads took as long as the rest: 28 us for 76,000 token pairs of an SM). A
+// row that holds a NaN or +inf is not asked for. Here and where p and q are made from weights the roundings are written out: every place that
+// needs a token's p gets the same bits.
+constexpr int TABLE = 128, COPIES = 16;
 __device__ __forceinline__ double weight(float x, const Ref& r, const double* tab) {
-  const double t = __dmul_rn(__dadd_rn((double)fmaxf(x, r.cut), -r.top), r.scale);      // 256 log2 of the weight
-  const double big = 6755399441055744.0;                                  // 1.5 * 2^52: the low bits of the sum are the nearest whole number
-  const double shifted = __dadd_rn(t, big), f = __dadd_rn(t, -__dadd_rn(shifted, -big));
+  const double d = __dadd_rn((double)fmaxf(x, r.cut), -r.top);
+  const double big = 6755399441055744.0;                  // 1.5 * 2^52: the low bits of the sum are the nearest whole number
+  const double shifted = __fma_rn(d, r.scale, big);
+  const double f = __fma_rn(d, r.scale, -__dadd_rn(shifted, -big));
   const int k = __double2loint(shifted);
-  constexpr double c1 = 0.0027076061740622863, c2 = 3.6655655969101062e-06, c3 = 3.3083026805413713e-09;      // (ln 2 / 256)^i / i!
-  const double e = __dmul_rn(tab[k & 255], fma(f, fma(f, fma(f, c3, c2), c1), 1.0));
-  return __hiloint2double(__double2hiint(e) + (k & ~255) * 4096, __double2loint(e));
+  constexpr double c1 = 0.0054152123481245725, c2 = 1.4662262387640425e-05, c3 = 2.646642144433097e-08;      // (ln 2 / 128)^i / i!
+  const double e = __dmul_rn(tab[(k & (TABLE - 1)) * COPIES], __fma_rn(f, __fma_rn(f, __fma_rn(f, c3, c2), c1), 1.0));
+  return __hiloint2double(__double2hiint(e) + (k & ~(TABLE - 1)) * (1048576 / TABLE), __double2loint(e));
 }
 
 __device__ __forceinline__ bool better(float v, int i, float bv, int bi) {      // numpy.argmax: a NaN is the maximum, then the lower index
@@ -74,21 +78,6 @@ struct alignas(16) Slot {      // what a block tells the others after a pass
 struct alignas(8) Found {     // a node's rows, quick; or the argmax (p.top, arg)
   float top_p, sum_p, top_q, sum_q;
   int arg, bad;      // bad: 1 p's row has no distribution, 2 q's
-};
-
-struct Shared {
-  double tab[256];
-  Slot slot[2], sums;
-  Found found[2], warp_found[WARPS], node_found;
-  int who;
-  double block_run[16];
-  double sum_p[WARPS], sum_q[WARPS], over[WARPS], under[WARPS], run[WARPS];
-  // the request's tree
-  double uniform[MAX_NODES];
-  int token[MAX_NODES], parent[MAX_NODES];
-  // the rejected siblings at the node: token, 1 / sum of p after it, 1 / sum of q before it
-  double scale_p[MAX_NODES], scale_q[MAX_NODES];
-  int fallen[MAX_NODES];
 };
 
 constexpr int CHUNK = 16;      // tokens of a row that a lane has in registers at a time
@@ -137,22 +126,15 @@ __device__ __forceinline__ void quick_chunk(const float (&x)[CHUNK], Quick& r, f
   r.sum += (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// The statistics of a warp's run of one or two rows, the next chunk's loads under way while one is computed.
+// The statistics of a warp's run of one or two rows.
 __device__ __forceinline__ void quick_rows(const float* __restrict__ lrow, const float* __restrict__ drow, int lo, int hi, bool vec, int lane, float scale2,
                                            Quick& p, Quick& q) {
-  float a[CHUNK], b[CHUNK];
-  if (lo < hi) {
-    load_chunk(lrow, lo, hi, vec, lane, a);
-    if (drow) load_chunk(drow, lo, hi, vec, lane, b);
-  }
   for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
-    float c[CHUNK], d[CHUNK];
-    load_chunk(lrow, i0 + 32 * CHUNK, hi, vec, lane, c);
-    if (drow) load_chunk(drow, i0 + 32 * CHUNK, hi, vec, lane, d);
+    float a[CHUNK], b[CHUNK];
+    load_chunk(lrow, i0, hi, vec, lane, a);
+    if (drow) load_chunk(drow, i0, hi, vec, lane, b);
     quick_chunk(a, p, scale2);
     if (drow) quick_chunk(b, q, scale2);
-#pragma unroll
-    for (int j = 0; j < CHUNK; ++j) a[j] = c[j], b[j] = d[j];
   }
 }
 
@@ -218,6 +200,91 @@ __device__ __forceinline__ Found find_warp(const float* __restrict__ lrow, const
   return join_found(r, greedy, 32, scale2);
 }
 
+// A warp's part of the first exact pass: of p's weights (without token `gone`'s where there is no drafter), q's without it, max(a0 p - q,
+// 0), and the p for which that is not 0.
+struct Part { double sum_p, sum_q, over, under; };
+__device__ __noinline__ Part first_sums(const float* __restrict__ lrow, const float* __restrict__ drow, int lo, int hi, bool vec, int lane, const Ref& rp_,
+                                        const Ref& rq_, const double* tab, double a0, int gone) {
+  const Ref rp = rp_, rq = rq_;
+  double sp = 0.0, sq = 0.0, so = 0.0, su = 0.0;
+  for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
+    float a[CHUNK], b[CHUNK];
+    load_chunk(lrow, i0, hi, vec, lane, a);
+    const int it = gone - i0 - 4 * lane;
+    if (drow) {
+      load_chunk(drow, i0, hi, vec, lane, b);
+#pragma unroll
+      for (int j = 0; j < CHUNK; ++j) {      // (tokens from hi on weigh nothing)
+        const double wp = weight(a[j], rp, tab), wq = weight(b[j], rq, tab), over = fma(a0, wp, -wq);
+        sp += wp;
+        if (it != step(j)) sq += wq;
+        if (__double2hiint(over) >= 0) {      // (the sign bit)
+          so += over;
+          su += wp;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < CHUNK; ++j) {
+        const double wp = weight(a[j], rp, tab);
+        if (it != step(j)) sp += wp;
+      }
+    }
+  }
+  return {warp_sum_d(sp), warp_sum_d(sq), warp_sum_d(so), warp_sum_d(su)};
+}
+
+// A child that has fallen: its token, 1 / the sum of p after it, 1 / the sum of q before it.
+struct Fallen { double scale_p, scale_q; int token; };
+
+// A warp's part of a further pass: p and q after `rejected` children, `p_after` below for four tokens side by side.
+__device__ __noinline__ Part next_sums(const float* __restrict__ lrow, const float* __restrict__ drow, int lo, int hi, bool vec, int lane, const Ref& rp_,
+                                       const Ref& rq_, const double* tab, double inv_p, const Fallen* fallen, int rejected) {
+  const Ref rp = rp_, rq = rq_;
+  double sp = 0.0, sq = 0.0;
+  for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
+    float a[CHUNK], b[CHUNK];
+    load_chunk(lrow, i0, hi, vec, lane, a);
+    if (drow) load_chunk(drow, i0, hi, vec, lane, b);
+#pragma unroll
+    for (int j0 = 0; j0 < CHUNK; j0 += 4) {
+      double pv[4], qv[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        pv[j] = __dmul_rn(weight(a[j0 + j], rp, tab), inv_p);
+        qv[j] = drow ? weight(b[j0 + j], rq, tab) : 0.0;
+      }
+      for (int k = 0; k < rejected; ++k) {
+        const int it = fallen[k].token - i0 - 4 * lane;
+        const double kp = fallen[k].scale_p, kq = fallen[k].scale_q;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool here = it == step(j0 + j);
+          const double qk = drow ? __dmul_rn(qv[j], kq) : here ? 1.0 : 0.0;
+          pv[j] = __dmul_rn(fmax(__dadd_rn(pv[j], -qk), 0.0), kp);
+          if (here) qv[j] = 0.0;
+        }
+      }
+      sp += (pv[0] + pv[1]) + (pv[2] + pv[3]);
+      sq += (qv[0] + qv[1]) + (qv[2] + qv[3]);
+    }
+  }
+  return {warp_sum_d(sp), warp_sum_d(sq), 0.0, 0.0};
+}
+
+struct Shared {
+  double tab[TABLE * COPIES];
+  Slot slot[2], block[16], sums;
+  Found found[2], warp_found[WARPS], node_found;
+  int who;
+  Part part[WARPS];
+  double run[WARPS], warp_begin[WARPS + 1], block_begin[17];
+  // the request's tree
+  double uniform[MAX_NODES];
+  int token[MAX_NODES], parent[MAX_NODES];
+  Fallen fallen[MAX_NODES];      // the node's children that have fallen
+};
+
 constexpr int AHEAD_THREADS = 256, AHEAD_WARPS = AHEAD_THREADS / 32, MAX_SLICES = 32;
 __global__ void __launch_bounds__(AHEAD_THREADS)
 verify_stats_kernel(const float* __restrict__ logits, const float* __restrict__ draft, const float* __restrict__ temperature,
@@ -269,7 +336,11 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
   fz_grid_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int s = blockIdx.x / BLOCKS, rank = blockIdx.x % BLOCKS;
-  if (tid < 256) sh.tab[tid] = exp2((double)tid / 256.0);
+  if (tid < TABLE) {
+    const double v = exp2((double)tid / TABLE);
+    for (int c = 0; c < COPIES; ++c) sh.tab[tid * COPIES + c] = v;
+  }
+  const double* tab = sh.tab + lane % COPIES;
   fz_grid_wait();
   const int row0 = seg[4 * s], n = seg[4 * s + 1];
   const float T = temperature[s];
@@ -289,7 +360,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
   }
   __syncthreads();
   const bool greedy = !(T > 0.f);
-  const double scale = 369.3299304675746 / (double)T;      // 256 log2(e) / T
+  const double scale = 184.6649652337873 / (double)T, reach = (1015.0 * 0.6931471805599453) * (double)T;      // 128 log2(e) / T
   const float scale2 = (float)fmin(1.4426950408889634 / (double)T, 3.4e38);
   // this warp's run of tokens: [lo, hi), within the block's part of the vocabulary; multiples of four
   const int per_warp = ((V + BLOCKS * WARPS - 1) / (BLOCKS * WARPS) + 3) & ~3;
@@ -299,17 +370,13 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
   // Every block leaves what it found in a slot of its own; after the barrier the first warp of every block reads all of them (loads from
   // other blocks by all warps would queue: 28 against 16 us for a walk of one request), joins them in the same order everywhere and
   // tells its block. The next exchange writes the other slot.
-  auto meet = [&] {
-    if (BLOCKS > 1) cluster.sync();
-    else __syncthreads();
-  };
   auto exchange_sums = [&](const Slot& mine) -> Slot {      // mine: the first warp's
     if (tid == 0) sh.slot[turn] = mine;
     if (BLOCKS > 1) {
       cluster.sync();
       if (warp == 0) {
         Slot r = {0.0, 0.0, 0.0, 0.0};
-        if (lane < BLOCKS) r = *cluster.map_shared_rank(&sh.slot[turn], lane);
+        if (lane < BLOCKS) sh.block[lane] = r = *cluster.map_shared_rank(&sh.slot[turn], lane);
 #pragma unroll
         for (int o = BLOCKS >> 1; o > 0; o >>= 1) {
           r.sum_p += __shfl_xor_sync(0xffffffffu, r.sum_p, o);
@@ -320,7 +387,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
         if (lane == 0) sh.sums = r;
       }
     } else if (tid == 0) {
-      sh.sums = mine;
+      sh.block[0] = sh.sums = mine;
     }
     turn ^= 1;
     __syncthreads();
@@ -392,36 +459,36 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     }
     if ((all.bad & 1) || !(all.sum_p > 0.f)) break;      // a row without a distribution: V - 1
     const bool dead_q = with_q && ((all.bad & 2) || !(all.sum_q > 0.f));      // a drafter's row without one: no child stands, p stays
-    const Ref rp = ref_of(all.top_p, scale), rq = ref_of(all.top_q, scale);
+    const Ref rp = ref_of(all.top_p, scale, reach), rq = ref_of(all.top_q, scale, reach);
     const float near_p = 1.f / all.sum_p, near_q = with_q && !dead_q ? 1.f / all.sum_q : 0.f;      // quick
     double inv_p = 0.0, inv_q = 0.0;      // exact
-    double run = 0.0, total = 0.0;      // what the draw goes by: this warp's part of it and the whole
-    bool exact = false, plain = true;   // plain: the draw goes by p itself (weights not divided by their sum)
+    // what the draw goes by: a warp's or block's part is (sum_p or over + shift * under) * unit of its sums, the whole 1 or all of p
+    double total = 0.0, shift = 0.0, unit = 1.0;
+    double own_p = 0.0, own_over = 0.0, own_under = 0.0;
+    bool exact = false, stale = false;  // stale: the last pass's sums are not the draw's
+    bool by_over = false, plain = true;   // plain: the draw goes by p itself (weights not divided by their sum)
     int rejected = 0;
     // p of a token after `r` rejections, and its q before it is divided by its sum
     auto p_after = [&](int i, float l, float d, int r, double& qv) {
-      double pv = __dmul_rn(weight(l, rp, sh.tab), inv_p);
-      double base = with_q ? weight(d, rq, sh.tab) : 0.0;
+      double pv = __dmul_rn(weight(l, rp, tab), inv_p);
+      double base = with_q ? weight(d, rq, tab) : 0.0;
       for (int k = 0; k < r; ++k) {
-        const bool it = i == sh.fallen[k];
-        const double qk = with_q ? __dmul_rn(base, sh.scale_q[k]) : it ? 1.0 : 0.0;
-        pv = __dmul_rn(fmax(__dadd_rn(pv, -qk), 0.0), sh.scale_p[k]);
+        const bool it = i == sh.fallen[k].token;
+        const double qk = with_q ? __dmul_rn(base, sh.fallen[k].scale_q) : it ? 1.0 : 0.0;
+        pv = __dmul_rn(fmax(__dadd_rn(pv, -qk), 0.0), sh.fallen[k].scale_p);
         if (it) base = 0.0;
       }
       qv = base;
       return pv;
     };
-    // one exchange of four sums over all tokens; the warp's own stay in sp, sq, so, su
-    auto add_up = [&](double& sp, double& sq, double& so, double& su) {
-      Slot mine = {0.0, 0.0, 0.0, 0.0};
-      sp = warp_sum_d(sp), sq = warp_sum_d(sq), so = warp_sum_d(so), su = warp_sum_d(su);
-      if (lane == 0) { sh.sum_p[warp] = sp; sh.sum_q[warp] = sq; sh.over[warp] = so; sh.under[warp] = su; }
+    // one exchange of the warps' parts
+    auto add_up = [&](const Part& part) {
+      if (lane == 0) sh.part[warp] = part;
       __syncthreads();
+      Slot mine = {0.0, 0.0, 0.0, 0.0};
       if (warp == 0) {
-        const bool in = lane < WARPS;
-        double u = in ? sh.sum_p[lane] : 0.0, v = in ? sh.sum_q[lane] : 0.0, w = in ? sh.over[lane] : 0.0, z = in ? sh.under[lane] : 0.0;
-        u = warp_sum_d(u), v = warp_sum_d(v), w = warp_sum_d(w), z = warp_sum_d(z);
-        mine = {u, v, w, z};
+        const Part z = lane < WARPS ? sh.part[lane] : Part{0.0, 0.0, 0.0, 0.0};
+        mine = {warp_sum_d(z.sum_p), warp_sum_d(z.sum_q), warp_sum_d(z.over), warp_sum_d(z.under)};
       }
       return exchange_sums(mine);
     };
@@ -429,38 +496,14 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     // the sum of max(p - q, 0) came out too small to be had this way (p and q nearly the same).
     auto first_pass = [&](int gone, float lg, float dg, bool fell) -> bool {
       const double a0 = with_q ? (double)near_p / (double)near_q : 0.0;
-      double sp = 0.0, sq = 0.0, so = 0.0, su = 0.0;
-      for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
-        float a[CHUNK], b[CHUNK];
-        load_chunk(lrow, i0, hi, vec, lane, a);
-        const int it = gone - i0 - 4 * lane;
-        if (with_q) {
-          load_chunk(drow, i0, hi, vec, lane, b);
-#pragma unroll
-          for (int j = 0; j < CHUNK; ++j) {      // (tokens from hi on weigh nothing)
-            const double wp = weight(a[j], rp, sh.tab), wq = weight(b[j], rq, sh.tab), over = fma(a0, wp, -wq);
-            sp += wp;
-            if (it != step(j)) sq += wq;
-            if (over > 0.0) {
-              so += over;
-              su += wp;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < CHUNK; ++j) {
-            const double wp = weight(a[j], rp, sh.tab);
-            if (it != step(j)) sp += wp;
-          }
-        }
-      }
-      const Slot sum = add_up(sp, sq, so, su);
-      const double wg = gone >= 0 ? weight(lg, rp, sh.tab) : 0.0, dgw = gone >= 0 && with_q ? weight(dg, rq, sh.tab) : 0.0;
+      const Part mine = first_sums(lrow, with_q ? drow : nullptr, lo, hi, vec, lane, rp, rq, tab, a0, gone);
+      const Slot sum = add_up(mine);
+      const double wg = gone >= 0 ? weight(lg, rp, tab) : 0.0, dgw = gone >= 0 && with_q ? weight(dg, rq, tab) : 0.0;
       const double all_p = with_q ? sum.sum_p : sum.sum_p + wg, all_q = sum.sum_q + dgw;
       inv_p = 1.0 / all_p;
       if (with_q) inv_q = 1.0 / all_q;
       exact = true;
-      run = sp, total = sum.sum_p, plain = true;
+      own_p = mine.sum_p, own_over = mine.over, own_under = mine.under, shift = 0.0, unit = 1.0, total = sum.sum_p, plain = true, by_over = false;
       if (!fell) return true;
       // the list's entry for x; the draw's sums
       double left = 0.0;
@@ -469,18 +512,16 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
         const double da = all_q / all_p - a0;
         left = (sum.over + da * sum.under) / all_q;
         good = left > 1e-6;
-        if (good) run = (so + da * su) / all_q / left, total = 1.0, plain = false;
+        if (good) shift = da, unit = 1.0 / (all_q * left), total = 1.0, plain = false, by_over = true;
       } else if (sum.sum_p > NOTHING) {
         left = sum.sum_p / all_p;
-        run = sp / sum.sum_p, total = 1.0, plain = false;
+        unit = 1.0 / sum.sum_p, total = 1.0, plain = false;
       } else {
-        run = sp + (gone >= lo && gone < hi ? wg : 0.0), total = all_p;      // (p stays what it was)
+        stale = true;      // (p, all of it on the fallen child, stays what it was)
       }
       if (!good) return false;
       if (tid == 0) {
-        sh.fallen[0] = !with_q && left <= 0.0 ? -1 : gone;
-        sh.scale_p[0] = left > 0.0 ? 1.0 / left : 1.0;
-        sh.scale_q[0] = inv_q;
+        sh.fallen[0] = {left > 0.0 ? 1.0 / left : 1.0, inv_q, !with_q && left <= 0.0 ? -1 : gone};
       }
       __syncthreads();
       if (with_q) inv_q = sum.sum_q > NOTHING ? 1.0 / sum.sum_q : 0.0;
@@ -488,43 +529,37 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       return true;
     };
     // a further pass: child `gone` falls from p and q as `rejected` children have left them
-    auto next_pass = [&](int gone) {
+    auto next_pass = [&](int gone, bool fell) {      // (not fell: the sums as they are)
       __syncthreads();      // (nobody still reads the list's last entry)
-      if (tid == 0) { sh.fallen[rejected] = gone; sh.scale_p[rejected] = 1.0; sh.scale_q[rejected] = inv_q; }
+      if (tid == 0 && fell) sh.fallen[rejected] = {1.0, inv_q, gone};
       __syncthreads();
-      double sp = 0.0, sq = 0.0, so = 0.0, su = 0.0;
-      for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
-        float a[CHUNK], b[CHUNK];
-        load_chunk(lrow, i0, hi, vec, lane, a);
-        if (with_q) load_chunk(drow, i0, hi, vec, lane, b);
-#pragma unroll
-        for (int j = 0; j < CHUNK; ++j) {      // (tokens from hi on weigh nothing)
-          double qv;
-          sp += p_after(i0 + 4 * lane + step(j), a[j], with_q ? b[j] : 0.f, rejected + 1, qv);
-          sq += qv;
-        }
+      if (fell) ++rejected;
+      const Part mine = next_sums(lrow, with_q ? drow : nullptr, lo, hi, vec, lane, rp, rq, tab, inv_p, sh.fallen, rejected);
+      const Slot left = add_up(mine);
+      own_p = mine.sum_p, shift = 0.0, total = 1.0, plain = by_over = false;
+      if (!fell) {
+        unit = 1.0, total = left.sum_p, stale = false;
+        return;
       }
-      const Slot left = add_up(sp, sq, so, su);
-      if (left.sum_p > NOTHING) {
-        total = 1.0;
-        plain = false;
-        run = sp / left.sum_p;
-        if (tid == 0) sh.scale_p[rejected] = 1.0 / left.sum_p;
-      } else if (tid == 0) {      // nothing is left: p stays what it was (the rejection had no probability)
-        sh.scale_q[rejected] = 0.0;
-        if (!with_q) sh.fallen[rejected] = -1;
+      const int k = rejected - 1;
+      stale = !(left.sum_p > NOTHING);      // nothing is left: p stays what it was (the rejection had no probability)
+      if (!stale) unit = 1.0 / left.sum_p;
+      if (tid == 0) {
+        if (!stale) sh.fallen[k].scale_p = unit;
+        else sh.fallen[k].scale_q = 0.0;
+        if (stale && !with_q) sh.fallen[k].token = -1;
       }
       __syncthreads();
       if (with_q) inv_q = left.sum_q > NOTHING ? 1.0 / left.sum_q : 0.0;
-      ++rejected;
     };
     bool stands = false;
     for (;;) {
-      enum { EXACT, FALL_FIRST, FALL_NEXT } todo = EXACT;
+      enum { EXACT, FALL_FIRST, FALL_NEXT, RECOUNT } todo = EXACT;
       int gone = -1;
       float lg = 0.f, dg = 0.f;
       if (child < 0 || dead_q) {
-        if (exact) break;      // (the draw's sums are there)
+        if (exact && !stale) break;      // (the draw's sums are there)
+        if (exact) todo = RECOUNT;
       } else {
         if (!ok && first) atomicOr(err, FZ_ERR_TOKEN_RANGE);
         bool sure = true, yes;
@@ -551,8 +586,8 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
           lx = ok ? lrow[x] : 0.f, dx = ok && with_q ? drow[x] : 0.f;
         }
       }
-      if (todo != FALL_NEXT && !first_pass(gone, lg, dg, todo == FALL_FIRST)) todo = FALL_NEXT;
-      if (todo == FALL_NEXT) next_pass(gone);
+      if (todo < FALL_NEXT && !first_pass(gone, lg, dg, todo == FALL_FIRST)) todo = FALL_NEXT;
+      if (todo >= FALL_NEXT) next_pass(gone, todo == FALL_NEXT);
     }
     if (stands) {
       node = child;
@@ -560,46 +595,57 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       ++kept;
       continue;
     }
-    // The draw: the first token whose running sum, in index order, exceeds u * total. Where a warp's run begins and ends among the
-    // running sums: the blocks before, then the warps before, added up the same way by all, so that every end is the next one's
-    // beginning.
+    // The draw: the first token whose running sum, in index order, exceeds u * total. Where the blocks' runs begin among the running
+    // sums, then this block's warps': each end is the next one's beginning, the same number in every block.
     const double target = fmax(sh.uniform[0], 0.0) * total;      // (a NaN: 0)
-    if (lane == 0) sh.run[warp] = run;
+    if (lane == 0) sh.run[warp] = (by_over ? fmax(fma(shift, own_under, own_over), 0.0) : own_p) * unit;
     __syncthreads();
-    if (tid == 0) {
-      double sum = 0.0;
-      for (int w = 0; w < WARPS; ++w) sum += sh.run[w];
-      sh.slot[turn].sum_p = sum;
-    }
-    meet();
-    if (tid < BLOCKS) sh.block_run[tid] = BLOCKS == 1 ? sh.slot[turn].sum_p : cluster.map_shared_rank(&sh.slot[turn], tid)->sum_p;
-    __syncthreads();
-    double blocks = 0.0, behind = 0.0, own_sum = 0.0;
-    for (int b = 0; b < BLOCKS; ++b) {
-      const double sum = sh.block_run[b];
-      if (b < rank) blocks += sum;
-      else if (b > rank) behind += sum;
-      else own_sum = sum;
-    }
-    turn ^= 1;
-    // (nothing behind: u so near 1 that the sums' roundings end below the target: the last token that has any probability)
-    if (own_sum > NOTHING && blocks <= target && (blocks + own_sum > target || behind <= NOTHING)) {
-      // this block's: the warp whose run holds it, then all threads share that run, a few neighbouring tokens each
-      int who = -1;
-      double part = 0.0, begin = 0.0;
-      for (int w = 0; w < WARPS; ++w) {
-        const double end = part + sh.run[w];
-        if (sh.run[w] > NOTHING && blocks + part <= target) { who = w; begin = blocks + part; }      // (the last one that begins at or before it)
-        part = end;
+    if (warp == 0) {
+      const Slot b = lane < BLOCKS ? sh.block[lane] : Slot{0.0, 0.0, 0.0, 0.0};
+      double run = (by_over ? fmax(fma(shift, b.under, b.over), 0.0) : b.sum_p) * unit;
+#pragma unroll
+      for (int o = 1; o < BLOCKS; o <<= 1) {
+        const double v = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += v;
       }
+      if (lane < BLOCKS) sh.block_begin[lane + 1] = run;
+      const double start = __shfl_sync(0xffffffffu, run, (rank + 31) & 31);      // (the block before's end)
+      double w = lane < WARPS ? sh.run[lane] : 0.0;
+#pragma unroll
+      for (int o = 1; o < WARPS; o <<= 1) {
+        const double v = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += v;
+      }
+      if (lane == 0) sh.block_begin[0] = 0.0, sh.who = -1;
+      if (lane < WARPS) sh.warp_begin[lane + 1] = (rank > 0 ? start : 0.0) + w;
+      if (lane == 0) sh.warp_begin[0] = rank > 0 ? start : 0.0;
+    }
+    __syncthreads();
+    // the last block that has any probability and begins at or before the target holds the token (u may be so near 1 that the sums'
+    // roundings end below the target)
+    int holder = 0;
+    for (int b = 1; b < BLOCKS; ++b)
+      if (sh.block_begin[b] <= target && sh.block_begin[b + 1] - sh.block_begin[b] > NOTHING) holder = b;
+    if (holder == rank) {
+      // its last such warp; then all threads share that warp's run, a few neighbouring tokens each
+      int who = 0;
+      for (int w = 1; w < WARPS; ++w)
+        if (sh.run[w] > NOTHING && sh.warp_begin[w] <= target) who = w;
+      const double begin = sh.warp_begin[who];
       const int from = min(V, (rank * WARPS + who) * per_warp), to = min(V, from + per_warp);
       const int each = (to - from + THREADS - 1) / THREADS, i0 = min(to, from + tid * each), i1 = min(to, i0 + each);
       auto value = [&](int i) {
         double unused;
-        return plain ? weight(lrow[i], rp, sh.tab) : p_after(i, lrow[i], with_q ? drow[i] : 0.f, rejected, unused);
+        const double v = plain ? weight(lrow[i], rp, tab) : p_after(i, lrow[i], with_q ? drow[i] : 0.f, rejected, unused);
+        return v > NOTHING ? v : 0.0;
       };
       double mass = 0.0;
-      for (int i = i0; i < i1; ++i) mass += value(i);
+      int i = i0;
+      for (; i + 4 <= i1; i += 4) {
+        const double v0 = value(i), v1 = value(i + 1), v2 = value(i + 2), v3 = value(i + 3);
+        mass += (v0 + v1) + (v2 + v3);
+      }
+      for (; i < i1; ++i) mass += value(i);
       double upto = mass;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -608,25 +654,41 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       }
       __syncthreads();      // (the runs have been read)
       if (lane == 31) sh.run[warp] = upto;
-      if (tid == 0) sh.who = -1;
       __syncthreads();
-      double ahead = begin;
-      for (int w = 0; w < warp; ++w) ahead += sh.run[w];
-      double at = ahead + (upto - mass);
-      // the last thread whose tokens begin at or before the target holds it (the very sums that follow decide within it)
-      if (mass > NOTHING && at <= target) atomicMax(&sh.who, tid);
-      __syncthreads();
-      if (tid == sh.who) {
-        int last = -1, found = -1;
-        for (int i = i0; i < i1 && found < 0; ++i) {
-          const double v = value(i);
-          at += v;
-          if (v > NOTHING) {
-            last = i;
-            if (at > target) found = i;
-          }
+      if (warp == 0) {
+        double w = lane < WARPS ? sh.run[lane] : 0.0;
+#pragma unroll
+        for (int o = 1; o < WARPS; o <<= 1) {
+          const double v = __shfl_up_sync(0xffffffffu, w, o);
+          if (lane >= o) w += v;
         }
-        next_ids[s] = found >= 0 ? found : last;
+        if (lane < WARPS) sh.warp_begin[lane + 1] = begin + w;
+        if (lane == 0) sh.warp_begin[0] = begin;
+      }
+      __syncthreads();
+      // the last thread that has any and begins at or before the target; its warp walks that thread's tokens together
+      const double at = sh.warp_begin[warp] + (upto - mass);
+      if (mass > 0.0 && at <= target) atomicMax(&sh.who, tid);
+      __syncthreads();
+      if (sh.who < 0 && tid == 0) next_ids[s] = V - 1;      // (a run whose sum is the roundings of sums that cancel)
+      if (sh.who >= 0 && sh.who >> 5 == warp) {
+        const int src = sh.who & 31, t0 = __shfl_sync(0xffffffffu, i0, src), t1 = __shfl_sync(0xffffffffu, i1, src);
+        double run = __shfl_sync(0xffffffffu, at, src);
+        int found = -1, last = -1;
+        for (int t = t0; t < t1 && found < 0; t += 32) {
+          const double v = t + lane < t1 ? value(t + lane) : 0.0;
+          double w = v;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += y;
+          }
+          const unsigned hit = __ballot_sync(0xffffffffu, v > 0.0 && run + w > target), some = __ballot_sync(0xffffffffu, v > 0.0);
+          if (hit) found = t + __ffs(hit) - 1;
+          if (some) last = t + 31 - __clz(some);
+          run += __shfl_sync(0xffffffffu, w, 31);
+        }
+        if (lane == 0) next_ids[s] = found >= 0 ? found : last;
       }
     }
     result = -1;      // (written)
@@ -674,18 +736,21 @@ int launch(const float* logits, const float* draft, const float* temperature, co
 }
 }  // namespace
 
-// Blocks per request: as many as the chip holds at once beside the other requests' (14 clusters of eight, 32 of four, 74 of two),
-// each with 2,048 tokens and more.
+// Blocks per request: as many as the chip holds at once beside the other requests' (8 clusters of sixteen, 14 of eight, 32 of four, 74 of
+// two), each with 2,048 tokens and more. us at 128,256 tokens with 2, 4, 8 and 16 blocks: one request with 5 nodes 36, 23, 18, 16; 8 with 16
+// 163, 94, 64, 50; 64 with 6 at 151,936 tokens 137, 140, 195, 408.
 FZ_API int fz_verify_blocks(int S, int V) {
-  if (const char* v = getenv("FZ_VB")) return atoi(v);
   int b = S <= 8 ? 16 : S <= 14 ? 8 : S <= 32 ? 4 : S <= 74 ? 2 : 1;
   while (b > 1 && V < 2048 * b) b >>= 1;
   return b;
 }
 
 // Slices of a row whose quick statistics a kernel of its own takes ahead of the walks (0: none; the scratch: N * slices * 24 bytes).
+// It reads rows that no walk visits, but all SMs share it evenly, while walks differ in length: it pays where trees are small, two to six
+// nodes on average (us without and with it, a drafter's logits throughout: 64 chains of up to 6 nodes over 151,936 tokens 141 and 123, 16 of
+// 8 over 128,256 82 and 57; 30 trees of 10 71 and 101, 8 of 16 45 and 61; single nodes, 64 of them 31 and 37).
 FZ_API int fz_verify_ahead(int S, int N, int V) {
-  if (const char* v = getenv("FZ_VA")) { if (v[0] == '0') return 0; }
+  if (N < 2 * S || N > 6 * S) return 0;
   int slices = (8 * 148 + N - 1) / N;
   if (slices > MAX_SLICES) slices = MAX_SLICES;
   while (slices > 1 && V < 4096 * slices) --slices;

@@ -226,7 +226,8 @@ attn_tree_context_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, 
 struct Pieces {
   const float *part_o, *part_ml;
   int pieces, Hq, window;
-  __device__ __forceinline__ Range range(int n, int h, int, int, int, int, int, int start, int) const {
+  __device__ __forceinline__ int2 early(int, int) const { return make_int2(0, 0); }
+  __device__ __forceinline__ Range range(int2, int n, int h, int, int, int, int, int start, int) const {
     const int places = start - context_first(start, window), piece = piece_length(places);
     return {min(pieces, (places + piece - 1) / piece), ((size_t)n * Hq + h) * pieces, 1, 0, 0};
   }

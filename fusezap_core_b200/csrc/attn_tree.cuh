@@ -57,173 +57,191 @@ struct Range {
   int step, extra_from, extra_to;
 };
 
-__device__ __forceinline__ float4 load4(const float* p) { return *(const float4*)p; }
-__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
-  const uint2 u = *(const uint2*)p;
-  const float2 a = __bfloat1622float2(*(const __nv_bfloat162*)&u.x), b = __bfloat1622float2(*(const __nv_bfloat162*)&u.y);
-  return make_float4(a.x, a.y, b.x, b.y);
+// 16 bytes of T as float32.
+__device__ __forceinline__ void as_floats(const uint4& r, float (&v)[4]) {
+  v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
 }
-__device__ __forceinline__ void save4(float* p, float4 v) { *(float4*)p = v; }
-__device__ __forceinline__ void save4(__nv_bfloat16* p, float4 v) {
-  const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-  *(uint2*)p = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
+__device__ __forceinline__ void as_floats(const uint4& r, float (&v)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(*(const __nv_bfloat162*)&w[i]);
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ uint4 as_raw(const float (&v)[4]) { return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])); }
+__device__ __forceinline__ uint4 as_raw(const float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *(const uint32_t*)&p;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 constexpr int MERGE_WARPS = 8;
 
-// A warp per row and head; a lane has the dimensions 4 lane + 128 c. The context's pieces in rising order of their keys, then
-// the row's set bits in rising order, four keys at a time so that their loads and their sums over the lanes overlap. m, l, o:
-// maximum (exp2 domain), sum of weights and weighted values so far, float32.
-template <typename T, typename Where, int CH>
+// A warp per row and head, cut into groups of LANES lanes which take one piece of the context, or one place, each at a time: a group's lane
+// has the dimensions VEC (lane + LANES c) + 0 .. VEC - 1, c < D / VEC. Pieces and places go round the groups in rising order (the
+// tree's, then those that the row sees beside them); every group keeps its own maximum m (exp2 domain), sum of weights l and weighted values
+// o, float32, and the groups' are joined at the end. Bound by the chain of loads (row -> request -> pieces, pages -> values) and by
+// fetching its instructions, hence short loops instead of unrolled ones, and no spills: local memory is as far away as the rest (a
+// warp with four dimensions a lane and eight places at a time took 15 us from start to end).
+template <typename T, typename Where, int LANES, int D>
 __global__ void __launch_bounds__(32 * MERGE_WARPS)
 attn_tree_merge_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, const T* __restrict__ v_pool, T* __restrict__ out,
                        const Where where, const TreeArgs A) {
+  constexpr int VEC = 16 / sizeof(T), NC = D / VEC, GROUPS = 32 / LANES;
   fz_grid_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane / LANES, gl = lane % LANES;
+  const int n = blockIdx.x, h = blockIdx.y * MERGE_WARPS + warp, group = A.Hq / A.Hkv, kvh = h / group;
   fz_grid_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = blockIdx.x, h = blockIdx.y * MERGE_WARPS + warp;
   if (h >= A.Hq) return;
-  T* dst = out + ((size_t)n * A.Hq + h) * A.hd;
+  const size_t at = ((size_t)n * A.Hq + h) * A.hd;
   const int s = A.seq_row[n];
-  const bool there = s >= 0 && s < A.S && n >= A.seg[4 * s] && n - A.seg[4 * s] < A.seg[4 * s + 1];
-  if (!there) {      // a padding row
-    if (s >= 0 && lane == 0) atomicOr(A.err, FZ_ERR_ROW_RANGE);
+  unsigned bits = (unsigned)A.ancestors[(size_t)n * A.words];
+  const int2 record = where.early(n, kvh);
+  const int pos = A.window > 0 ? A.pos[n] : 0;
+  float qv[D], o[D];
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-      if (4 * lane + 128 * c < A.hd) save4(dst + 4 * lane + 128 * c, make_float4(0.f, 0.f, 0.f, 0.f));
+  for (int c = 0; c < NC; ++c) {
+    const int d = VEC * (gl + LANES * c);
+    float x[VEC];
+    as_floats(d < A.hd ? *(const uint4*)(q + at + d) : make_uint4(0u, 0u, 0u, 0u), x);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) qv[c * VEC + i] = x[i] * A.scale_log2, o[c * VEC + i] = 0.f;
+  }
+  const bool named = s >= 0 && s < A.S;
+  const int row0 = named ? A.seg[4 * s] : 0, nodes = named ? A.seg[4 * s + 1] : 0, start = named ? A.seg[4 * s + 2] : 0;
+  if (!named || n < row0 || n - row0 >= nodes) {      // a padding row
+    if (s >= 0 && lane == 0) atomicOr(A.err, FZ_ERR_ROW_RANGE);
+    for (int d = VEC * lane; d < A.hd; d += 32 * VEC) *(uint4*)(out + at + d) = make_uint4(0u, 0u, 0u, 0u);
     return;
   }
-  const int row0 = A.seg[4 * s], nodes = A.seg[4 * s + 1], start = A.seg[4 * s + 2], kvh = h / (A.Hq / A.Hkv);
-  float m = -INFINITY, l = 0.f;
-  float4 o[CH], qv[CH];
-  const T* from = q + ((size_t)n * A.Hq + h) * A.hd;
-#pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    const bool in = 4 * lane + 128 * c < A.hd;
-    o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-    qv[c] = in ? load4(from + 4 * lane + 128 * c) : o[c];
-  }
-  const int group = A.Hq / A.Hkv;
-  const Range range = where.range(n, h, s, n - row0, kvh, h - kvh * group, nodes, start, A.pos[n]);
-  const int pieces = range.pieces;
-  for (int f0 = 0; f0 < pieces; f0 += 32) {
-    const int here = min(32, pieces - f0);
-    const float2 ml = lane < here ? *(const float2*)(where.part_ml + 2 * (range.first + (size_t)(f0 + lane) * range.step)) : make_float2(-INFINITY, 0.f);
-    float top = ml.x;
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    const float mn = fmaxf(m, top);
-    if (mn == -INFINITY) continue;      // (no row of these pieces saw a key)
-    const float corr = exp2f(m - mn), e = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mn);
-    m = mn;
-    l *= corr;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) { o[c].x *= corr; o[c].y *= corr; o[c].z *= corr; o[c].w *= corr; }
-#pragma unroll 4
-    for (int f = 0; f < here; ++f) {
-      const float w = __shfl_sync(0xffffffffu, e, f), add = __shfl_sync(0xffffffffu, ml.y, f);
-      if (w == 0.f) continue;      // (a piece of which the row sees nothing may hold anything)
-      l = fmaf(add, w, l);
-      const float* src = where.part_o + (range.first + (size_t)(f0 + f) * range.step) * A.hd;
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        if (4 * lane + 128 * c < A.hd) {
-          const float4 v = *(const float4*)(src + 4 * lane + 128 * c);
-          o[c].x = fmaf(v.x, w, o[c].x); o[c].y = fmaf(v.y, w, o[c].y); o[c].z = fmaf(v.z, w, o[c].z); o[c].w = fmaf(v.w, w, o[c].w);
-        }
-      }
-    }
-  }
+  const Range range = where.range(record, n, h, n - row0, h - kvh * group, group, nodes, start, pos);
+  // the pages of the tree's first places, a lane each
   const int* trow = A.table + (size_t)s * A.mb;
-  // up to four places (-1: none)
-  auto attend = [&](const int (&places)[4]) {
-    float4 kv[4][CH], vv[4][CH];
-    float sc[4];
-    bool ok[4];
+  const int page0 = start / A.page_size;
+  const int pages = page0 + lane < A.mb && (long long)(page0 + lane) * A.page_size < (long long)start + nodes ? trow[page0 + lane] : -1;
+  float m = -INFINITY, l = 0.f;
+  // the context's pieces
+#pragma unroll 2
+  for (int f = g; f < range.pieces; f += GROUPS) {
+    const size_t slot = range.first + (size_t)f * range.step;
+    const float2 ml = *(const float2*)(where.part_ml + 2 * slot);
+    const float* src = where.part_o + slot * A.hd;
+    float4 v[D / 4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      ok[u] = places[u] >= 0;
-      long long off = 0;
-      if (ok[u]) {
-        const int pi = places[u] / A.page_size;
-        const int page = pi < A.mb ? trow[pi] : -1;
-        ok[u] = page >= 0 && page < A.num_pages;
-        if (ok[u]) off = (long long)page * A.page_stride + ((long long)kvh * A.page_size + (places[u] - pi * A.page_size)) * A.hd;
-        else if (lane == 0) atomicOr(A.err, FZ_ERR_NO_PAGE);
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < VEC; i += 4) {
+        const int d = VEC * (gl + LANES * c) + i;
+        v[(c * VEC + i) / 4] = d < A.hd ? *(const float4*)(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const bool in = ok[u] && 4 * lane + 128 * c < A.hd;
-        kv[u][c] = in ? load4(k_pool + off + 4 * lane + 128 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
-        vv[u][c] = in ? load4(v_pool + off + 4 * lane + 128 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      sc[u] = 0.f;
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        sc[u] = fmaf(qv[c].x, kv[u][c].x, sc[u]); sc[u] = fmaf(qv[c].y, kv[u][c].y, sc[u]);
-        sc[u] = fmaf(qv[c].z, kv[u][c].z, sc[u]); sc[u] = fmaf(qv[c].w, kv[u][c].w, sc[u]);
-      }
-    }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) sc[u] += __shfl_xor_sync(0xffffffffu, sc[u], x);
-    float mn = m;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      sc[u] = ok[u] ? sc[u] * A.scale_log2 : -INFINITY;
-      mn = fmaxf(mn, sc[u]);
-    }
-    const float mu = mn == -INFINITY ? 0.f : mn, corr = exp2f(m - mu);
+    if (ml.x == -INFINITY) continue;      // (a piece of which the row sees nothing may hold anything)
+    const float mn = fmaxf(m, ml.x), corr = exp2f(m - mn), w = exp2f(ml.x - mn);
     m = mn;
-    l *= corr;
+    l = l * corr + ml.y * w;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) { o[c].x *= corr; o[c].y *= corr; o[c].z *= corr; o[c].w *= corr; }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (!ok[u]) continue;
-      const float e = exp2f(sc[u] - mu);
-      l += e;
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        o[c].x = fmaf(vv[u][c].x, e, o[c].x); o[c].y = fmaf(vv[u][c].y, e, o[c].y);
-        o[c].z = fmaf(vv[u][c].z, e, o[c].z); o[c].w = fmaf(vv[u][c].w, e, o[c].w);
-      }
+    for (int i = 0; i < D / 4; ++i) {
+      o[4 * i] = o[4 * i] * corr + v[i].x * w, o[4 * i + 1] = o[4 * i + 1] * corr + v[i].y * w;
+      o[4 * i + 2] = o[4 * i + 2] * corr + v[i].z * w, o[4 * i + 3] = o[4 * i + 3] * corr + v[i].w * w;
     }
-  };
-  for (int x = range.extra_from; x < range.extra_to; x += 4) {
-    const int places[4] = {x, x + 1 < range.extra_to ? x + 1 : -1, x + 2 < range.extra_to ? x + 2 : -1, x + 3 < range.extra_to ? x + 3 : -1};
-    attend(places);
   }
-  for (int w0 = 0; w0 < A.words && 32 * w0 < nodes; ++w0) {
-    unsigned bits = (unsigned)A.ancestors[(size_t)n * A.words + w0];
-    if (nodes - 32 * w0 < 32) bits &= (1u << (nodes - 32 * w0)) - 1u;
-    while (bits) {
-      int places[4];
+  // places, GROUPS at a time: the tree's whose bit is set, then the others
+  int w0 = 0, extra = range.extra_from;
+  if (nodes < 32) bits &= (1u << nodes) - 1u;
+#pragma unroll 1
+  for (;;) {
+    while (!bits && ++w0 < A.words && 32 * w0 < nodes) {
+      bits = (unsigned)A.ancestors[(size_t)n * A.words + w0];
+      if (nodes - 32 * w0 < 32) bits &= (1u << (nodes - 32 * w0)) - 1u;
+    }
+    int place = -1;
+    if (bits) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        places[u] = bits ? start + 32 * w0 + __ffs(bits) - 1 : -1;
+      for (int i = 0; i < GROUPS; ++i) {
+        if (i == g && bits) place = start + 32 * w0 + __ffs(bits) - 1;
         bits &= bits - 1;
       }
-      attend(places);
+    } else if (extra < range.extra_to) {
+      place = extra + g < range.extra_to ? extra + g : -1;
+      extra += GROUPS;
+    } else {
+      break;
+    }
+    const int pi = place / A.page_size, near = __shfl_sync(0xffffffffu, pages, (pi - page0) & 31);
+    const int page = place < 0 ? -1 : pi >= page0 && pi < page0 + 32 ? near : pi < A.mb ? trow[pi] : -1;
+    const bool seen = page >= 0 && page < A.num_pages;
+    if (place >= 0 && !seen && gl == 0) atomicOr(A.err, FZ_ERR_NO_PAGE);
+    const long long off = seen ? (long long)page * A.page_stride + ((long long)kvh * A.page_size + (place - pi * A.page_size)) * A.hd : 0;
+    uint4 kr[NC], vr[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int d = VEC * (gl + LANES * c);
+      const bool in = seen && d < A.hd;
+      kr[c] = in ? *(const uint4*)(k_pool + off + d) : make_uint4(0u, 0u, 0u, 0u);
+      vr[c] = in ? *(const uint4*)(v_pool + off + d) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    float sc = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      float x[VEC];
+      as_floats(kr[c], x);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sc = fmaf(qv[c * VEC + i], x[i], sc);
+    }
+#pragma unroll
+    for (int x = LANES / 2; x > 0; x >>= 1) sc += __shfl_xor_sync(0xffffffffu, sc, x);
+    if (!seen) continue;
+    const float mn = fmaxf(m, sc), mu = mn == -INFINITY ? 0.f : mn, corr = exp2f(m - mu), e = exp2f(sc - mu);
+    m = mn;
+    l = l * corr + e;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      float x[VEC];
+      as_floats(vr[c], x);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) o[c * VEC + i] = o[c * VEC + i] * corr + x[i] * e;
     }
   }
+  // the groups' results
+  float top = m;
+#pragma unroll
+  for (int x = LANES; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  const float w = m == -INFINITY ? 0.f : exp2f(m - top);
+  l *= w;
+#pragma unroll
+  for (int x = LANES; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
   const float inv = l == 0.f ? 0.f : 1.0f / l;      // (a row that sees no key gives zeros)
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
-    if (4 * lane + 128 * c < A.hd)
-      save4(dst + 4 * lane + 128 * c, make_float4(o[c].x * inv, o[c].y * inv, o[c].z * inv, o[c].w * inv));
+  for (int i = 0; i < D; ++i) {
+    float v = w == 0.f ? 0.f : o[i] * w;
+#pragma unroll
+    for (int x = LANES; x < 32; x <<= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
+    o[i] = v * inv;
+  }
+  if (g == 0) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int d = VEC * (gl + LANES * c);
+      float x[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[i] = o[c * VEC + i];
+      if (d < A.hd) *(uint4*)(out + at + d) = as_raw(x);
+    }
+  }
 }
 
 template <typename T, typename Where>
 int launch_merge(const T* q, const T* k, const T* v, T* out, const Where& where, const TreeArgs& A, cudaStream_t stream) {
-  const dim3 grid((unsigned)A.N, (unsigned)((A.Hq + MERGE_WARPS - 1) / MERGE_WARPS));
+  const dim3 grid((unsigned)A.N, (unsigned)((A.Hq + MERGE_WARPS - 1) / MERGE_WARPS)), block(32 * MERGE_WARPS);
   cudaError_t e;
-  if (A.hd <= 128) e = fz_launch(attn_tree_merge_kernel<T, Where, 1>, grid, dim3(32 * MERGE_WARPS), 0, stream, q, k, v, out, where, A);
-  else if (A.hd <= 256) e = fz_launch(attn_tree_merge_kernel<T, Where, 2>, grid, dim3(32 * MERGE_WARPS), 0, stream, q, k, v, out, where, A);
-  else e = fz_launch(attn_tree_merge_kernel<T, Where, 4>, grid, dim3(32 * MERGE_WARPS), 0, stream, q, k, v, out, where, A);
+  if (A.hd <= 64) e = fz_launch(attn_tree_merge_kernel<T, Where, 8, 8>, grid, block, 0, stream, q, k, v, out, where, A);
+  else if (A.hd <= 128) e = fz_launch(attn_tree_merge_kernel<T, Where, 8, 16>, grid, block, 0, stream, q, k, v, out, where, A);
+  else if (A.hd <= 256) e = fz_launch(attn_tree_merge_kernel<T, Where, 16, 16>, grid, block, 0, stream, q, k, v, out, where, A);
+  else e = fz_launch(attn_tree_merge_kernel<T, Where, 32, 16>, grid, block, 0, stream, q, k, v, out, where, A);
   return e == cudaSuccess ? FZ_OK : (int)e;
 }
 

@@ -46,67 +46,93 @@ struct Sizes {
   int S, NB, Hkv, window;
 };
 
-// Sums over the requests before `stop` (all: S) of their units and items; the whole warp takes part. With find >= 0: stops at the
-// request that holds unit `find`, whose number it returns (-1: none).
-__device__ __forceinline__ int sum_units(const Sizes& Z, int stop, int find, int& units, int& items) {
-  const int lane = threadIdx.x & 31;
-  units = items = 0;
-  for (int s0 = 0; s0 < stop; s0 += 32) {
-    int u = 0, t = 0;
-    if (s0 + lane < stop) {
-      const int2 sg = make_int2(Z.seg[4 * (s0 + lane) + 1], Z.seg[4 * (s0 + lane) + 2]);
+// The walk of a block (every role's own copy, warp-wide) over its run of units, one stretch at a time: a stretch is the block's share of
+// an item, `count` key tiles of the places [a, b) from place `key0` on. Requests are looked up only where the run crosses from one to the
+// next; within a request the next item follows by counting.
+struct Walk {
+  int G, u, u1;                                    // the next unit, the run's end
+  int s, n, row0, a, b, tiles, row_tiles;          // the request
+  int end, first_item;                             // its last unit + 1, its first item
+  int chunk, chunk_units, chunk_items;             // where the look-up goes on: 32 requests from `chunk`, units and items before them
+  int kvh, rt, item;                               // the item
+  int row, rows, key0, count;                      // the stretch: first row, (node, head) rows, first place, key tiles
+
+  // Sum of all requests' units.
+  static __device__ __forceinline__ int sum(const Sizes& Z) {
+    const int lane = threadIdx.x & 31;
+    int total = 0;
+    for (int s = lane; s < Z.S; s += 32) {
       int a, tiles, row_tiles;
-      request_units(sg.x, sg.y, Z.window, Z.NB, a, tiles, row_tiles);
-      t = Z.Hkv * row_tiles;
-      u = t * tiles;
+      request_units(Z.seg[4 * s + 1], Z.seg[4 * s + 2], Z.window, Z.NB, a, tiles, row_tiles);
+      total += Z.Hkv * row_tiles * tiles;
     }
-    int uu = u, tt = t;
+    return __reduce_add_sync(0xffffffffu, total);
+  }
+  // The request that holds unit u, and the item and tile within it.
+  __device__ __forceinline__ void find(const Sizes& Z) {
+    const int lane = threadIdx.x & 31;
+    int units = chunk_units, items = chunk_items;
+    for (int s0 = chunk; s0 < Z.S; s0 += 32) {
+      int nn = 0, bb = 0, rr = 0, aa = 0, tt = 0, rt_ = 0;
+      if (s0 + lane < Z.S) {
+        const int* e = Z.seg + 4 * (s0 + lane);
+        rr = e[0], nn = e[1], bb = e[2];
+        request_units(nn, bb, Z.window, Z.NB, aa, tt, rt_);
+      }
+      const int mine_i = Z.Hkv * rt_, mine_u = mine_i * tt;
+      int iu = mine_u, ii = mine_i;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, uu, o), y = __shfl_up_sync(0xffffffffu, tt, o);
-      if (lane >= o) { uu += x; tt += y; }
-    }
-    if (find >= 0) {
-      const unsigned hit = __ballot_sync(0xffffffffu, units + uu > find);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, iu, o), y = __shfl_up_sync(0xffffffffu, ii, o);
+        if (lane >= o) { iu += x; ii += y; }
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, units + iu > u);
       if (hit) {
         const int who = __ffs(hit) - 1;
-        units += __shfl_sync(0xffffffffu, uu - u, who);
-        items += __shfl_sync(0xffffffffu, tt - t, who);
-        return s0 + who;
+        chunk = s0, chunk_units = units, chunk_items = items;
+        s = s0 + who;
+        n = __shfl_sync(0xffffffffu, nn, who), b = __shfl_sync(0xffffffffu, bb, who), row0 = __shfl_sync(0xffffffffu, rr, who);
+        a = __shfl_sync(0xffffffffu, aa, who), tiles = __shfl_sync(0xffffffffu, tt, who), row_tiles = __shfl_sync(0xffffffffu, rt_, who);
+        end = units + __shfl_sync(0xffffffffu, iu, who);
+        const int begin = end - __shfl_sync(0xffffffffu, mine_u, who);
+        first_item = items + __shfl_sync(0xffffffffu, ii - mine_i, who);
+        const int within = u - begin, k = within / tiles;
+        kvh = k / row_tiles;
+        rt = k - kvh * row_tiles;
+        item = first_item + k;
+        tile = within - k * tiles;
+        return;
       }
+      units += __shfl_sync(0xffffffffu, iu, 31);
+      items += __shfl_sync(0xffffffffu, ii, 31);
     }
-    units += __shfl_sync(0xffffffffu, uu, 31);
-    items += __shfl_sync(0xffffffffu, tt, 31);
   }
-  return -1;
-}
-
-// A block's share of an item: key tiles of the places [a, b), the first of which starts at place `key0`.
-struct Stretch {
-  int s, kvh, row, rows, key0, tiles, a, b, item;
+  int tile;      // the stretch's first within its item
+  // The next stretch; false at the run's end.
+  __device__ __forceinline__ bool next(const Sizes& Z) {
+    if (u >= u1) return false;
+    if (u >= end) {
+      find(Z);
+    } else {
+      tile = 0;
+      ++item;
+      if (++rt == row_tiles) rt = 0, ++kvh;
+    }
+    const int node0 = rt * Z.NB;
+    row = row0 + node0;
+    rows = min(Z.NB, n - node0) * G;
+    key0 = (a / BN + tile) * BN;
+    count = min(tiles - tile, u1 - u);
+    u += count;
+    return true;
+  }
 };
-__device__ __forceinline__ void get_stretch(const Sizes& Z, int G, int u, int u1, Stretch& x) {
-  int units, items;
-  x.s = sum_units(Z, Z.S, u, units, items);
-  const int n = Z.seg[4 * x.s + 1];
-  x.b = Z.seg[4 * x.s + 2];
-  int tiles, row_tiles;
-  request_units(n, x.b, Z.window, Z.NB, x.a, tiles, row_tiles);
-  const int within = u - units, item = within / tiles, tile = within - item * tiles;
-  x.kvh = item / row_tiles;
-  const int node0 = (item - x.kvh * row_tiles) * Z.NB;
-  x.row = Z.seg[4 * x.s] + node0;
-  x.rows = min(Z.NB, n - node0) * G;
-  x.key0 = (x.a / BN + tile) * BN;
-  x.tiles = min(tiles - tile, u1 - u);
-  x.item = items + item;
-}
 
 template <int HD, int BOX>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map, const __nv_bfloat16* __restrict__ v_pool,
                     const Sizes Z, const int* __restrict__ table, int mb, int page_size, int num_pages, int Hq, float scale_log2,
-                    int slots, float* __restrict__ part_o, float* __restrict__ part_ml, int* err) {
+                    int N, int slots, float* __restrict__ part_o, float* __restrict__ part_ml, int2* __restrict__ records, int* err) {
   constexpr int HALVES = HD / 64;                     // 64-column halves of a head
   constexpr int STAGES = HD <= 64 ? 6 : 3;            // key tiles and value tiles in flight
   constexpr int HALF_BYTES = 128 * 128;               // 128 rows of 128 bytes
@@ -149,6 +175,9 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     mbar_init_fence();
   }
   if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
+  // (brought into L2 ahead of the wait on the kernel before; read behind it)
+  if (warp == 2)
+    for (int i = lane * 8; i < Z.S; i += 256) asm volatile("prefetch.global.L2 [%0];" ::"l"(Z.seg + 4 * i));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -156,22 +185,20 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
   fz_grid_launch_dependents();
   fz_grid_wait();
   const int G = Hq / Z.Hkv;
-  int total, unused;
-  sum_units(Z, Z.S, -1, total, unused);
-  const int share = (total + gridDim.x - 1) / gridDim.x;
+  const int total = Walk::sum(Z), share = (total + gridDim.x - 1) / gridDim.x;
   const int u0 = min(total, (int)blockIdx.x * share), u1 = min(total, u0 + share);
   // Every role walks the same stretches and counts the key tiles it has gone through (`g`): ring stages, streams and barrier phases
   // follow from that count and carry over from one stretch to the next.
   bool ok = true;
-  Stretch x;
+  Walk x;
+  x.G = G, x.u = u0, x.u1 = u1, x.end = x.chunk = x.chunk_units = x.chunk_items = 0;
 
   if (warp == 0 || warp == 18) {
     // ---------------- producers
     const bool is_v = warp == 18;
     const int rows_per_page = 2 * Z.Hkv * page_size;
     int g = 0, n_q = 0;
-    for (int u = u0; ok && u < u1; u += x.tiles) {
-      get_stretch(Z, G, u, u1, x);
+    while (ok && x.next(Z)) {
       if (!is_v) {
         // the one Q buffer is free once the last score product of the stretch before is done
         if (n_q > 0) ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (n_q - 1) & 1));
@@ -186,7 +213,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
         ++n_q;
       }
       const int* trow = table + (size_t)x.s * mb;
-      for (int t = 0; t < x.tiles && ok; ++t, ++g) {
+      for (int t = 0; t < x.count && ok; ++t, ++g) {
         const int s = g % STAGES, round = g / STAGES;
         const int key0 = x.key0 + t * BN;
         // op -> (page box, column half). Keys: boxes with any place of [a, b). Values: boxes of groups of 16 places that lie in it whole.
@@ -251,9 +278,9 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     // ---------------- MMA issuer (the warp walks the stretches together, lane 0 issues)
     constexpr uint32_t idesc_s = make_idesc(BM, BN, false), idesc_pv = make_idesc(BM, HD, true);
     // The scores run two tiles ahead of the products with the values: two walks over the same stretches.
-    Stretch y;
-    int su = u0, st = 0, sg = 0, n_q = 0;      // the score walk: unit, tile within its stretch, tiles so far
-    if (su < u1) get_stretch(Z, G, su, u1, y);
+    Walk y = x;
+    int st = 0, sg = 0, n_q = 0;               // the score walk: tile within its stretch, tiles so far, stretches so far
+    bool more = y.next(Z);
     auto issue_s = [&]() -> bool {             // S(sg) = Q K(sg)^T into the scores of stream sg & 1; frees the key stage when done
       bool fine = true;
       if (lane == 0) {
@@ -271,25 +298,23 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
           }
           umma_commit(&s_ready[sg & 1]);
           umma_commit(&k_empty[s]);
-          if (st + 1 == y.tiles) umma_commit(q_empty);      // the stretch's last score product: Q may be overwritten when it is done
+          if (st + 1 == y.count) umma_commit(q_empty);      // the stretch's last score product: Q may be overwritten when it is done
         }
       }
       fine = __shfl_sync(0xffffffffu, (int)fine, 0);
       if (!fine) return false;
       ++sg;
-      if (++st == y.tiles) {
-        su += y.tiles;
+      if (++st == y.count) {
         st = 0;
         ++n_q;
-        if (su < u1) get_stretch(Z, G, su, u1, y);
+        more = y.next(Z);
       }
       return true;
     };
     int g = 0;
-    for (int i = 0; i < 2 && ok && su < u1; ++i) ok = issue_s();
-    for (int u = u0; ok && u < u1; u += x.tiles) {
-      get_stretch(Z, G, u, u1, x);
-      for (int t = 0; t < x.tiles && ok; ++t, ++g) {
+    for (int i = 0; i < 2 && ok && more; ++i) ok = issue_s();
+    while (ok && x.next(Z)) {
+      for (int t = 0; t < x.count && ok; ++t, ++g) {
         if (lane == 0) {
           const int s = g % STAGES, tq = g & 1;
           ok = mbar_wait(&v_full[s], (g / STAGES) & 1) && mbar_wait(&p_ready[tq], (g >> 1) & 1);      // P(g) written, O rescaled if it had to be
@@ -303,12 +328,12 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
               const uint32_t p = tmem_p + (uint32_t)(kk < 4 ? 8 * kk : 64 + 8 * (kk - 4));
               umma_bf16_a_tmem(tmem_o, p, desc_mn_major(sv + kk * 16 * 128, HALF_BYTES), idesc_pv, (t >= 2 || kk > k0) ? 1u : 0u);
             }
-            if (t + 2 >= x.tiles) umma_commit(&o_ready[tq]);      // the stream's last of the stretch
+            if (t + 2 >= x.count) umma_commit(&o_ready[tq]);      // the stream's last of the stretch
             umma_commit(&v_empty[s]);
           }
         }
         ok = __shfl_sync(0xffffffffu, (int)ok, 0);
-        if (ok && su < u1) ok = issue_s();      // the stream's next scores go behind the product that reads its P
+        if (ok && more) ok = issue_s();      // the stream's next scores go behind the product that reads its P
       }
     }
     if (!ok && lane == 0) flag[0] = 1;
@@ -324,12 +349,17 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     float* mx_mine = s_mx + (tq * 2 + hf) * BM + r;
     const float* mx_other = s_mx + (tq * 2 + (hf ^ 1)) * BM + r;
     int g0 = 0, n_s = 0, n_o[2] = {0, 0};      // tiles of the block, of this stream, and stretches with tiles of either stream so far
-    for (int u = u0; ok && u < u1; u += x.tiles) {
-      get_stretch(Z, G, u, u1, x);
+    while (ok && x.next(Z)) {
+      // which slots the item's rows will find their stretches in, from the block that has its first: (first slot, stretches)
+      if (x.tile == 0 && idx == 0) {
+        const int last = (x.u - x.count + x.tiles - 1) / share;
+        for (int i = lane; i < x.rows / G; i += 32)
+          if (x.row + i < N) records[(size_t)(x.row + i) * Z.Hkv + x.kvh] = make_int2(blockIdx.x + x.item, last - blockIdx.x + 1);
+      }
       const bool live = quad * 32 < x.rows;      // (the warp has rows)
       const int first = (g0 ^ tq) & 1;           // the first tile of the stretch that is this stream's
       float m_run = -INFINITY, l_part = 0.f;     // the maximum in use (exp2 domain) and this thread's half of the row's sum
-      for (int t = first; t < x.tiles && ok; t += 2) {
+      for (int t = first; t < x.count && ok; t += 2) {
         ok = __all_sync(0xffffffffu, mbar_wait(&s_ready[tq], n_s & 1));
         if (!ok) break;
         ++n_s;
@@ -423,14 +453,14 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
       }
       if (!ok) break;
       // the stretch's end: both streams' last products, then the two results joined, a quarter of the dimensions per thread
-      const bool has[2] = {x.tiles > ((g0 ^ 0) & 1), x.tiles > ((g0 ^ 1) & 1)};
+      const bool has[2] = {x.count > ((g0 ^ 0) & 1), x.count > ((g0 ^ 1) & 1)};
       // (warps without rows do not wait here: the barriers below, which keep a row quarter's warps within one stretch of one another,
       // are not theirs, and a phase that has come round twice cannot be told from one that has not)
       for (int j = 0; j < 2 && ok; ++j) {
         if (has[j] && live) ok = __all_sync(0xffffffffu, mbar_wait(&o_ready[j], n_o[j] & 1));
         n_o[j] += has[j];
       }
-      g0 += x.tiles;
+      g0 += x.count;
       if (!ok) break;
       if (!live) continue;
       tc_fence_after();
@@ -442,10 +472,12 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
       asm volatile("bar.sync %0, 128;" ::"r"(quad_bar) : "memory");
       const float f0 = fast_exp2(m0 - mu), f1 = fast_exp2(m1 - mu);      // (a stream without tiles: maximum -inf, weight 0)
       const float l = (s_mx[r] + s_mx[BM + r]) * f0 + (s_mx[2 * BM + r] + s_mx[3 * BM + r]) * f1;
-      const size_t at = ((size_t)(blockIdx.x + x.item)) * BM + r;
-      const bool mine = r < x.rows && (int)blockIdx.x + x.item < slots;
-      if ((int)blockIdx.x + x.item >= slots && lane == 0) atomicOr(err, FZ_ERR_ROW_RANGE);      // (requests with more rows than the step has)
-      const int d0 = (tq * 2 + hf) * JD;
+      const size_t slot0 = ((size_t)(blockIdx.x + x.item)) * BM;
+      const bool in_slots = (int)blockIdx.x + x.item < slots;
+      if (!in_slots && lane == 0) atomicOr(err, FZ_ERR_ROW_RANGE);      // (requests with more rows than the step has)
+      // A lane has one row: a store instruction would touch 32 lines with 16 bytes each. So every four lanes exchange first, four vectors
+      // of four dimensions each: then a lane has vector `lane % 4` of all four rows, and an instruction writes 64 bytes of eight rows.
+      const int d0 = (tq * 2 + hf) * JD, base = quad * 32 + (lane & ~3);
 #pragma unroll
       for (int c = 0; c < JD; c += 16) {
         float a[16], b[16];
@@ -453,12 +485,26 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
         tmem_ld16(tmem_base + 256u + (uint32_t)(HD + d0 + c) + lane_sel, b);
 #pragma unroll
         for (int j = 0; j < 16; ++j) a[j] = (has[0] ? a[j] * f0 : 0.f) + (has[1] ? b[j] * f1 : 0.f);
-        if (mine) {
 #pragma unroll
-          for (int j = 0; j < 16; j += 4) *(float4*)(part_o + at * HD + d0 + c + j) = make_float4(a[j], a[j + 1], a[j + 2], a[j + 3]);
+        for (int k = 2; k > 0; k >>= 1) {
+          const bool up = lane & k;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (i & k) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float got = __shfl_xor_sync(0xffffffffu, up ? a[4 * i + j] : a[4 * (i | k) + j], k);
+              if (up) a[4 * i + j] = got;
+              else a[4 * (i | k) + j] = got;
+            }
+          }
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)      // (a[4 j ..] is now vector lane % 4 of row `base + j`)
+          if (in_slots && base + j < x.rows)
+            *(float4*)(part_o + (slot0 + base + j) * HD + d0 + c + 4 * (lane & 3)) = make_float4(a[4 * j], a[4 * j + 1], a[4 * j + 2], a[4 * j + 3]);
       }
-      if (mine && d0 == 0) *(float2*)(part_ml + 2 * at) = make_float2(m, l);
+      if (in_slots && r < x.rows && d0 == 0) *(float2*)(part_ml + 2 * (slot0 + r)) = make_float2(m, l);
       // nobody of this row quarter starts on the next stretch's tiles (whose products overwrite O) before all four have read
       tc_fence_before();
       asm volatile("bar.sync %0, 128;" ::"r"(quad_bar) : "memory");
@@ -474,32 +520,25 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
   if (tid == 0 && flag[0]) atomicOr(err, FZ_ERR_WAIT_TIMEOUT);
 }
 
-// Where a row's stretches lie, by the same arithmetic.
+// Where a row's stretches lie: as the record says that the block with its item's first stretch has left (none for an item without units).
 struct Stretches {
   const float *part_o, *part_ml;
-  Sizes Z;
-  int blocks, Hq;
-  __device__ __forceinline__ Range range(int, int, int s, int node, int kvh, int head_in_group, int n, int start, int pos) const {
-    int total, before, items, unused;
-    sum_units(Z, Z.S, -1, total, unused);
-    sum_units(Z, s, -1, before, items);
-    const int G = Hq / Z.Hkv, share = (total + blocks - 1) / blocks;
+  const int2* records;
+  int NB, Hkv, window, slots;
+  __device__ __forceinline__ int2 early(int n, int kvh) const { return records[(size_t)n * Hkv + kvh]; }
+  __device__ __forceinline__ Range range(int2 record, int, int, int node, int head_in_group, int group, int nodes, int start, int pos) const {
     int a, tiles, row_tiles;
-    request_units(n, start, Z.window, Z.NB, a, tiles, row_tiles);
+    request_units(nodes, start, window, NB, a, tiles, row_tiles);
     Range x;
     x.extra_from = x.extra_to = 0;
-    if (Z.window > 0) {      // places that this row sees and a later one does not
-      x.extra_from = max(0, pos - Z.window + 1);
+    if (window > 0) {      // places that this row sees and a later one does not
+      x.extra_from = max(0, pos - window + 1);
       x.extra_to = min(a, start);
     }
-    x.pieces = 0;
-    x.first = 0;
+    const bool there = tiles > 0 && record.x >= 0 && record.y > 0 && record.x <= slots - record.y;
+    x.pieces = there ? record.y : 0;
+    x.first = there ? (size_t)record.x * BM + (node % NB) * group + head_in_group : 0;
     x.step = BM;
-    if (tiles == 0) return x;
-    const int item = kvh * row_tiles + node / Z.NB, u = before + item * tiles;
-    const int b0 = u / share, b1 = (u + tiles - 1) / share;
-    x.pieces = b1 - b0 + 1;
-    x.first = (size_t)(b0 + items + item) * BM + (node % Z.NB) * G + head_in_group;
     return x;
   }
 };
@@ -529,14 +568,14 @@ int query_map(const void* q, int N, int Hq, int hd, int G, int NB, CUtensorMap* 
 
 template <int HD, int BOX>
 int launch(const CUtensorMap& qm, const CUtensorMap& kvm, const void* v_pool, const Sizes& Z, const int* table, int mb, int page_size, int num_pages,
-           int Hq, float scale_log2, int blocks, int slots, float* part_o, float* part_ml, int* err, cudaStream_t stream) {
+           int N, int Hq, float scale_log2, int blocks, int slots, float* part_o, float* part_ml, int2* records, int* err, cudaStream_t stream) {
   constexpr int HALVES = HD / 64, STAGES = HD <= 64 ? 6 : 3;
   constexpr size_t smem = (size_t)HALVES * 128 * 128 * (1 + 2 * STAGES) + 4 * BM * 4 + 8 * (8 + 4 * STAGES + 1) + 8;
   static_assert(smem <= FZ_MOST_SMEM);
   auto kern = attn_tree_tc_kernel<HD, BOX>;
   FZ_RAISE_SMEM(kern);
   const cudaError_t e = fz_launch(kern, dim3((unsigned)blocks), dim3(THREADS), smem, stream, qm, kvm, (const __nv_bfloat16*)v_pool, Z, table, mb, page_size,
-                                  num_pages, Hq, scale_log2, slots, part_o, part_ml, err);
+                                  num_pages, Hq, scale_log2, N, slots, part_o, part_ml, records, err);
   return e == cudaSuccess ? FZ_OK : (int)e;
 }
 }  // namespace
@@ -549,7 +588,8 @@ FZ_API int fz_attn_tree_tc_check(int Hq, int Hkv, int hd, int page_size) {
   return FZ_OK;
 }
 
-// Slots of the scratch (each 128 * (hd + 2) floats): a step's stretches are fewer than its blocks and items together.
+// Slots of the scratch (each 128 * (hd + 2) floats; behind them 2 * N * Hkv ints): a step's stretches are fewer than its blocks and items
+// together.
 FZ_API long long fz_attn_tree_tc_slots(int N, int S, int Hq, int Hkv) {
   const int NB = BM / (Hq / Hkv);
   const long long tiles = (long long)N / NB + S;
@@ -577,15 +617,16 @@ FZ_API int fz_attn_tree_tc(const void* q, const void* k_pool, const void* v_pool
   const long long slots = fz_attn_tree_tc_slots(N, S, Hq, Hkv);
   if (slots > 2147483647LL) return FZ_TOO_LARGE;
   float* part_ml = part + (size_t)slots * BM * hd;
+  int2* records = (int2*)(part_ml + (size_t)slots * BM * 2);
   const Sizes Z = {seg, S, NB, Hkv, window};
-#define FZ_T(HD_, BOX_) st = launch<HD_, BOX_>(qm, kvm, v_pool, Z, table, mb, page_size, num_pages, Hq, scale_log2, blocks, (int)slots, part, part_ml, err, stream)
+#define FZ_T(HD_, BOX_) st = launch<HD_, BOX_>(qm, kvm, v_pool, Z, table, mb, page_size, num_pages, N, Hq, scale_log2, blocks, (int)slots, part, part_ml, records, err, stream)
   if (hd == 64 && box == 8) FZ_T(64, 8);
   else if (hd == 64) FZ_T(64, 16);
   else if (box == 8) FZ_T(128, 8);
   else FZ_T(128, 16);
 #undef FZ_T
   if (st != FZ_OK) return st;
-  const Stretches P = {part, part_ml, Z, blocks, Hq};
+  const Stretches P = {part, part_ml, records, NB, Hkv, window, (int)slots};
   const TreeArgs R = {pos, seq_row, seg, ancestors, table, S, words, mb, page_stride, page_size, num_pages, N, Hq, Hkv, hd, scale_log2, window, err};
   return launch_merge<__nv_bfloat16>((const __nv_bfloat16*)q, (const __nv_bfloat16*)k_pool, (const __nv_bfloat16*)v_pool, (__nv_bfloat16*)out, P, R, stream);
 }

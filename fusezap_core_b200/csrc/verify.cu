@@ -296,7 +296,7 @@ verify_stats_kernel(const float* __restrict__ logits, const float* __restrict__ 
   const int row = blockIdx.x, slices = gridDim.y;
   int s = -1, row0 = 0, n = 0;
   for (int s0 = 0; s0 < S && s < 0; s0 += 32) {
-    const int2 sg = s0 + lane < S ? *(const int2*)(seg + 4 * (s0 + lane)) : make_int2(0, 0);
+    const int2 sg = s0 + lane < S ? make_int2(seg[4 * (s0 + lane)], seg[4 * (s0 + lane) + 1]) : make_int2(0, 0);
     const unsigned hit = __ballot_sync(0xffffffffu, row >= sg.x && row - sg.x < sg.y);
     if (hit) {
       const int who = __ffs(hit) - 1;
@@ -767,7 +767,7 @@ FZ_API int fz_verify_tree(const float* logits, const float* draft, const float* 
   static_assert(sizeof(Found) == 24, "what callers size the scratch by");
   if (S <= 0) return FZ_OK;
   if (V <= 0 || N < 0 || slices < 0 || slices > MAX_SLICES || (slices > 0 && !scratch)) return FZ_BAD_SHAPE;
-  if ((uintptr_t)scratch & 7 || (uintptr_t)seg & 15) return FZ_BAD_ALIGNMENT;
+  if ((uintptr_t)scratch & 7) return FZ_BAD_ALIGNMENT;
   if ((long long)S * 16 > 2147483647LL) return FZ_TOO_LARGE;
   Found* stats = slices > 0 ? (Found*)scratch : nullptr;
   if (stats && N > 0) {

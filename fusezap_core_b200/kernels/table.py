@@ -857,7 +857,7 @@ class CudaOps(Ops):
                 self.drafts_tc.fz_attn_tree_tc_check(num_heads, num_kv_heads, head_dim, cache.page_size) == 0 and \
                 page_stride == 2 * num_kv_heads * cache.page_size * head_dim and v.data_ptr() - k.data_ptr() == page_stride:
             slots = self.drafts_tc.fz_attn_tree_tc_slots(n, segments, num_heads, num_kv_heads)
-            part = torch.empty(slots * 128 * (head_dim + 2), dtype=torch.float32, device=self.device)
+            part = torch.empty(slots * 128 * (head_dim + 2) + 2 * n * num_kv_heads, dtype=torch.float32, device=self.device)
             self._launch(self.drafts_tc.fz_attn_tree_tc, "tree_attention (tensor cores)",
                          (_p(q), _p(k), _p(v), _p(meta.pos), _p(meta.seq_row), _p(seg), segments, _p(bits), bits.shape[1], _p(table), pages,
                           c_longlong(page_stride), cache.page_size, num_pages, _p(out), n, num_heads, num_kv_heads, head_dim, c_float(scale),

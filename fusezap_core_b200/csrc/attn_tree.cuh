@@ -89,7 +89,7 @@ constexpr int MERGE_WARPS = 8;
 // fetching its instructions, hence short loops instead of unrolled ones, and no spills: local memory is as far away as the rest (a
 // warp with four dimensions a lane and eight places at a time took 15 us from start to end).
 template <typename T, typename Where, int LANES, int D>
-__global__ void __launch_bounds__(32 * MERGE_WARPS)
+__global__ void __launch_bounds__(32 * MERGE_WARPS, D == 8 ? 4 : 2)
 attn_tree_merge_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, const T* __restrict__ v_pool, T* __restrict__ out,
                        const Where where, const TreeArgs A) {
   constexpr int VEC = 16 / sizeof(T), NC = D / VEC, GROUPS = 32 / LANES;
@@ -103,15 +103,15 @@ attn_tree_merge_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, co
   unsigned bits = (unsigned)A.ancestors[(size_t)n * A.words];
   const int2 record = where.early(n, kvh);
   const int pos = A.window > 0 ? A.pos[n] : 0;
-  float qv[D], o[D];
+  uint4 qr[NC];
+  float o[D];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int d = VEC * (gl + LANES * c);
-    float x[VEC];
-    as_floats(d < A.hd ? *(const uint4*)(q + at + d) : make_uint4(0u, 0u, 0u, 0u), x);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) qv[c * VEC + i] = x[i] * A.scale_log2, o[c * VEC + i] = 0.f;
+    qr[c] = d < A.hd ? *(const uint4*)(q + at + d) : make_uint4(0u, 0u, 0u, 0u);
   }
+#pragma unroll
+  for (int i = 0; i < D; ++i) o[i] = 0.f;
   const bool named = s >= 0 && s < A.S;
   const int row0 = named ? A.seg[4 * s] : 0, nodes = named ? A.seg[4 * s + 1] : 0, start = named ? A.seg[4 * s + 2] : 0;
   if (!named || n < row0 || n - row0 >= nodes) {      // a padding row
@@ -187,13 +187,15 @@ attn_tree_merge_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, co
     float sc = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      float x[VEC];
+      float x[VEC], y[VEC];
       as_floats(kr[c], x);
+      as_floats(qr[c], y);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sc = fmaf(qv[c * VEC + i], x[i], sc);
+      for (int i = 0; i < VEC; ++i) sc = fmaf(y[i], x[i], sc);
     }
 #pragma unroll
     for (int x = LANES / 2; x > 0; x >>= 1) sc += __shfl_xor_sync(0xffffffffu, sc, x);
+    sc *= A.scale_log2;
     if (!seen) continue;
     const float mn = fmaxf(m, sc), mu = mn == -INFINITY ? 0.f : mn, corr = exp2f(m - mu), e = exp2f(sc - mu);
     m = mn;
@@ -238,7 +240,11 @@ template <typename T, typename Where>
 int launch_merge(const T* q, const T* k, const T* v, T* out, const Where& where, const TreeArgs& A, cudaStream_t stream) {
   const dim3 grid((unsigned)A.N, (unsigned)((A.Hq + MERGE_WARPS - 1) / MERGE_WARPS)), block(32 * MERGE_WARPS);
   cudaError_t e;
+  // Head size 128: groups of 8 lanes while the rows' warps find room at once (two blocks per SM with 16 dimensions a lane), of 16 lanes where
+  // twice as many warps on an SM make up for half as many loads each
+  const bool many = (long long)A.N * A.Hq > 148LL * 2 * MERGE_WARPS;
   if (A.hd <= 64) e = fz_launch(attn_tree_merge_kernel<T, Where, 8, 8>, grid, block, 0, stream, q, k, v, out, where, A);
+  else if (A.hd <= 128 && many) e = fz_launch(attn_tree_merge_kernel<T, Where, 16, 8>, grid, block, 0, stream, q, k, v, out, where, A);
   else if (A.hd <= 128) e = fz_launch(attn_tree_merge_kernel<T, Where, 8, 16>, grid, block, 0, stream, q, k, v, out, where, A);
   else if (A.hd <= 256) e = fz_launch(attn_tree_merge_kernel<T, Where, 16, 16>, grid, block, 0, stream, q, k, v, out, where, A);
   else e = fz_launch(attn_tree_merge_kernel<T, Where, 32, 16>, grid, block, 0, stream, q, k, v, out, where, A);

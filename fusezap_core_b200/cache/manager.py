@@ -6,7 +6,8 @@ Cache slots (one per schedule entry that writes a cache) with the same need (kv 
 same page in every slot of the group (the reference keeps one table for all layers: fusezap/serve/kv_cache.py:436-460).
 A full group keeps every page until the request ends; a window group gives back the pages that lie wholly before the
 window of the request's next position (their table entries become -1) as soon as `commit` says how far the request is
-computed. Position p of a request lives in page `table[p // page_size]` at offset `p % page_size`
+computed. A request can be continued several ways (`fork`): full pages are then shared, and given back by each holder; `trim` gives back the
+pages behind what is computed, where drafted tokens lay that were not kept. Position p of a request lives in page `table[p // page_size]` at offset `p % page_size`
 (kv_cache.py:452-455).
 
 Beside the pages there are `StateSlots`: per-request state of fixed size for mixers that declare some (the dense decoder
@@ -121,6 +122,42 @@ class KVGroup:
         if gone.size:
             self.allocator.free(gone.tolist())
             head[:] = -1
+
+    def trim(self, req: Hashable, n_tokens: int) -> None:
+        """Gives back the pages that hold none of the first n_tokens places."""
+        row, keep = self.rows.get(req), -(-n_tokens // self.page_size)
+        n = self.lens.get(req, 0)
+        if row is None or n <= keep:
+            return
+        tail = row[keep:n]
+        self.allocator.free(tail[tail >= 0].tolist())
+        tail[:] = -1
+        self.lens[req] = keep
+
+    def fork_pages(self, req: Hashable, computed: int) -> tuple[int, int]:
+        """(pages of `req` that a fork shares, pages it gets of its own): those full of computed tokens, and the one that is not."""
+        row, full = self.rows.get(req), computed // self.page_size
+        held = 0 if row is None else int((row[: min(full, self.lens[req])] >= 0).sum())
+        return held, 1 if row is not None and computed % self.page_size and self.lens[req] > full and row[full] >= 0 else 0
+
+    def fork(self, req: Hashable, new: Hashable, computed: int) -> list[tuple[int, int]]:
+        """Gives `new` a block table over the first `computed` places of `req`: the full pages are shared, the last, which both go on
+        writing, is a page of its own. Returns what is to be copied: [(page of req, page of new)], one or none."""
+        old, full = self.rows.get(req), computed // self.page_size
+        if old is None:
+            return []
+        row = np.full(old.shape[0], -1, dtype=np.int32)
+        n = min(full, self.lens[req])
+        row[:n] = old[:n]
+        copies = []
+        if self.fork_pages(req, computed)[1]:
+            row[full] = self.allocator.allocate(1)[0]
+            copies = [(int(old[full]), int(row[full]))]
+            n = full + 1
+        shared = row[:full]
+        self.allocator.share(shared[shared >= 0].tolist())
+        self.rows[new], self.lens[new] = row, n
+        return copies
 
     def free(self, req: Hashable) -> None:
         row = self.rows.pop(req, None)
@@ -251,6 +288,35 @@ class CacheManager:
         for g in self.groups:
             g.release_before(req, n_computed)
 
+    def trim(self, req: Hashable) -> None:
+        """Gives back the pages behind what `commit` said is computed (a tree's nodes that were not kept)."""
+        if req not in self.computed:
+            raise KeyError(f"request {req!r} holds nothing")
+        for g in self.groups:
+            g.trim(req, self.computed[req])
+
+    def can_fork(self, req: Hashable) -> bool:
+        """Whether `fork(req, ..)` finds the pages (and the state slot) it needs."""
+        if self.has_state and req in self.states.owner and not self.states.num_free:
+            return False
+        c = self.computed[req]
+        return all(g.fork_pages(req, c)[1] <= g.allocator.num_free for g in self.groups)
+
+    def fork(self, req: Hashable, new: Hashable) -> tuple[list[list[tuple[int, int]]], tuple[int, int] | None]:
+        """A second request `new` over what `req` has computed: the pages that are full are shared between the two, the last one and
+        the state are to be copied by the caller before either runs again. Returns (per group [(page, page of new)], (state slot, slot of new)
+        or None)."""
+        if req not in self.computed:
+            raise KeyError(f"request {req!r} holds nothing")
+        if new in self.computed:
+            raise ValueError(f"request {new!r} holds pages already")
+        if not self.can_fork(req):
+            raise OutOfPages(f"no page or state slot free to fork request {req!r}; free pages: {[g.allocator.num_free for g in self.groups]}")
+        c = self.computed[new] = self.computed[req]
+        copies = [g.fork(req, new, c) for g in self.groups]
+        slot = self.states.owner.get(req)
+        return copies, None if slot is None else (slot, self.states.acquire(new))
+
     def free(self, req: Hashable) -> None:
         for g in self.groups:
             g.free(req)
@@ -295,18 +361,20 @@ class CacheManager:
         return self.states.owner.get(req, -1)
 
     def check(self) -> None:
-        """Invariants: allocators consistent, and every held page is in exactly one table of its group."""
+        """Invariants: allocators consistent, and every held page is in as many tables of its group as it has holders (one, unless
+        requests were forked)."""
         for g in self.groups:
             g.allocator.check()
-            seen: set[int] = set()
+            seen: dict[int, int] = {}
             for req, t in g.tables.items():
                 assert all(p >= 0 for p in t[g.first_live_page(self.computed.get(req, 0)):]), f"{req!r} lacks a live page"
                 kept = min(len(t), -(-getattr(g.need, "keep_first", 0) // g.page_size))
                 assert all(p >= 0 for p in t[:kept]), f"{req!r} lost a page of its kept first tokens"
                 for p in t:
                     if p >= 0:
-                        assert p not in seen, f"page {p} is in two block tables"
-                        seen.add(p)
+                        seen[p] = seen.get(p, 0) + 1
+            for p, n in seen.items():
+                assert n == g.allocator.holders(p), f"page {p} is in {n} block tables and has {g.allocator.holders(p)} holders"
             assert len(seen) == g.num_pages - g.allocator.num_free, \
                 f"{g.num_pages - g.allocator.num_free} pages held, {len(seen)} in tables"
         assert len(set(self.states.owner.values())) == len(self.states.owner), "a state slot has two owners"

@@ -20,11 +20,13 @@ using namespace fztree;
 constexpr int THREADS = 256;
 
 // The context of one request as the kernels cut it: places [first, end), in pieces of `piece` from `first` on. first: the
-// first place that any row sees, rounded down to a multiple of 64. Up to 32 pieces of at least 256 places: the pieces' results are
-// written and read once more, (hd + 2) floats a row against 2 hd values a key.
+// first place that any row sees, rounded down to a multiple of 64. Up to 32 pieces of at least 64 places (a key tile): the pieces' results
+// are written and read once more, (hd + 2) floats a row against 2 hd values a key, but a step of short contexts has few blocks otherwise (4
+// requests of 13 nodes behind 500 places, 14 heads of 64 over 2: 46 us with pieces of 256 and tiles of 64 rows, 19 with pieces of 64 and
+// tiles of 16).
 __host__ __device__ __forceinline__ int piece_length(int places) {
   const int p = ((places + 31) / 32 + 63) / 64 * 64;
-  return p < 256 ? 256 : p;
+  return p < 64 ? 64 : p;
 }
 
 struct Args {
@@ -249,8 +251,8 @@ int launch_context(const void* q, const void* k, const void* v, const Args& A, i
 template <typename T>
 int context(const void* q, const void* k, const void* v, const Args& A, cudaStream_t stream) {
   const int G = A.Hq / A.Hkv;
-  // rows a request has per kv head, on average: tiles of 16 rows where they fill no more than one of those
-  const bool few = (long long)A.N * G <= 16LL * A.S;
+  // tiles of 16 rows where a request's rows fill no more than one of those on average, or where larger ones would be too few blocks
+  const bool few = (long long)A.N * G <= 16LL * A.S || ((long long)A.N * G / 64 + A.S) * A.Hkv * A.pieces < 2 * 148;
   auto tiles = [&](int RM) {
     const int NB = RM / (G < RM ? G : RM);
     const long long t = (long long)A.N / NB + A.S;
@@ -273,7 +275,7 @@ FZ_API int fz_attn_tree_pieces(int max_context, int window) {
   int places = max_context > 0 ? max_context : 1;
   if (window > 0 && places > window + 64) places = window + 64;
   // (a shorter context may be cut into as many pieces: 32 of its own length)
-  const int most = (places + 255) / 256;
+  const int most = (places + 63) / 64;
   return most < 32 ? most : 32;
 }
 

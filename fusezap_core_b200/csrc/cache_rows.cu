@@ -5,7 +5,7 @@
 #include "common.cuh"
 
 namespace {
-constexpr int KEEP_THREADS = 128;
+constexpr int KEEP_THREADS = 256;
 constexpr int KEEP_NODES = 1024;      // kept rows of a request at most
 
 template <typename V>
@@ -16,9 +16,11 @@ struct Pool {
 };
 
 // The kept nodes of a request's tree: place start + path[k] -> start + k. path rises, so path[k] >= k and a place is read
-// before or at the time it is written if the kept nodes go in order: a thread owns one vector of every row (of one slot and part)
-// and takes eight rows at a time, loads first, so eight loads are in flight. Grid (slots x parts x vectors of a row, requests).
-template <typename V>
+// before or at the time it is written if the kept nodes go in order: a thread owns PER vectors of every row (each of one slot and part)
+// and takes a few rows at a time, loads first, so eight loads are in flight. Grid (slots x parts x vectors of a row, requests). Bound by the
+// chain count -> path -> page -> row in every block, so blocks are few where there is enough to do: PER = 4 (64 requests of up to
+// 16 nodes, 32 layers of 8 heads of 128: 12 us with 4,096 blocks, 11 with 512 and all of them on the chip at once).
+template <typename V, int PER>
 __global__ void __launch_bounds__(KEEP_THREADS)
 keep_rows_kernel(const Pool<V> P, const int* __restrict__ table, int S, int mb, const int* __restrict__ seg,
                  const int* __restrict__ path, const int* __restrict__ count, int N, int* err) {
@@ -55,22 +57,30 @@ keep_rows_kernel(const Pool<V> P, const int* __restrict__ table, int S, int mb, 
     if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(err, bad);
     return;
   }
-  const long long e = (long long)blockIdx.x * KEEP_THREADS + threadIdx.x;
   const int per_slot = P.parts * P.width;
-  if (e >= (long long)P.slots * per_slot) return;
-  const int slot = (int)(e / per_slot), in_slot = (int)(e - (long long)slot * per_slot);
-  const int part = in_slot / P.width, v = in_slot - part * P.width;
-  V* base = P.data + slot * P.slot_stride + part * P.part_stride + v;
+  V* base[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const long long e = ((long long)blockIdx.x * PER + i) * KEEP_THREADS + threadIdx.x;
+    const int slot = (int)(e / per_slot), in_slot = (int)(e - (long long)slot * per_slot);
+    const int part = in_slot / P.width, v = in_slot - part * P.width;
+    base[i] = slot < P.slots ? P.data + slot * P.slot_stride + part * P.part_stride + v : nullptr;
+  }
   int k = 0;
   while (k < kept && s_from[k] == s_to[k]) ++k;      // (the root, and a chain that stands: already there)
-  for (; k < kept; k += 8) {
-    V x[8];
+  constexpr int ROWS = 8 / PER;
+  for (; k < kept; k += ROWS) {
+    V x[ROWS][PER];
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (k + u < kept) x[u] = base[s_from[k + u]];
+    for (int u = 0; u < ROWS; ++u)
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (k + u < kept) base[s_to[k + u]] = x[u];
+      for (int i = 0; i < PER; ++i)
+        if (k + u < kept && base[i]) x[u][i] = base[i][s_from[k + u]];
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (k + u < kept && base[i]) base[i][s_to[k + u]] = x[u][i];
   }
 }
 
@@ -109,9 +119,13 @@ int keep(void* pool, int slots, int num_pages, int parts, int page_size, int row
   P.page_stride = parts * P.part_stride;
   P.slot_stride = num_pages * P.page_stride;
   P.slots = slots, P.parts = parts, P.page_size = page_size, P.num_pages = num_pages;
-  const long long blocks = ((long long)slots * parts * P.width + KEEP_THREADS - 1) / KEEP_THREADS;
+  const long long vectors = (long long)slots * parts * P.width;
+  const int per = vectors * S >= 4LL * KEEP_THREADS * 148 ? 4 : 1;
+  const long long blocks = (vectors + per * KEEP_THREADS - 1) / (per * KEEP_THREADS);
   if (blocks > 2147483647LL || (long long)parts * P.width > 2147483647LL) return FZ_TOO_LARGE;
-  const cudaError_t e = fz_launch(keep_rows_kernel<V>, dim3((unsigned)blocks, (unsigned)S), dim3(KEEP_THREADS), 0, stream, P, table, S, mb, seg, path, count, N, err);
+  const dim3 grid((unsigned)blocks, (unsigned)S);
+  const cudaError_t e = per == 4 ? fz_launch(keep_rows_kernel<V, 4>, grid, dim3(KEEP_THREADS), 0, stream, P, table, S, mb, seg, path, count, N, err)
+                                 : fz_launch(keep_rows_kernel<V, 1>, grid, dim3(KEEP_THREADS), 0, stream, P, table, S, mb, seg, path, count, N, err);
   return e == cudaSuccess ? FZ_OK : (int)e;
 }
 

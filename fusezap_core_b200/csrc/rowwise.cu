@@ -554,7 +554,7 @@ FZ_API int fz_normed_sum(const float* t0, const float* t1, const float* t2, cons
 // angle of the row's position; q goes to q_out, k and v to the row's slot of the paged pool.
 template <typename T>
 __global__ void rope_kv_write_kernel(const float* __restrict__ qkv, const float* __restrict__ cos_t,
-                                     const float* __restrict__ sin_t, const int* __restrict__ pos,
+                                     const float* __restrict__ sin_t, const int* __restrict__ pos, const int* __restrict__ place,
                                      const int* __restrict__ seq_row, const int* __restrict__ table, int mb,
                                      T* __restrict__ k_pool, T* __restrict__ v_pool, long long page_stride,
                                      int page_size, int write, T* __restrict__ q_out, int Hq, int Hkv, int hd,
@@ -580,11 +580,12 @@ __global__ void rope_kv_write_kernel(const float* __restrict__ qkv, const float*
   const float* sr = sin_t + (size_t)p * half;
   long long slot_base = -1;
   if (write) {
-    const int page = table[(size_t)row * mb + p / page_size];
+    const int at = place ? place[n] : p;      // (drafted trees: the row's place in the cache is not its position)
+    const int page = at >= 0 && at / page_size < mb ? table[(size_t)row * mb + at / page_size] : -1;
     if (page < 0) {
       if (threadIdx.x == 0) atomicOr(err, FZ_ERR_NO_PAGE);
     } else {
-      slot_base = (long long)page * page_stride + (long long)(p % page_size) * hd;
+      slot_base = (long long)page * page_stride + (long long)(at % page_size) * hd;
     }
   }
   const long long head_stride = (long long)page_size * hd;
@@ -623,7 +624,7 @@ __device__ __forceinline__ void store4(__nv_bfloat16* d, float a, float b, float
 
 template <typename T>
 __global__ void rope_kv_write_vec_kernel(const float* __restrict__ qkv, const float* __restrict__ cos_t,
-                                         const float* __restrict__ sin_t, const int* __restrict__ pos,
+                                         const float* __restrict__ sin_t, const int* __restrict__ pos, const int* __restrict__ place,
                                          const int* __restrict__ seq_row, const int* __restrict__ table, int mb,
                                          T* __restrict__ k_pool, T* __restrict__ v_pool, long long page_stride,
                                          int page_size, int write, T* __restrict__ q_out, int Hq, int Hkv, int hd,
@@ -646,9 +647,10 @@ __global__ void rope_kv_write_vec_kernel(const float* __restrict__ qkv, const fl
       sn = *(const float4*)(sin_t + (size_t)p * half + j);
     }
     if (write && head >= Hq) {
-      const int page = table[(size_t)row * mb + p / page_size];
+      const int at = place ? place[n] : p;
+      const int page = at >= 0 && at / page_size < mb ? table[(size_t)row * mb + at / page_size] : -1;
       no_page = page < 0;
-      if (!no_page) slot_base = (long long)page * page_stride + (long long)(p % page_size) * hd;
+      if (!no_page) slot_base = (long long)page * page_stride + (long long)(at % page_size) * hd;
     }
   }
   fz_grid_wait();
@@ -689,7 +691,8 @@ __global__ void rope_kv_write_vec_kernel(const float* __restrict__ qkv, const fl
   }
 }
 
-FZ_API int fz_rope_kv_write(const float* qkv, const float* cos_t, const float* sin_t, const int* pos,
+// place: null, or the rows' places in the cache where they are not their positions.
+FZ_API int fz_rope_kv_write_at(const float* qkv, const float* cos_t, const float* sin_t, const int* pos, const int* place,
                             const int* seq_row, const int* table, int mb, void* k_pool, void* v_pool,
                             long long page_stride, int page_size, int write, void* q_out, int dtype, int N, int Hq,
                             int Hkv, int hd, int max_len, int* err, cudaStream_t stream) {
@@ -703,26 +706,34 @@ FZ_API int fz_rope_kv_write(const float* qkv, const float* cos_t, const float* s
     const int threads = items < 256 ? ((items + 31) / 32) * 32 : 256;
     dim3 grid(N, (items + threads - 1) / threads);
     if (dtype == FZ_F32)
-      fz_launch(rope_kv_write_vec_kernel<float>, grid, dim3(threads), 0, stream, qkv, cos_t, sin_t, pos, seq_row, table, mb,
+      fz_launch(rope_kv_write_vec_kernel<float>, grid, dim3(threads), 0, stream, qkv, cos_t, sin_t, pos, place, seq_row, table, mb,
                 (float*)k_pool, (float*)v_pool, page_stride, page_size, write, (float*)q_out, Hq, Hkv, hd, max_len, err);
     else
-      fz_launch(rope_kv_write_vec_kernel<__nv_bfloat16>, grid, dim3(threads), 0, stream, qkv, cos_t, sin_t, pos, seq_row,
+      fz_launch(rope_kv_write_vec_kernel<__nv_bfloat16>, grid, dim3(threads), 0, stream, qkv, cos_t, sin_t, pos, place, seq_row,
                 table, mb, (__nv_bfloat16*)k_pool, (__nv_bfloat16*)v_pool, page_stride, page_size, write,
                 (__nv_bfloat16*)q_out, Hq, Hkv, hd, max_len, err);
     FZ_LAUNCH_CHECK();
     return FZ_OK;
   }
   if (dtype == FZ_F32)
-    fz_launch(rope_kv_write_kernel<float>, dim3(N), dim3(256), 0, stream, qkv, cos_t, sin_t, pos, seq_row, table, mb,
+    fz_launch(rope_kv_write_kernel<float>, dim3(N), dim3(256), 0, stream, qkv, cos_t, sin_t, pos, place, seq_row, table, mb,
               (float*)k_pool, (float*)v_pool, page_stride, page_size, write, (float*)q_out, Hq, Hkv, hd, max_len, err);
   else if (dtype == FZ_BF16)
-    fz_launch(rope_kv_write_kernel<__nv_bfloat16>, dim3(N), dim3(256), 0, stream, qkv, cos_t, sin_t, pos, seq_row, table,
+    fz_launch(rope_kv_write_kernel<__nv_bfloat16>, dim3(N), dim3(256), 0, stream, qkv, cos_t, sin_t, pos, place, seq_row, table,
               mb, (__nv_bfloat16*)k_pool, (__nv_bfloat16*)v_pool, page_stride, page_size, write, (__nv_bfloat16*)q_out,
               Hq, Hkv, hd, max_len, err);
   else
     return FZ_BAD_DTYPE;
   FZ_LAUNCH_CHECK();
   return FZ_OK;
+}
+
+FZ_API int fz_rope_kv_write(const float* qkv, const float* cos_t, const float* sin_t, const int* pos,
+                            const int* seq_row, const int* table, int mb, void* k_pool, void* v_pool,
+                            long long page_stride, int page_size, int write, void* q_out, int dtype, int N, int Hq,
+                            int Hkv, int hd, int max_len, int* err, cudaStream_t stream) {
+  return fz_rope_kv_write_at(qkv, cos_t, sin_t, pos, nullptr, seq_row, table, mb, k_pool, v_pool, page_stride, page_size, write, q_out, dtype,
+                             N, Hq, Hkv, hd, max_len, err, stream);
 }
 
 // ------------------------------------------------------------------------------------------------ SwiGLU

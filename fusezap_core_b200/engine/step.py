@@ -13,6 +13,19 @@ wanted (-1: none), a segment is (first row, rows, first position, state slot) of
 to the kernel table: the parts of the model say what kinds of step data their kernels need (`Part.step_needs()`), the
 table says how many int32 it wants for them (`Ops.step_extra_ints`) and fills them when the step is packed
 (`Ops.plan_step`), before the one copy. The step function itself knows nothing of any kernel's tiling.
+
+A step can also run drafted trees (`Portion.parents`, runners made with `max_tree_nodes`): a request's tokens are then the nodes of
+a tree below its last token, node j lies in place (computed + j) of the cache while its position is that of its depth, and a node sees the
+computed tokens and its ancestors. Behind the block stand place[N], parents[N] and the ancestors' bits of every row. What
+`StepRunner.verify` lets stand, `StepRunner.keep` moves together in the cache:
+
+  runner = StepRunner(model, cache, max_rows=256, max_tree_nodes=32)
+  portions = [Portion("a", [last, x, y, z], range(4), parents=[-1, 0, 0, 1])]
+  starts = runner.prepare(portions)
+  logits = runner.forward()
+  path, count, next_ids = runner.verify(logits, temperature, uniform, draft)
+  runner.keep(path, count)                                # the cache as if only the kept tokens had been run
+  runner.commit_kept(portions, starts, count.tolist())    # the host's books
 """
 from __future__ import annotations
 from dataclasses import dataclass, field
@@ -25,6 +38,7 @@ from ..cache import CacheManager
 from ..parts import LayerCache, PendingSum
 from .model import DecoderModel
 
+MAX_TREE_NODES = 1024      # of a drafted tree (what `Ops.verify_tree` takes)
 
 
 @dataclass
@@ -35,6 +49,29 @@ class Portion:
     want: Sequence[int] = ()
     src: int = -1      # >= 0 (single-token portions only): the token is the id the previous step chose for its wanted
                        # row `src`, taken on the device; `tokens` then only gives the count
+    parents: Sequence[int] | None = None      # a drafted tree: the parent of every token among these tokens (the first, the
+                       # request's last token: -1; every other's stands before it); a step's other portions are then chains
+
+
+def check_tree(portion: Portion, max_nodes: int) -> Sequence[int]:
+    """The parents of a portion's tokens in a step of trees (a portion without any is a chain); refuses what is no tree."""
+    n = len(portion.tokens)
+    if n > max_nodes:
+        raise ValueError(f"request {portion.req!r}: {n} tokens exceed max_tree_nodes ({max_nodes})")
+    if portion.parents is None:
+        return range(-1, n - 1)
+    tree = [int(x) for x in portion.parents]
+    if len(tree) != n or tree[0] != -1 or any(not 0 <= x < j for j, x in enumerate(tree) if j):
+        raise ValueError(f"request {portion.req!r}: parents {tree} are no tree over its {n} tokens (the first has parent -1, the others one before them)")
+    return tree
+
+
+def tree_depth(parents: Sequence[int]) -> int:
+    """Nodes on the longest way down."""
+    depth = []
+    for x in parents:
+        depth.append(depth[x] + 1 if x >= 0 else 1)
+    return max(depth)
 
 
 @dataclass
@@ -85,7 +122,7 @@ class Workspace:
 class StepMeta:
     """The step's int32 metadata: a pinned host block and its device copy with fixed offsets for a given capacity."""
     def __init__(self, device: torch.device, max_rows: int, max_wanted: int, max_segments: int, num_groups: int,
-                 pages_per_request: int, extra_ints: int = 0):
+                 pages_per_request: int, extra_ints: int = 0, max_tree_nodes: int = 0):
         self.device = device
         self.max_rows, self.max_wanted, self.max_segments = max_rows, max_wanted, max_segments
         self.num_groups, self.mb = num_groups, pages_per_request
@@ -99,6 +136,11 @@ class StepMeta:
         self.o_tab, o = o, o + num_groups * max_segments * pages_per_request
         self.extra_ints = extra_ints
         self.o_extra, o = o, o + extra_ints
+        # steps of drafted trees: places, parents and ancestors of the rows
+        self.max_tree_nodes, self.tree_words = max_tree_nodes, -(-max_tree_nodes // 32)
+        self.o_place, o = o, o + (max_rows if max_tree_nodes else 0)
+        self.o_parents, o = o, o + (max_rows if max_tree_nodes else 0)
+        self.o_ancestors, o = o, o + max_rows * self.tree_words
         self.size = o
         # a ring of pinned host blocks: a block is rewritten only after the copy that read it has finished
         pin = device.type == "cuda"
@@ -116,6 +158,7 @@ class StepMeta:
         self.max_context = 0      # the longest context (position + 1) among the step's rows
         self.page_size = 0        # of the cache the step was packed against
         self.max_portion = 0      # the longest portion
+        self.tree = False         # the step's portions are drafted trees
         self.plan = None          # whatever the kernel table's `plan_step` keeps about this step (launch sizes and the like)
         self.latent_extra = 0     # kernel table: how many blocks beyond rows x heads / 64 the latent attention launches
 
@@ -144,6 +187,15 @@ class StepMeta:
     def extra(self) -> torch.Tensor: return self.dev[self.o_extra: self.o_extra + self.extra_ints]
     @property
     def extra_host(self) -> np.ndarray: return self.np[self.o_extra: self.o_extra + self.extra_ints]
+    @property
+    def place(self) -> torch.Tensor | None: return self._view(self.o_place, self.n_rows) if self.tree else None
+    @property
+    def parents(self) -> torch.Tensor | None: return self._view(self.o_parents, self.n_rows) if self.tree else None
+    @property
+    def ancestors(self) -> torch.Tensor | None:
+        if not self.tree:
+            return None
+        return self.dev[self.o_ancestors: self.o_ancestors + self.n_rows * self.tree_words].view(self.n_rows, self.tree_words)
     def table(self, group: int) -> torch.Tensor:
         n = self.max_segments * self.mb
         return self._view(self.o_tab + group * n, n, self.mb)
@@ -181,6 +233,13 @@ class StepMeta:
         seg[len(portions):] = 0
         self.segments = []
         self.page_size = cache.page_size
+        self.tree = any(p.parents is not None for p in portions)
+        if self.tree and not self.max_tree_nodes:
+            raise ValueError("drafted trees need a runner made with max_tree_nodes")
+        if self.tree:
+            place, parents = (a[o: o + n_rows] for o in (self.o_place, self.o_parents))
+            bits = a[self.o_ancestors: self.o_ancestors + n_rows * self.tree_words].reshape(n_rows, self.tree_words).view(np.uint32)
+            place[n:], parents[n:], bits[n:] = 0, -1, 0
         at = w = 0
         self.max_context = self.max_portion = 0
         for s, (p, start) in enumerate(zip(portions, starts)):
@@ -191,6 +250,17 @@ class StepMeta:
                     raise ValueError(f"request {p.req!r}: only a single token can come from the previous step's ids")
                 src[at] = p.src
             pos[at: at + k] = np.arange(start, start + k)
+            if self.tree:
+                tree = check_tree(p, self.max_tree_nodes)
+                place[at: at + k] = pos[at: at + k]
+                parents[at: at + k] = tree
+                seen, depth = [1], [start]      # (Python's own integers: a step has few nodes, and numpy calls cost a microsecond each)
+                for j, parent in enumerate(tree):
+                    if j:
+                        seen.append(seen[parent] | 1 << j)
+                        depth.append(depth[parent] + 1)
+                pos[at: at + k] = depth
+                bits[at: at + k] = np.frombuffer(b"".join(m.to_bytes(4 * self.tree_words, "little") for m in seen), np.uint32).reshape(k, -1)
             row[at: at + k] = s
             for j in p.want:
                 if not 0 <= j < k:
@@ -237,16 +307,19 @@ class StepContext:
 class StepRunner:
     """Owns the step's metadata and scratch buffers and runs the model over them."""
     def __init__(self, model: DecoderModel, cache: CacheManager, max_rows: int, max_wanted: int | None = None,
-                 max_segments: int | None = None):
+                 max_segments: int | None = None, max_tree_nodes: int = 0):
+        """max_tree_nodes: the most nodes of a drafted tree (0: the runner takes none)."""
         self.model, self.cache, self.ops = model, cache, model.ops
         dev = model.device
         self.max_rows = max_rows
+        if max_tree_nodes:
+            self._check_takes_trees(max_tree_nodes)
         # what kinds of step data the mixers' kernels need, and how many int32 the kernel table wants for them
         self.needs = tuple(sorted({k for part in model.parts() for k in getattr(part, "step_needs", tuple)()}))
         max_segments = max_segments or max_rows
         extra = getattr(self.ops, "step_extra_ints", lambda *a: 0)(self.needs, max_rows, max_segments)
         self.meta = StepMeta(dev, max_rows, max_wanted or max_rows, max_segments, len(cache.groups),
-                             cache.max_pages_per_request, extra)
+                             cache.max_pages_per_request, extra, max_tree_nodes)
         self.ws = Workspace(dev, max_rows)
         self.ctx = StepContext(self.ops, self.ws, self.meta, model.positions, model)
         self.prev_ids: torch.Tensor | None = None     # device int32: the ids the previous step chose (see Portion.src)
@@ -262,6 +335,17 @@ class StepRunner:
             self.layer_caches.append(lc)
         self.keep_embedding = any(e.add_embedding for e in model.spec.schedule)
         self.embed_state = {name: t for (entry, name), t in cache.states.tensors.items() if entry == -1}
+
+    def _check_takes_trees(self, max_tree_nodes: int) -> None:
+        """Refuses trees where a part would take a step's rows for consecutive tokens."""
+        model = self.model
+        if not 0 < max_tree_nodes <= MAX_TREE_NODES:
+            raise ValueError(f"max_tree_nodes is {max_tree_nodes}: 1 to {MAX_TREE_NODES}")
+        wrong = sorted({type(layer.mixer).__name__ for layer in model.layers if not getattr(layer.mixer, "takes_trees", False)})
+        if wrong:
+            raise ValueError(f"drafted trees are not taken by {', '.join(wrong)}")
+        if model.embed_extras or model.state_needs():
+            raise ValueError("drafted trees are not taken by models that keep a state from token to token")
 
     def forward(self, ids_out: torch.Tensor | None = None) -> torch.Tensor | None:
         """Runs the model over the metadata already filled; returns logits (n_wanted, vocab) float32. With `ids_out`
@@ -325,6 +409,7 @@ class StepRunner:
         cache = self.cache
         seen = set()
         starts = []
+        trees = any(p.parents is not None for p in portions)
         for p in portions:
             if p.req in seen:
                 raise ValueError(f"request {p.req!r} appears twice in one step")
@@ -332,17 +417,78 @@ class StepRunner:
                 raise ValueError(f"request {p.req!r} brings no tokens")
             seen.add(p.req)
             start = cache.computed.get(p.req, 0)
+            if trees:
+                self._check_tree(p)
             cache.ensure(p.req, start + len(p.tokens))
             starts.append(start)
         self.meta.fill(cache, portions, starts, pad_rows, pad_wanted, self.ops, self.needs)
         return starts
 
+    def _check_tree(self, portion: Portion) -> None:
+        if not self.meta.max_tree_nodes:
+            raise ValueError("drafted trees need a runner made with max_tree_nodes")
+        if portion.src >= 0:
+            raise ValueError(f"request {portion.req!r}: a tree's tokens are given, not taken from the previous step's ids")
+        tree = check_tree(portion, self.meta.max_tree_nodes)
+        windows = [g.need.window for g in self.cache.groups if g.need.window]
+        if windows:
+            depth, window = tree_depth(tree), min(windows)
+            if depth > window:
+                raise ValueError(f"request {portion.req!r}: a tree {depth} deep exceeds the window of {window}")
+
     def commit(self, portions: Sequence[Portion], starts: Sequence[int]) -> None:
+        if self.meta.tree:
+            raise ValueError("a step of drafted trees is committed by what is kept of it (commit_kept)")
         for p, s in zip(portions, starts):
             self.cache.commit(p.req, s + len(p.tokens))
 
     def run(self, portions: Sequence[Portion]) -> torch.Tensor:
+        if any(p.parents is not None for p in portions):
+            raise ValueError("run: of drafted trees only what stands is computed; see verify, keep and commit_kept")
         starts = self.prepare(portions)
         logits = self.forward()
         self.commit(portions, starts)
         return logits
+
+    # ---- drafted trees: what stands, and the cache afterwards
+    def verify(self, logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.Tensor,
+               draft: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """`Ops.verify_tree` on the step just run, every row of which was wanted: (path (N,), count (S,), next ids (S,)), on the device.
+        temperature (S,) float32 and uniform (N,) float64 on the device, S and N the step's requests and rows; draft: the drafter's
+        logits (N, vocab), or None."""
+        meta = self.meta
+        n, s = meta.n_rows, meta.n_segments
+        if not meta.tree:
+            raise ValueError("verify: the last step had no drafted trees")
+        if logits is None or logits.shape[0] != n or meta.n_wanted != n or not np.array_equal(meta.np[meta.o_sel: meta.o_sel + n], np.arange(n)):
+            raise ValueError("verify: the logits of every row of the step are needed, in order")
+        path, count, ids = (self.ws.get(tag, (k,), torch.int32) for tag, k in (("tree_path", n), ("tree_count", s), ("tree_ids", s)))
+        self.ops.verify_tree(logits, draft, temperature, uniform, meta.tokens, meta.parents, meta.seg[:s], path, count, ids)
+        return path, count, ids
+
+    def keep(self, path: torch.Tensor, count: torch.Tensor) -> None:
+        """The kept nodes' keys and values move together behind what was computed, in every layer's cache (`Ops.keep_rows`)."""
+        meta = self.meta
+        if not meta.tree:
+            raise ValueError("keep: the last step had no drafted trees")
+        for g, group in enumerate(self.cache.groups):
+            self.ops.keep_rows(group.pool, meta.table(g)[: meta.n_segments], meta.seg[: meta.n_segments], path, count)
+
+    def commit_kept(self, portions: Sequence[Portion], starts: Sequence[int], counts: Sequence[int]) -> None:
+        """The host's books after `keep`: each request has so many tokens more, and pages that only held other nodes go back."""
+        for p, s, n in zip(portions, starts, counts):
+            if not 1 <= n <= len(p.tokens):
+                raise ValueError(f"request {p.req!r}: {n} of its {len(p.tokens)} tokens kept")
+            self.cache.commit(p.req, s + int(n))
+            self.cache.trim(p.req)
+
+    def fork(self, req: Hashable, new: Hashable) -> None:
+        """A second request `new` that has computed what `req` has: full pages are shared, the last one and the state are copied."""
+        copies, slots = self.cache.fork(req, new)
+        for group, pairs in zip(self.cache.groups, copies):
+            if pairs:
+                src, dst = torch.tensor(pairs, dtype=torch.int32).T.contiguous().to(self.model.device)
+                self.ops.copy_pages(group.pool, src, dst)
+        if slots is not None:
+            for t in self.cache.states.tensors.values():
+                t[slots[1]].copy_(t[slots[0]])

@@ -410,7 +410,8 @@ class Ops:
                       q_out: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int) -> None:
         """qkv: (N, (Hq + 2 Hkv) * hd) float32, heads [q | k | v]. Rotates q and k heads by the row's position
         (pairs j, j + hd/2, angles from the float32 tables cos/sin (max_len, hd/2)); writes q to q_out (N, Hq*hd) T
-        and, if cache.write, k and v to the row's page slot of cache.keys / cache.values."""
+        and, if cache.write, k and v to the row's page slot of cache.keys / cache.values: that of its position, or, in a step of
+        drafted trees (meta.place int32 (N,), not None), of its place."""
         raise NotImplementedError
 
     def linear_rope_kv_write(self, a: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None, cos: torch.Tensor,

@@ -7,6 +7,7 @@ without a page) set a bit in a device error word instead of faulting; `check_err
 """
 from __future__ import annotations
 import ctypes
+import math
 from ctypes import byref, c_int, c_void_p, c_float, c_longlong
 
 import torch
@@ -119,6 +120,8 @@ class CudaOps(Ops):
         self._index = self.device.index if self.device.index is not None else torch.cuda.current_device()
         self.core = load("fzb200_core")
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._err_ptr = self.err.data_ptr()
+        self._tree_sizes: dict[tuple, bool] = {}
         self._err_host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
         self.launches = 0
         self._stream_handle = None
@@ -223,15 +226,24 @@ class CudaOps(Ops):
     def drafts(self):
         """Drafted tokens: attention of a tree over the cache, the verdict on it, cache rows and pages moved."""
         if self._drafts is None:
-            self._drafts = load("fzb200_drafts")
+            lib = load("fzb200_drafts")
+            P, I, L, F = c_void_p, c_int, c_longlong, c_float
+            lib.fz_attn_tree.argtypes = [P] * 6 + [I, P, I, P, I, L, I, I, P, I, I, I, I, I, F, I, I, P, P, P]
+            lib.fz_verify_tree.argtypes = [P] * 7 + [I] * 3 + [P] * 4 + [I, P, P]
+            lib.fz_keep_rows.argtypes = [P] + [I] * 5 + [P, I, I, P, P, P, I, P, P]
+            lib.fz_copy_pages.argtypes = [P, I, I, L, P, P, I, P, P]
+            self._drafts = lib
         return self._drafts
 
     @property
     def drafts_tc(self):
         """That attention on tensor cores (bfloat16)."""
         if self._drafts_tc is None:
-            self._drafts_tc = load("fzb200_drafts_tc")
-            self._drafts_tc.fz_attn_tree_tc_slots.restype = c_longlong
+            lib = load("fzb200_drafts_tc")
+            P, I, L, F = c_void_p, c_int, c_longlong, c_float
+            lib.fz_attn_tree_tc_slots.restype = L
+            lib.fz_attn_tree_tc.argtypes = [P] * 6 + [I, P, I, P, I, L, I, I, P, I, I, I, I, F, I, P, P, P]
+            self._drafts_tc = lib
         return self._drafts_tc
 
     @property
@@ -344,7 +356,7 @@ class CudaOps(Ops):
             # requests in its rows, so it allows one per row.
             single = all(sg.n == 1 for sg in meta.segments)
             meta.latent_extra = meta.n_rows if single else meta.n_segments
-        if "attention" not in needs:
+        if "attention" not in needs or getattr(meta, "tree", False):      # (a tree's attention plans nothing on the host)
             meta.plan = None
             return
         # tiles are cut along the keys only for the kernel that can leave partial results (tcgen05, pages TMA can box)
@@ -621,8 +633,11 @@ class CudaOps(Ops):
             raise KernelError(f"rope_kv_write: qkv {tuple(qkv.shape)}, q {tuple(q_out.shape)}, cos {tuple(cos.shape)}")
         k, v, page_stride = self._pool(cache, num_kv_heads, head_dim)
         table = meta.table(cache.group)
-        self._check(self.core.fz_rope_kv_write(
-            _p(qkv), _p(cos), _p(sin), _p(meta.pos), _p(meta.seq_row), _p(table), c_int(table.shape[1]), _p(k), _p(v),
+        place = getattr(meta, "place", None)
+        if place is not None:
+            self._here(place, "places", torch.int32, (n,))
+        self._check(self.core.fz_rope_kv_write_at(
+            _p(qkv), _p(cos), _p(sin), _p(meta.pos), _p(place), _p(meta.seq_row), _p(table), c_int(table.shape[1]), _p(k), _p(v),
             c_longlong(page_stride), c_int(cache.page_size), c_int(1 if cache.write else 0), _p(q_out),
             c_int(_CODE[self.dtype]), c_int(n), c_int(num_heads), c_int(num_kv_heads), c_int(head_dim),
             c_int(cos.shape[0]), _p(self.err), self._stream()), "rope_kv_write")
@@ -630,7 +645,7 @@ class CudaOps(Ops):
     def linear_rope_kv_write(self, a, w, bias, cos, sin, meta, cache, q_out, num_heads, num_kv_heads, head_dim) -> bool:
         a, factors = self._factors(a)
         m, k = a.shape
-        if not (self.use_tensor_cores and self.fuse_rope and self.dtype == torch.bfloat16):
+        if not (self.use_tensor_cores and self.fuse_rope and self.dtype == torch.bfloat16) or getattr(meta, "place", None) is not None:
             return False
         if self.tc.fz_gemm_tc_qkv_rope_check(c_int(m), c_int(head_dim)) != 0:
             # many rows: 16 bytes at a time
@@ -823,14 +838,29 @@ class CudaOps(Ops):
         raise KernelError(f"{name} is not contiguous")
 
     def _launch(self, call, what: str, args: tuple, ideal_bytes: int = 0, kernels: int = 1) -> None:
-        """Runs a C entry on this table's device, whichever is current, and its current stream."""
-        if torch.cuda.current_device() != self._index:
+        """Runs a C entry (its argument types declared) on this table's device, whichever is current, and its current stream."""
+        stream = self._stream_handle
+        if stream is None:
+            stream = torch._C._cuda_getCurrentRawStream(self._index)
+        if torch._C._cuda_getDevice() != self._index:
             with torch.cuda.device(self._index):
-                status = call(*args, self._stream())
+                status = call(*args, stream)
         else:
-            status = call(*args, self._stream())
+            status = call(*args, stream)
         self._check(status, what, ideal_bytes)
         self.launches += kernels - 1
+
+    def _tree_kernel(self, num_heads, num_kv_heads, head_dim, page_size) -> bool:
+        """Whether the tensor-core kernel takes these sizes; raises for sizes that no kernel takes."""
+        key = (num_heads, num_kv_heads, head_dim, page_size)
+        tc = self._tree_sizes.get(key)
+        if tc is None:
+            if self.drafts.fz_attn_tree_check(num_heads, num_kv_heads, head_dim) != 0:
+                raise KernelError(f"tree_attention: {num_heads} heads, {num_kv_heads} kv heads, head_dim {head_dim} (need heads % kv_heads == 0, "
+                                  f"head_dim % 16 == 0 and head_dim <= 512)")
+            tc = self.use_tensor_cores and self.drafts_tc.fz_attn_tree_tc_check(*key) == 0
+            self._tree_sizes[key] = tc
+        return tc
 
     def tree_attention(self, q, cache, meta, out, num_heads, num_kv_heads, head_dim, scale, window) -> None:
         n = q.shape[0]
@@ -839,36 +869,34 @@ class CudaOps(Ops):
         k, v, page_stride = self._pool(cache, num_kv_heads, head_dim)
         if k.get_device() != self._index or v.get_device() != self._index:
             raise KernelError(f"the cache is on {k.device}; this kernel table works on {self.device}")
-        table, seg, bits = meta.table(cache.group), meta.seg, meta.ancestors
+        table, seg, bits, pos, row = meta.table(cache.group), meta.seg, meta.ancestors, meta.pos, meta.seq_row
         segments, pages = table.shape
+        words = bits.shape[-1]
         self._here(table, "block tables", torch.int32, (segments, pages))
         self._here(seg, "segments", torch.int32, (segments, 4))
-        self._here(meta.pos, "positions", torch.int32, (n,))
-        self._here(meta.seq_row, "table rows", torch.int32, (n,))
-        self._here(bits, "ancestors", torch.int32, (n, bits.shape[-1]))
-        if self.drafts.fz_attn_tree_check(num_heads, num_kv_heads, head_dim) != 0:
-            raise KernelError(f"tree_attention: {num_heads} heads, {num_kv_heads} kv heads, head_dim {head_dim} (need heads % kv_heads == 0, "
-                              f"head_dim % 16 == 0 and head_dim <= 512)")
+        self._here(pos, "positions", torch.int32, (n,))
+        self._here(row, "table rows", torch.int32, (n,))
+        self._here(bits, "ancestors", torch.int32, (n, words))
+        page_size, kp, vp = cache.page_size, k.data_ptr(), v.data_ptr()
+        tc = self._tree_kernel(num_heads, num_kv_heads, head_dim, page_size)
         if n == 0:
             return
-        # scratch of the call alone (from the stream's allocator, or the graph's that records it): two calls never share it
-        num_pages = k.shape[0]
-        if self.tree_tensor_cores and self.use_tensor_cores and \
-                self.drafts_tc.fz_attn_tree_tc_check(num_heads, num_kv_heads, head_dim, cache.page_size) == 0 and \
-                page_stride == 2 * num_kv_heads * cache.page_size * head_dim and v.data_ptr() - k.data_ptr() == page_stride:
+        # scratch of the call alone (from the stream's allocator, or the graph's that records it): two calls never share it.
+        # Tensor cores: keys and values in one pool, (pages, 2, kv heads, page size, head size)
+        if tc and self.tree_tensor_cores and page_stride == 2 * num_kv_heads * page_size * head_dim and vp - kp == page_stride // 2 * k.element_size():
             slots = self.drafts_tc.fz_attn_tree_tc_slots(n, segments, num_heads, num_kv_heads)
             part = torch.empty(slots * 128 * (head_dim + 2) + 2 * n * num_kv_heads, dtype=torch.float32, device=self.device)
             self._launch(self.drafts_tc.fz_attn_tree_tc, "tree_attention (tensor cores)",
-                         (_p(q), _p(k), _p(v), _p(meta.pos), _p(meta.seq_row), _p(seg), segments, _p(bits), bits.shape[1], _p(table), pages,
-                          c_longlong(page_stride), cache.page_size, num_pages, _p(out), n, num_heads, num_kv_heads, head_dim, c_float(scale),
-                          window, _p(part), _p(self.err)), kernels=2)
+                         (q.data_ptr(), kp, vp, pos.data_ptr(), row.data_ptr(), seg.data_ptr(), segments, bits.data_ptr(), words, table.data_ptr(), pages,
+                          page_stride, page_size, k.shape[0], out.data_ptr(), n, num_heads, num_kv_heads, head_dim, scale, window, part.data_ptr(),
+                          self._err_ptr), kernels=2)
             return
         pieces = self.drafts.fz_attn_tree_pieces(meta.max_context, window)
         part = torch.empty(n * num_heads * pieces * (head_dim + 2), dtype=torch.float32, device=self.device)
         self._launch(self.drafts.fz_attn_tree, "tree_attention",
-                     (_p(q), _p(k), _p(v), _p(meta.pos), _p(meta.seq_row), _p(seg), segments, _p(bits), bits.shape[1], _p(table), pages,
-                      c_longlong(page_stride), cache.page_size, num_pages, _p(out), _CODE[self.dtype], n, num_heads, num_kv_heads, head_dim,
-                      c_float(scale), window, pieces, _p(part), _p(self.err)), kernels=2)
+                     (q.data_ptr(), kp, vp, pos.data_ptr(), row.data_ptr(), seg.data_ptr(), segments, bits.data_ptr(), words, table.data_ptr(), pages,
+                      page_stride, page_size, k.shape[0], out.data_ptr(), _CODE[self.dtype], n, num_heads, num_kv_heads, head_dim, scale, window,
+                      pieces, part.data_ptr(), self._err_ptr), kernels=2)
 
     def verify_tree(self, logits, draft, temperature, uniform, tokens, parents, seg, path, count, next_ids) -> None:
         if logits.dim() != 2 or seg.dim() != 2:
@@ -893,19 +921,19 @@ class CudaOps(Ops):
         slices = self.drafts.fz_verify_ahead(segments, n, vocab)
         stats = torch.empty(n * slices * 24, dtype=torch.uint8, device=self.device) if slices else None
         self._launch(self.drafts.fz_verify_tree, "verify_tree",
-                     (_p(logits), _p(draft), _p(temperature), _p(uniform), _p(tokens), _p(parents), _p(seg), segments, n, vocab, _p(path),
-                      _p(count), _p(next_ids), _p(stats), slices, _p(self.err)), kernels=2 if slices else 1)
+                     (logits.data_ptr(), None if draft is None else draft.data_ptr(), temperature.data_ptr(), uniform.data_ptr(), tokens.data_ptr(),
+                      parents.data_ptr(), seg.data_ptr(), segments, n, vocab, path.data_ptr(), count.data_ptr(), next_ids.data_ptr(),
+                      None if stats is None else stats.data_ptr(), slices, self._err_ptr), kernels=2 if slices else 1)
 
     def _group_pool(self, pool) -> tuple[int, int, int, int, int]:
         """(slots, pages, parts, page size, bytes of a row) of a cache group's pool (see `KVNeed.pool_shape`, `LatentNeed.pool_shape`)."""
-        if not 4 <= pool.dim() <= 6:
-            raise KernelError(f"a cache pool has 4 to 6 dimensions, not {pool.dim()}")
-        self._here(pool, "cache pool", pool.dtype, pool.shape)
         shape = pool.shape
-        parts = 1
-        for x in shape[2:-2]:
-            parts *= x
-        return shape[0], shape[1], parts, shape[-2], shape[-1] * pool.element_size()
+        if not 4 <= len(shape) <= 6:
+            raise KernelError(f"a cache pool has 4 to 6 dimensions, not {len(shape)}")
+        if pool.element_size() < 2:
+            raise KernelError(f"a cache pool of {pool.dtype}: elements of 2 bytes and more are moved")
+        self._here(pool, "cache pool", pool.dtype, shape)
+        return shape[0], shape[1], math.prod(shape[2:-2]), shape[-2], shape[-1] * pool.element_size()
 
     def keep_rows(self, pool, table, seg, path, count) -> None:
         slots, num_pages, parts, page_size, row_bytes = self._group_pool(pool)
@@ -918,8 +946,8 @@ class CudaOps(Ops):
         if pool.numel() == 0 or segments == 0 or n == 0:
             return
         self._launch(self.drafts.fz_keep_rows, "keep_rows",
-                     (_p(pool), slots, num_pages, parts, page_size, row_bytes, _p(table), segments, pages, _p(seg), _p(path), _p(count), n,
-                      _p(self.err)))
+                     (pool.data_ptr(), slots, num_pages, parts, page_size, row_bytes, table.data_ptr(), segments, pages, seg.data_ptr(), path.data_ptr(),
+                      count.data_ptr(), n, self._err_ptr))
 
     def copy_pages(self, pool, src, dst) -> None:
         slots, num_pages, parts, page_size, row_bytes = self._group_pool(pool)
@@ -928,9 +956,9 @@ class CudaOps(Ops):
         self._here(dst, "destination pages", torch.int32, (m,))
         if pool.numel() == 0 or m == 0:
             return
+        page_bytes = parts * page_size * row_bytes
         self._launch(self.drafts.fz_copy_pages, "copy_pages",
-                     (_p(pool), slots, num_pages, c_longlong(parts * page_size * row_bytes), _p(src), _p(dst), m, _p(self.err)),
-                     2 * m * slots * parts * page_size * row_bytes)
+                     (pool.data_ptr(), slots, num_pages, page_bytes, src.data_ptr(), dst.data_ptr(), m, self._err_ptr), 2 * m * slots * page_bytes)
 
     # ---- the gated parallel block
     def select_tokens(self, tokens, src, prev_ids, out) -> None:

@@ -19,6 +19,8 @@ from ..kernels.interface import ScaledRows
 
 @register_mixer("gqa_attention")
 class GQAttention(Mixer):
+    takes_trees = True
+
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
                  window: int = 0, position: str | None = "rope",
                  names: tuple[str, str, str, str] = ("q_proj", "k_proj", "v_proj", "o_proj")):
@@ -75,5 +77,6 @@ class GQAttention(Mixer):
             ops.linear(h, self.wqkv, self.bqkv, qkv)
             position.rotate_and_store(ctx, qkv, q, cache, Hq, Hkv, hd)
         o = ws.get("attn_out", (n, Hq * hd), ops.dtype)
-        ops.paged_attention(q, cache, ctx.meta, o, Hq, Hkv, hd, self.scale, self.window)
+        attend = ops.tree_attention if getattr(ctx.meta, "tree", False) else ops.paged_attention
+        attend(q, cache, ctx.meta, o, Hq, Hkv, hd, self.scale, self.window)
         return PendingProduct(o, self.wo, self.bo)

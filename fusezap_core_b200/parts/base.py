@@ -212,6 +212,8 @@ class Part:
 
 
 class Mixer(Part):
+    takes_trees = False      # whether forward runs steps of drafted trees (meta.tree): rows that are not consecutive places
+
     def cache_need(self) -> "KVNeed | LatentNeed | None":
         return None
 

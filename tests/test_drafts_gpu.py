@@ -560,3 +560,173 @@ def test_refusals():
         with pytest.raises(KernelError):
             ops.copy_pages(**{**dict(pool=pool, src=i32(3), dst=i32(3)), **bad})
     ops.check_errors()
+
+
+# ---------------------------------------------------------------------------------------------- the step function
+
+def small_model(name, dtype, tmp_path, max_len=1024):
+    from fusezap_core_b200 import load_model
+    from util import make_model_dir
+    d, cfg, opts = make_model_dir(name, tmp_path, dtype)
+    return load_model(d, dtype, "cuda:0", max_len=max_len), cfg, opts
+
+
+def runner_for(model, page, pages=700, nodes=64, rows=640):
+    from fusezap_core_b200.cache import CacheManager
+    from fusezap_core_b200.engine import StepRunner
+    cache = CacheManager(model.cache_needs(), model.state_needs(), page, pages, 8, model.max_len, model.ops.dtype, "cuda:0")
+    return StepRunner(model, cache, max_rows=rows, max_segments=8, max_tree_nodes=nodes), cache
+
+
+@pytest.mark.parametrize("name,dtype,page", [("tiny_llama", "float32", 4), ("tiny_window", "float32", 8), ("tiny_hd64", "float32", 16),
+                                              ("tiny_hd64", "bfloat16", 16), ("tiny_hd128", "bfloat16", 16), ("tiny_hd128", "bfloat16", 8), ("tiny_hd128", "bfloat16", 4)])
+def test_drafted_steps_equal_steps_of_single_tokens(name, dtype, page, tmp_path):
+    """Trees around the tokens that plain decoding gives, verified greedily, kept and continued. float32: the tokens are the same and so are
+    the logits, up to the tolerance of one model in two cuttings; bfloat16: the logits are, the tokens are taken as they come."""
+    from fusezap_core_b200.engine import Portion
+    from util import assert_close, prompts
+    model, cfg, opts = small_model(name, dtype, tmp_path, max_len=512 if name != "tiny_llama" else 128)
+    run, cache = runner_for(model, page)
+    plain_run, plain_cache = runner_for(model, page)
+    P = prompts(cfg, (5, 41, 90), seed=3) if name == "tiny_llama" else prompts(cfg, (33, 200, 310), seed=3)
+    for r, c in ((run, cache), (plain_run, plain_cache)):
+        r.run([Portion(i, p[:-1], []) for i, p in enumerate(P)])
+    rng = np.random.default_rng(0)
+    have = [list(p) for p in P]
+    V = cfg["vocab_size"]
+    for step in range(6):
+        # what plain decoding gives next, on a copy of the books: two tokens of each request, forgotten afterwards
+        portions = []
+        for i in range(len(P)):
+            tokens, parents, under = [have[i][-1], int(rng.integers(V))], [-1, 0], 0
+            for _ in range(int(rng.integers(0, 4))):
+                tokens += [int(rng.integers(V)), int(rng.integers(V))]
+                parents += [under, under]
+                under = len(tokens) - 2
+            portions.append(Portion(i, tokens, range(len(tokens)), parents=parents))
+        # the right token among the root's children in every other step
+        first = plain_run.run([Portion(i, [have[i][-1]], [0]) for i in range(len(P))]).argmax(1).tolist()
+        if step % 2:
+            for p, t in zip(portions, first):
+                p.tokens[1] = t
+        starts = run.prepare(portions)
+        logits = run.forward()
+        n, s = logits.shape[0], len(P)
+        path, count, ids = run.verify(logits, torch.zeros(s, device="cuda"), torch.zeros(n, dtype=torch.float64, device="cuda"))
+        run.keep(path, count)
+        model.ops.check_errors()
+        got, kept = logits.clone(), count.tolist()
+        run.commit_kept(portions, starts, kept)
+        cache.check()
+        at = 0
+        for i, (p, k) in enumerate(zip(portions, kept)):
+            nodes = path[at:at + k].tolist()
+            assert dtype == "bfloat16" or not step % 2 or k > 1, "the right token was among the root's children"
+            new = [p.tokens[j] for j in nodes[1:]] + [int(ids[i])]
+            # the same tokens one by one (the first has run above)
+            ref = []
+            for j, t in enumerate(new[:-1]):
+                ref.append(plain_run.run([Portion(i, [t], [0])])[0].clone())
+            if ref:
+                assert_close(got[[at + j for j in nodes[1:]]].cpu().numpy(), torch.stack(ref).cpu().numpy(), dtype, f"step {step}, request {i}")
+            if dtype == "float32":
+                assert int(ids[i]) == (int(ref[-1].argmax()) if ref else first[i])
+            have[i] += new
+            at += len(p.tokens)
+            assert cache.computed[i] == plain_cache.computed[i] == len(have[i]) - 1
+    # the caches hold the same: the next token's logits agree
+    last = [run_.run([Portion(i, [h[-1]], [0]) for i, h in enumerate(have)]).clone() for run_ in (run, plain_run)]
+    assert_close(last[0].cpu().numpy(), last[1].cpu().numpy(), dtype, "after the drafts")
+
+
+@pytest.mark.parametrize("name,dtype", [("tiny_hd64", "float32"), ("tiny_hd128", "bfloat16")])
+def test_a_recorded_step_of_trees_replayed_over_others(name, dtype, tmp_path):
+    """One recorded tree step with its verdict and the move of the kept rows, replayed with other trees, contexts and requests."""
+    from fusezap_core_b200.engine import Portion
+    from util import prompts
+    model, cfg, opts = small_model(name, dtype, tmp_path)
+    run, cache = runner_for(model, 16)
+    other, other_cache = runner_for(model, 16)
+    P = prompts(cfg, (60, 130, 311), seed=5)
+    for r in (run, other):
+        r.run([Portion(i, p[:-1], []) for i, p in enumerate(P)])
+    V = cfg["vocab_size"]
+    rng = np.random.default_rng(7)
+    temperature, uniform = torch.tensor([0.0, 0.8, 1.1], device="cuda"), torch.empty(24, dtype=torch.float64, device="cuda")
+    graph = out = None
+    for step in range(5):
+        portions = []
+        for i, n in enumerate((9, 5, 10)):
+            parents = [-1] + [int(rng.integers(0, j)) for j in range(1, n)]
+            portions.append(Portion(i, [int(t) for t in rng.integers(0, V, n)], range(n), parents=parents))
+        uniform.copy_(torch.from_numpy(rng.random(24)))
+        results = []
+        for r, c in ((run, cache), (other, other_cache)):
+            starts = r.prepare(portions)
+            r.meta.max_context = 512
+
+            def step_of(r=r):
+                logits = r.forward()
+                path, count, ids = r.verify(logits, temperature, uniform)
+                r.keep(path, count)
+                return logits, path, count, ids
+
+            if r is run and step == 1:
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    out = step_of()
+            if r is run and graph is not None:
+                graph.replay()
+                got = out
+            else:
+                got = step_of()
+            model.ops.check_errors()
+            results.append([t.clone() for t in got])
+            r.commit_kept(portions, starts, got[2].tolist())
+            c.check()
+        assert all(torch.equal(a, b) for a, b in zip(*results)), f"step {step}"
+
+
+def test_forked_requests_on_the_device(tmp_path):
+    from fusezap_core_b200.engine import Portion
+    from util import assert_close, prompts
+    model, cfg, opts = small_model("tiny_hd128", "bfloat16", tmp_path)
+    run, cache = runner_for(model, 16)
+    p = prompts(cfg, (75,), seed=6)[0]
+    run.run([Portion("a", p, [])])
+    run.fork("a", "b")
+    cache.check()
+    more = {r: prompts(cfg, (9,), seed=s)[0] for r, s in (("a", 7), ("b", 8))}
+    for j in range(9):
+        lg = run.run([Portion(r, [more[r][j]], [0]) for r in ("a", "b")]).clone()
+    for k, r in enumerate(("a", "b")):
+        cache.reset()
+        ref = run.run([Portion("x", p, [])])
+        for t in more[r]:
+            ref = run.run([Portion("x", [t], [0])]).clone()
+        assert_close(lg[k:k + 1].cpu().numpy(), ref.cpu().numpy(), "bfloat16", r)
+    model.ops.check_errors()
+
+
+@pytest.mark.parametrize("heads,kv,hd,page", [(4, 4, 64, 16), (32, 8, 128, 16), (10, 2, 128, 8)])
+def test_the_general_kernel_takes_what_the_tensor_core_kernel_takes(heads, kv, hd, page):
+    ops = ops_of("bfloat16")
+    c = tree_case("bfloat16", heads, kv, hd, page, [(37, bushy(9)), (0, bushy(5, 1)), (700, chain(3)), (300, [-1])], pad=3)
+    assert_tree(c, run_tree(c))
+    ops.tree_tensor_cores = False
+    try:
+        assert_tree(c, run_tree(c))
+    finally:
+        ops.tree_tensor_cores = True
+
+
+def test_bad_tables_are_reported():
+    """A page that is missing, one outside the pool, a row outside its request: an error, and nothing outside is read or written."""
+    from fusezap_core_b200.kernels.table import KernelError
+    for dtype in ("float32", "bfloat16"):
+        for change, why in ((lambda m: m.tables.__setitem__((0, 2), -1), "no page"), (lambda m: m.tables.__setitem__((0, 2), 10 ** 6), "no page"),
+                            (lambda m: m.seq_row.__setitem__(0, 7), "outside the step"), (lambda m: m.seg.__setitem__((0, 1), 3), "outside the step")):
+            c = tree_case(dtype, 8, 2, 64, 16, [(60, bushy(9)), (20, bushy(4))])
+            change(c.meta)
+            with pytest.raises(KernelError, match=why):
+                run_tree(c)

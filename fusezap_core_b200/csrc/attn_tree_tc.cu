@@ -46,16 +46,23 @@ struct Sizes {
   int S, NB, Hkv, window;
 };
 
-// The walk of a block (every role's own copy, warp-wide) over its run of units, one stretch at a time: a stretch is the block's share of
-// an item, `count` key tiles of the places [a, b) from place `key0` on. Requests are looked up only where the run crosses from one to the
-// next; within a request the next item follows by counting.
+// A block's share of an item: `count` key tiles of the places [a, b) from place `key0` on, for `rows` (node, head) rows from row `row` on.
+// stretches: how many the item has in all where this is its first, else 0.
+struct Stretch {
+  int s, kvh, row, rows, key0, count, a, b, item, stretches;
+};
+constexpr int RING = 8;      // stretches that the key producer may be ahead of the others' reading (the queries' one buffer keeps it within four)
+
+// The walk of a block over its run of units, one stretch at a time, by the warp that fetches queries and keys; it leaves every stretch in
+// shared memory for the other roles, ahead of its data (each role walking by itself took 2 us of the softmax warps' time between two requests,
+// and their registers). Requests are looked up only where the run crosses from one to the next; within a request the next item
+// follows by counting.
 struct Walk {
   int G, u, u1;                                    // the next unit, the run's end
   int s, n, row0, a, b, tiles, row_tiles;          // the request
   int end, first_item;                             // its last unit + 1, its first item
   int chunk, chunk_units, chunk_items;             // where the look-up goes on: 32 requests from `chunk`, units and items before them
   int kvh, rt, item;                               // the item
-  int row, rows, key0, count;                      // the stretch: first row, (node, head) rows, first place, key tiles
 
   // Sum of all requests' units.
   static __device__ __forceinline__ int sum(const Sizes& Z) {
@@ -108,8 +115,8 @@ struct Walk {
     }
   }
   int tile;      // the stretch's first within its item
-  // The next stretch; false at the run's end.
-  __device__ __forceinline__ bool next(const Sizes& Z) {
+  // The next stretch; false at the run's end. share: units per block.
+  __device__ __forceinline__ bool next(const Sizes& Z, int share, Stretch& x) {
     if (u >= u1) return false;
     if (u >= end) {
       find(Z);
@@ -118,11 +125,9 @@ struct Walk {
       ++item;
       if (++rt == row_tiles) rt = 0, ++kvh;
     }
-    const int node0 = rt * Z.NB;
-    row = row0 + node0;
-    rows = min(Z.NB, n - node0) * G;
-    key0 = (a / BN + tile) * BN;
-    count = min(tiles - tile, u1 - u);
+    const int node0 = rt * Z.NB, count = min(tiles - tile, u1 - u);
+    x = {s, kvh, row0 + node0, min(Z.NB, n - node0) * G, (a / BN + tile) * BN, count, a, b, item,
+         tile == 0 ? (u + tiles - 1) / share - u / share + 1 : 0};
     u += count;
     return true;
   }
@@ -151,7 +156,9 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
   uint64_t* s_ready = v_empty + STAGES;    // one per stream
   uint64_t* p_ready = s_ready + 2;
   uint64_t* o_ready = p_ready + 2;
-  uint32_t* tmem_slot = (uint32_t*)(o_ready + 2);
+  uint64_t* listed = o_ready + 2;          // RING: stretch j stands in ring[j % RING]
+  Stretch* ring = (Stretch*)(listed + RING);
+  uint32_t* tmem_slot = (uint32_t*)(ring + RING);
   int* flag = (int*)(tmem_slot + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -171,6 +178,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
       mbar_init(&p_ready[i], 256);
       mbar_init(&o_ready[i], 1);
     }
+    for (int i = 0; i < RING; ++i) mbar_init(&listed[i], 1);
     flag[0] = 0;
     mbar_init_fence();
   }
@@ -187,19 +195,32 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
   const int G = Hq / Z.Hkv;
   const int total = Walk::sum(Z), share = (total + gridDim.x - 1) / gridDim.x;
   const int u0 = min(total, (int)blockIdx.x * share), u1 = min(total, u0 + share);
-  // Every role walks the same stretches and counts the key tiles it has gone through (`g`): ring stages, streams and barrier phases
-  // follow from that count and carry over from one stretch to the next.
+  // Every role goes through the same stretches and counts the key tiles it has gone through (`g`, up to u1 - u0): ring stages, streams and
+  // barrier phases follow from that count and carry over from one stretch to the next.
   bool ok = true;
-  Walk x;
-  x.G = G, x.u = u0, x.u1 = u1, x.end = x.chunk = x.chunk_units = x.chunk_items = 0;
+  Stretch x;
+  auto read = [&](int j) -> bool {      // stretch number j, once the key producer has listed it
+    if (!__all_sync(0xffffffffu, mbar_wait(&listed[j % RING], (j / RING) & 1))) return false;
+    x = ring[j % RING];
+    return true;
+  };
 
   if (warp == 0 || warp == 18) {
     // ---------------- producers
     const bool is_v = warp == 18;
     const int rows_per_page = 2 * Z.Hkv * page_size;
     int g = 0, n_q = 0;
-    while (ok && x.next(Z)) {
-      if (!is_v) {
+    Walk walk;
+    walk.G = G, walk.u = u0, walk.u1 = u1, walk.end = walk.chunk = walk.chunk_units = walk.chunk_items = 0;
+    while (ok && g < u1 - u0) {
+      if (is_v) {
+        if (!(ok = read(n_q++))) break;
+      } else {
+        walk.next(Z, share, x);
+        if (lane == 0) {
+          ring[n_q % RING] = x;
+          mbar_arrive(&listed[n_q % RING]);
+        }
         // the one Q buffer is free once the last score product of the stretch before is done
         if (n_q > 0) ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (n_q - 1) & 1));
         if (!ok) break;
@@ -278,10 +299,12 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     // ---------------- MMA issuer (the warp walks the stretches together, lane 0 issues)
     constexpr uint32_t idesc_s = make_idesc(BM, BN, false), idesc_pv = make_idesc(BM, HD, true);
     // The scores run two tiles ahead of the products with the values: two walks over the same stretches.
-    Walk y = x;
-    int st = 0, sg = 0, n_q = 0;               // the score walk: tile within its stretch, tiles so far, stretches so far
-    bool more = y.next(Z);
+    int st = 0, sg = 0, n_q = 0, scores = 0;   // the score walk: tile within its stretch, tiles so far, stretches so far, tiles of its stretch
     auto issue_s = [&]() -> bool {             // S(sg) = Q K(sg)^T into the scores of stream sg & 1; frees the key stage when done
+      if (st == 0) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&listed[n_q % RING], (n_q / RING) & 1))) return false;
+        scores = ring[n_q % RING].count;
+      }
       bool fine = true;
       if (lane == 0) {
         const int s = sg % STAGES;
@@ -298,22 +321,22 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
           }
           umma_commit(&s_ready[sg & 1]);
           umma_commit(&k_empty[s]);
-          if (st + 1 == y.count) umma_commit(q_empty);      // the stretch's last score product: Q may be overwritten when it is done
+          if (st + 1 == scores) umma_commit(q_empty);      // the stretch's last score product: Q may be overwritten when it is done
         }
       }
       fine = __shfl_sync(0xffffffffu, (int)fine, 0);
       if (!fine) return false;
       ++sg;
-      if (++st == y.count) {
+      if (++st == scores) {
         st = 0;
         ++n_q;
-        more = y.next(Z);
       }
       return true;
     };
-    int g = 0;
-    for (int i = 0; i < 2 && ok && more; ++i) ok = issue_s();
-    while (ok && x.next(Z)) {
+    int g = 0, n_x = 0;
+    for (int i = 0; i < 2 && ok && sg < u1 - u0; ++i) ok = issue_s();
+    while (ok && g < u1 - u0) {
+      if (!(ok = read(n_x++))) break;
       for (int t = 0; t < x.count && ok; ++t, ++g) {
         if (lane == 0) {
           const int s = g % STAGES, tq = g & 1;
@@ -333,7 +356,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
           }
         }
         ok = __shfl_sync(0xffffffffu, (int)ok, 0);
-        if (ok && more) ok = issue_s();      // the stream's next scores go behind the product that reads its P
+        if (ok && sg < u1 - u0) ok = issue_s();      // the stream's next scores go behind the product that reads its P
       }
     }
     if (!ok && lane == 0) flag[0] = 1;
@@ -348,13 +371,13 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     const int pair_bar = 1 + tq * 4 + quad, quad_bar = 9 + quad;
     float* mx_mine = s_mx + (tq * 2 + hf) * BM + r;
     const float* mx_other = s_mx + (tq * 2 + (hf ^ 1)) * BM + r;
-    int g0 = 0, n_s = 0, n_o[2] = {0, 0};      // tiles of the block, of this stream, and stretches with tiles of either stream so far
-    while (ok && x.next(Z)) {
+    int g0 = 0, n_x = 0, n_s = 0, n_o[2] = {0, 0};      // tiles of the block, of this stream, and stretches with tiles of either stream so far
+    while (ok && g0 < u1 - u0) {
+      if (!(ok = read(n_x++))) break;
       // which slots the item's rows will find their stretches in, from the block that has its first: (first slot, stretches)
-      if (x.tile == 0 && idx == 0) {
-        const int last = (x.u - x.count + x.tiles - 1) / share;
+      if (x.stretches > 0 && idx == 0) {
         for (int i = lane; i < x.rows / G; i += 32)
-          if (x.row + i < N) records[(size_t)(x.row + i) * Z.Hkv + x.kvh] = make_int2(blockIdx.x + x.item, last - blockIdx.x + 1);
+          if (x.row + i < N) records[(size_t)(x.row + i) * Z.Hkv + x.kvh] = make_int2(blockIdx.x + x.item, x.stretches);
       }
       const bool live = quad * 32 < x.rows;      // (the warp has rows)
       const int first = (g0 ^ tq) & 1;           // the first tile of the stretch that is this stream's
@@ -478,7 +501,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
       // A lane has one row: a store instruction would touch 32 lines with 16 bytes each. So every four lanes exchange first, four vectors
       // of four dimensions each: then a lane has vector `lane % 4` of all four rows, and an instruction writes 64 bytes of eight rows.
       const int d0 = (tq * 2 + hf) * JD, base = quad * 32 + (lane & ~3);
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < JD; c += 16) {
         float a[16], b[16];
         tmem_ld16(tmem_base + 256u + (uint32_t)(d0 + c) + lane_sel, a);
@@ -570,7 +593,7 @@ template <int HD, int BOX>
 int launch(const CUtensorMap& qm, const CUtensorMap& kvm, const void* v_pool, const Sizes& Z, const int* table, int mb, int page_size, int num_pages,
            int N, int Hq, float scale_log2, int blocks, int slots, float* part_o, float* part_ml, int2* records, int* err, cudaStream_t stream) {
   constexpr int HALVES = HD / 64, STAGES = HD <= 64 ? 6 : 3;
-  constexpr size_t smem = (size_t)HALVES * 128 * 128 * (1 + 2 * STAGES) + 4 * BM * 4 + 8 * (8 + 4 * STAGES + 1) + 8;
+  constexpr size_t smem = (size_t)HALVES * 128 * 128 * (1 + 2 * STAGES) + 4 * BM * 4 + 8 * (8 + 4 * STAGES + RING) + RING * sizeof(Stretch) + 8;
   static_assert(smem <= FZ_MOST_SMEM);
   auto kern = attn_tree_tc_kernel<HD, BOX>;
   FZ_RAISE_SMEM(kern);

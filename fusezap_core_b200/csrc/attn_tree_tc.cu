@@ -576,17 +576,24 @@ int sm_count() {
   return sms;
 }
 
-// Queries as (N, Hq, hd): boxes of NB nodes x the G heads of a kv head x 64 columns.
-int query_map(const void* q, int N, int Hq, int hd, int G, int NB, CUtensorMap* out) {
+// Queries as (N, Hq, hd): boxes of NB nodes x the G heads of a kv head x 64 columns. The pool as rows of hd values: boxes of `box` rows x 64.
+int encode(const void* p, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box, CUtensorMap* out) {
   EncodeTiled enc = encode_fn();
   if (!enc) return FZ_NO_DRIVER_ENTRY;
-  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)Hq, (cuuint64_t)N};
-  const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)Hq * hd * 2};
-  const cuuint32_t box[3] = {64u, (cuuint32_t)G, (cuuint32_t)NB};
   const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? FZ_OK : FZ_TMAP_ENCODE;
+}
+int query_map(const void* q, int N, int Hq, int hd, int G, int NB, CUtensorMap* out) {
+  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)Hq, (cuuint64_t)N}, strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)Hq * hd * 2};
+  const cuuint32_t box[3] = {64u, (cuuint32_t)G, (cuuint32_t)NB};
+  return encode(q, 3, dims, strides, box, out);
+}
+int pool_map(const void* pool, long long rows, int hd, int box_rows, CUtensorMap* out) {
+  const cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)hd * 2};
+  const cuuint32_t box[2] = {64u, (cuuint32_t)box_rows};
+  return encode(pool, 2, dims, strides, box, out);
 }
 
 template <int HD, int BOX>
@@ -635,7 +642,7 @@ FZ_API int fz_attn_tree_tc(const void* q, const void* k_pool, const void* v_pool
   int st = query_map(q, N, Hq, hd, G, NB, &qm);
   if (st != FZ_OK) return st;
   const int box = page_size == 8 ? 8 : 16;
-  if ((st = get_map_bf16(k_pool, pool_rows, hd, box, &kvm)) != FZ_OK) return st;
+  if ((st = pool_map(k_pool, pool_rows, hd, box, &kvm)) != FZ_OK) return st;
   const float scale_log2 = scale * 1.4426950408889634f;
   const long long slots = fz_attn_tree_tc_slots(N, S, Hq, Hkv);
   if (slots > 2147483647LL) return FZ_TOO_LARGE;

@@ -611,6 +611,11 @@ class CudaOps(Ops):
 
     def _pool(self, cache, hkv: int, hd: int):
         k, v = cache.keys, cache.values
+        page, strides = cache.page_size, k.stride()
+        if k.is_cuda and v.is_cuda and k.dtype == self.dtype == v.dtype and k.shape == v.shape and strides == v.stride() and \
+                k.shape[1:] == (hkv, page, hd) and strides[1:] == (page * hd, hd, 1):
+            return k, v, strides[0]
+        # (what is wrong with it)
         for t, name in ((k, "key pool"), (v, "value pool")):
             if not t.is_cuda or t.dtype != self.dtype:
                 raise KernelError(f"{name}: device {t.device}, dtype {t.dtype}; expected CUDA {self.dtype}")

@@ -159,6 +159,19 @@ def test_tree_attention_long_contexts(dtype):
     assert_tree(c, run_tree(c))
 
 
+@pytest.mark.parametrize("heads,kv,hd,page", [(32, 8, 128, 16), (10, 2, 128, 8), (14, 2, 64, 16), (8, 1, 64, 32)])
+def test_tree_attention_more_rows_than_a_tile(heads, kv, hd, page):
+    """Steps whose requests have more than 128 rows per kv head on average, beside some that have few, none or one tile too many."""
+    G = heads // kv
+    full, many = 128 // G, 1 + 300 // G
+    c = tree_case("bfloat16", heads, kv, hd, page, [(300, bushy(many)), (700, bushy(2 * full, 1)), (129, bushy(2 * full + 1, 2)), (50, [-1]), (0, bushy(many, 3)),
+                                                    (1500, bushy(3 * full, 4)), (128, bushy(4 * full + 3, 5)), (77, None)], pad=2)
+    assert c.q.shape[0] * G > 128 * 8
+    assert_tree(c, run_tree(c))
+    c = tree_case("bfloat16", heads, kv, hd, page, [(333, bushy(many)), (40, chain(full + 5))], window=90 + full)
+    assert_tree(c, run_tree(c))
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_tree_attention_many_requests_and_empty_ones(dtype):
     rng = np.random.default_rng(5)

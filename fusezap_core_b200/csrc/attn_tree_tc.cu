@@ -22,9 +22,6 @@
 // window on; the merge kernel walks the few before), so scores are masked in the first and last tile alone, and value rows
 // outside [a, b) never meet the tensor core: products take whole groups of 16 places, and a group cut by an end is filled by the
 // producer's lanes, zeros outside. What a page holds beside the context therefore does not matter.
-// PAIR: trees with more rows than a tile has (nodes x G > 128): an item is two row tiles, the two streams are the two tiles, and every key
-// and value stage is fetched once for both; each stream leaves its own rows, in a slot of its own (4 requests of up to 64 nodes behind 12,000
-// places, 40 heads of 128 over 8: 91 us with one tile per item, PAIRTIME with two).
 // Waits are bounded; a wait that gives up sets the error bit. No multicast.
 #include "attn_tree.cuh"
 #include "umma.cuh"
@@ -37,6 +34,34 @@ using namespace fzumma;
 constexpr int BM = 128, BN = 128, THREADS = 608;
 constexpr float RESCALE_STEP = 8.f;
 
+// The warp that issues MMAs runs together, with values that are the same in all lanes, and one lane's instruction counts (`lead`): the
+// operands of an MMA are then computed once for the warp. Inside a branch of one lane every operand is moved there for every
+// instruction, and the issue, 8 + 8 MMAs per key tile, took longer than the tile's data (1.6 against 1.5 us; MMATIME like this).
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(smem_u32(bar)), "r"(lead) : "memory");
+}
+__device__ __forceinline__ int same(int v) { return __shfl_sync(0xffffffffu, v, 0); }      // a value that is the same in all lanes, known to be
+
 // The context places of a request that the units cover, in key tiles, and its row tiles.
 __host__ __device__ __forceinline__ void request_units(int n, int start, int window, int NB, int& a, int& tiles, int& row_tiles) {
   a = window > 0 ? max(0, start + n - window) : 0;
@@ -46,7 +71,7 @@ __host__ __device__ __forceinline__ void request_units(int n, int start, int win
 
 struct Sizes {
   const int* seg;
-  int S, NB, Hkv, window;      // NB: nodes of an item
+  int S, NB, Hkv, window;
 };
 
 // A block's share of an item: `count` key tiles of the places [a, b) from place `key0` on, for `rows` (node, head) rows from row `row` on.
@@ -136,31 +161,27 @@ struct Walk {
   }
 };
 
-__host__ __device__ constexpr int key_stages(int hd) { return hd <= 64 ? 6 : 3; }
-__host__ __device__ constexpr int value_stages(int hd, bool pair) { return hd <= 64 ? 6 : pair ? 2 : 3; }      // (what shared memory holds)
-
-template <int HD, int BOX, bool PAIR>
+template <int HD, int BOX>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map, const __nv_bfloat16* __restrict__ v_pool,
                     const Sizes Z, const int* __restrict__ table, int mb, int page_size, int num_pages, int Hq, float scale_log2,
                     int N, int slots, float* __restrict__ part_o, float* __restrict__ part_ml, int2* __restrict__ records, int* err) {
   constexpr int HALVES = HD / 64;                     // 64-column halves of a head
-  constexpr int KS = key_stages(HD), VS = value_stages(HD, PAIR);      // key tiles and value tiles in flight
-  constexpr int Q_TILES = PAIR ? 2 : 1;
+  constexpr int STAGES = HD <= 64 ? 6 : 3;            // key tiles and value tiles in flight
   constexpr int HALF_BYTES = 128 * 128;               // 128 rows of 128 bytes
   constexpr int Q_BYTES = HALVES * HALF_BYTES, KV_BYTES = HALVES * HALF_BYTES;
   constexpr int TMEM_COLS = 512;                      // S0 / P0: 0.., S1 / P1: 128.., O0: 256.., O1: 256 + HD..
   constexpr int OPS = (BN / BOX) * HALVES;            // TMA boxes per key tile, for K and again for V
   extern __shared__ __align__(1024) uint8_t smem[];
-  const uint32_t s_q = smem_u32(smem), s_k = s_q + Q_TILES * Q_BYTES, s_v = s_k + KS * KV_BYTES;
-  float* s_mx = (float*)(smem + Q_TILES * Q_BYTES + (KS + VS) * KV_BYTES);      // [stream][half][128 rows]
+  const uint32_t s_q = smem_u32(smem), s_k = s_q + Q_BYTES, s_v = s_k + STAGES * KV_BYTES;
+  float* s_mx = (float*)(smem + Q_BYTES + 2 * STAGES * KV_BYTES);      // [stream][half][128 rows]
   uint64_t* q_full = (uint64_t*)(s_mx + 4 * BM);
   uint64_t* q_empty = q_full + 1;
-  uint64_t* k_full = q_empty + 1;          // one per stage
-  uint64_t* k_empty = k_full + KS;
-  uint64_t* v_full = k_empty + KS;
-  uint64_t* v_empty = v_full + VS;
-  uint64_t* s_ready = v_empty + VS;        // one per stream
+  uint64_t* k_full = q_empty + 1;          // STAGES each
+  uint64_t* k_empty = k_full + STAGES;
+  uint64_t* v_full = k_empty + STAGES;
+  uint64_t* v_empty = v_full + STAGES;
+  uint64_t* s_ready = v_empty + STAGES;    // one per stream
   uint64_t* p_ready = s_ready + 2;
   uint64_t* o_ready = p_ready + 2;
   uint64_t* listed = o_ready + 2;          // RING: stretch j stands in ring[j % RING]
@@ -168,7 +189,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
   uint32_t* tmem_slot = (uint32_t*)(ring + RING);
   int* flag = (int*)(tmem_slot + 1);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = same(tid >> 5), lane = tid & 31;
   if (s_q & 1023u) {      // (the swizzle needs it; the declaration asks for it)
     fz_grid_wait();
     if (tid == 0) atomicOr(err, FZ_ERR_WAIT_TIMEOUT);
@@ -177,8 +198,9 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
   if (tid == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
-    for (int s = 0; s < KS; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
-    for (int s = 0; s < VS; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_ready[i], 1);
       mbar_init(&p_ready[i], 256);
@@ -195,10 +217,10 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = (uint32_t)same((int)*tmem_slot);
   fz_grid_launch_dependents();
   fz_grid_wait();
-  const int G = Hq / Z.Hkv, tile_nodes = Z.NB / Q_TILES, tile_rows = tile_nodes * G;
+  const int G = Hq / Z.Hkv;
   const int total = Walk::sum(Z), share = (total + gridDim.x - 1) / gridDim.x;
   const int u0 = min(total, (int)blockIdx.x * share), u1 = min(total, u0 + share);
   // Every role goes through the same stretches and counts the key tiles it has gone through (`g`, up to u1 - u0): ring stages, streams and
@@ -231,20 +253,17 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
         if (n_q > 0) ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (n_q - 1) & 1));
         if (!ok) break;
         if (lane == 0) {
-          const int tiles = PAIR && x.rows > tile_rows ? 2 : 1;
-          mbar_expect_tx(q_full, tiles * tile_rows * 128 * HALVES);
-          for (int i = 0; i < tiles; ++i)
+          mbar_expect_tx(q_full, Z.NB * G * 128 * HALVES);
 #pragma unroll
-            for (int hf = 0; hf < HALVES; ++hf)
-              asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-                           ::"r"(s_q + i * Q_BYTES + hf * HALF_BYTES), "l"(&q_map), "r"(smem_u32(q_full)), "r"(64 * hf), "r"(x.kvh * G),
-                           "r"(x.row + i * tile_nodes) : "memory");
+          for (int hf = 0; hf < HALVES; ++hf)
+            asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                         ::"r"(s_q + hf * HALF_BYTES), "l"(&q_map), "r"(smem_u32(q_full)), "r"(64 * hf), "r"(x.kvh * G), "r"(x.row) : "memory");
         }
         ++n_q;
       }
       const int* trow = table + (size_t)x.s * mb;
       for (int t = 0; t < x.count && ok; ++t, ++g) {
-        const int stages = is_v ? VS : KS, s = g % stages, round = g / stages;
+        const int s = g % STAGES, round = g / STAGES;
         const int key0 = x.key0 + t * BN;
         // op -> (page box, column half). Keys: boxes with any place of [a, b). Values: boxes of groups of 16 places that lie in it whole.
         int op_row[(OPS + 31) / 32];
@@ -305,121 +324,69 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     }
     if (!ok && lane == 0) flag[0] = 1;
   } else if (warp == 1) {
-    // ---------------- MMA issuer (the warp walks the stretches together, lane 0 issues)
+    // ---------------- MMA issuer (the warp goes through the stretches together, lane 0's instructions count)
     constexpr uint32_t idesc_s = make_idesc(BM, BN, false), idesc_pv = make_idesc(BM, HD, true);
-    // The scores run ahead of the products with the values (two tiles; PAIR: one): two walks over the same stretches.
+    const uint32_t lead = lane == 0;
+    // The scores run two tiles ahead of the products with the values: two walks over the same stretches.
     int st = 0, sg = 0, n_q = 0, scores = 0;   // the score walk: tile within its stretch, tiles so far, stretches so far, tiles of its stretch
-    bool both = true;                          // (PAIR) that stretch has rows for both streams
-    // S = Q K(sg)^T into the scores of stream tq. first / last: of the products that read the key tile.
-    auto issue_s = [&](int tq, bool first, bool last) -> bool {
-      if (st == 0 && first) {
+    auto issue_s = [&]() -> bool {             // S(sg) = Q K(sg)^T into the scores of stream sg & 1; frees the key stage when done
+      if (st == 0) {
         if (!__all_sync(0xffffffffu, mbar_wait(&listed[n_q % RING], (n_q / RING) & 1))) return false;
-        scores = ring[n_q % RING].count;
-        both = ring[n_q % RING].rows > tile_rows;
-        last = last || (PAIR && !both);
+        scores = same(ring[n_q % RING].count);
+        if (!__all_sync(0xffffffffu, mbar_wait(q_full, n_q & 1))) return false;
       }
-      bool fine = true;
-      if (lane == 0) {
-        const int s = sg % KS;
-        if (st == 0 && first) fine = mbar_wait(q_full, n_q & 1);
-        if (first) fine = fine && mbar_wait(&k_full[s], (sg / KS) & 1);
-        if (fine) {
-          tc_fence_after();
-          const uint32_t sk = s_k + s * KV_BYTES, sq = s_q + (PAIR ? tq * Q_BYTES : 0), tmem_s = tmem_base + (uint32_t)tq * 128u;
+      const int s = sg % STAGES;
+      if (!__all_sync(0xffffffffu, mbar_wait(&k_full[s], (sg / STAGES) & 1))) return false;
+      tc_fence_after();
+      const uint32_t tmem_s = tmem_base + (uint32_t)(sg & 1) * 128u;
+      const uint64_t dq = desc_k_major(s_q), dk = desc_k_major(s_k + s * KV_BYTES);
 #pragma unroll
-          for (int hf = 0; hf < HALVES; ++hf) {
-            const uint64_t dq = desc_k_major(sq + hf * HALF_BYTES), dk = desc_k_major(sk + hf * HALF_BYTES);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) umma_bf16(tmem_s, dq + (uint64_t)(2 * k), dk + (uint64_t)(2 * k), idesc_s, (hf | k) ? 1u : 0u);
-          }
-          umma_commit(&s_ready[tq]);
-          if (last) {
-            umma_commit(&k_empty[s]);      // (frees the key stage when done)
-            if (st + 1 == scores) umma_commit(q_empty);      // the stretch's last score product: Q may be overwritten when it is done
-          }
-        }
+      for (int i = 0; i < 4 * HALVES; ++i) {      // 16 dimensions each: 32 bytes along a half's rows
+        const uint64_t step = (uint64_t)((i >> 2) * (HALF_BYTES >> 4) + 2 * (i & 3));
+        mma_ss(lead, tmem_s, dq + step, dk + step, idesc_s, i ? 1u : 0u);
       }
-      if (!__shfl_sync(0xffffffffu, (int)fine, 0)) return false;
-      if (last) {
-        ++sg;
-        if (++st == scores) {
-          st = 0;
-          ++n_q;
-        }
+      mma_commit(lead, &s_ready[sg & 1]);
+      mma_commit(lead, &k_empty[s]);
+      if (st + 1 == scores) mma_commit(lead, q_empty);      // the stretch's last score product: Q may be overwritten when it is done
+      ++sg;
+      if (++st == scores) {
+        st = 0;
+        ++n_q;
       }
       return true;
     };
-    // O += P V(g) of stream tq, the n-th tile of the stream. first: of the stream's in the stretch.
-    auto issue_pv = [&](int tq, int g, int n, int t, bool first, bool last, bool frees) -> bool {
-      bool fine = true;
-      if (lane == 0) {
-        const int s = g % VS;
-        fine = mbar_wait(&v_full[s], (g / VS) & 1) && mbar_wait(&p_ready[tq], n & 1);      // P written, O rescaled if it had to be
-        if (fine) {
-          tc_fence_after();
-          const uint32_t sv = s_v + s * KV_BYTES, tmem_p = tmem_base + (uint32_t)tq * 128u, tmem_o = tmem_base + 256u + (uint32_t)(tq * HD);
-          const int key0 = x.key0 + t * BN;
-          const int k0 = max(0, (x.a - key0) >> 4), k1 = min(BN / 16, (x.b - key0 + 15) >> 4);      // groups with places of [a, b)
-          // (P: the first 64 places over score columns 0..31, the others over 64..95; V: 16 places are 2,048 bytes, 128 in a descriptor)
-          const uint64_t dv = desc_mn_major(sv, HALF_BYTES);
-          if (k0 == 0 && k1 == BN / 16) {
-#pragma unroll
-            for (int kk = 0; kk < BN / 16; ++kk)
-              umma_bf16_a_tmem(tmem_o, tmem_p + (uint32_t)(kk < 4 ? 8 * kk : 64 + 8 * (kk - 4)), dv + (uint64_t)(128 * kk), idesc_pv, (!first || kk > 0) ? 1u : 0u);
-          } else {
-            for (int kk = k0; kk < k1; ++kk)
-              umma_bf16_a_tmem(tmem_o, tmem_p + (uint32_t)(kk < 4 ? 8 * kk : 64 + 8 * (kk - 4)), dv + (uint64_t)(128 * kk), idesc_pv, (!first || kk > k0) ? 1u : 0u);
-          }
-          if (last) umma_commit(&o_ready[tq]);
-          if (frees) umma_commit(&v_empty[s]);
-        }
-      }
-      return __shfl_sync(0xffffffffu, (int)fine, 0);
-    };
     int g = 0, n_x = 0;
-    const int tiles = u1 - u0;
-    if constexpr (PAIR) {
-      int n_t[2] = {0, 0};      // tiles of either stream so far
-      if (tiles > 0) {
-        ok = issue_s(0, true, false);
-        if (ok && both) ok = issue_s(1, false, true);
-      }
-      while (ok && g < tiles) {
-        if (!(ok = read(n_x++))) break;
-        const int streams = x.rows > tile_rows ? 2 : 1;
-        for (int t = 0; t < x.count && ok; ++t, ++g) {
-          const bool more = g + 1 < tiles;
-          bool next_both = false;
-          for (int tq = 0; tq < streams && ok; ++tq) {
-            ok = issue_pv(tq, g, n_t[tq]++, t, t == 0, t + 1 == x.count, tq + 1 == streams);
-            // the stream's next scores go behind the product that reads its P
-            if (ok && more) {
-              if (tq == 0) {
-                // (whether the next tile is for both streams: known once its stretch has been read)
-                ok = st == 0 ? issue_s(0, true, false) : issue_s(0, true, !both);
-                next_both = both;
-              } else if (next_both) {
-                ok = issue_s(1, false, true);
-              }
-            }
-          }
-          if (ok && more && streams == 1 && next_both) ok = issue_s(1, false, true);
+    for (int i = 0; i < 2 && ok && sg < u1 - u0; ++i) ok = issue_s();
+    while (ok && g < u1 - u0) {
+      if (!(ok = read(n_x++))) break;
+      const int xa = same(x.a), xb = same(x.b), xkey0 = same(x.key0), xcount = same(x.count);
+      for (int t = 0; t < xcount && ok; ++t, ++g) {
+        const int s = g % STAGES, tq = g & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&v_full[s], (g / STAGES) & 1) && mbar_wait(&p_ready[tq], (g >> 1) & 1));      // P(g) written, O rescaled if it had to be
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t tmem_p = tmem_base + (uint32_t)tq * 128u, tmem_o = tmem_base + 256u + (uint32_t)(tq * HD);
+        const int key0 = xkey0 + t * BN;
+        const int k0 = max(0, (xa - key0) >> 4), k1 = min(BN / 16, (xb - key0 + 15) >> 4);      // groups with places of [a, b)
+        // (P: the first 64 places over score columns 0..31, the others over 64..95; V: 16 places are 2,048 bytes, 128 in a descriptor)
+        const uint64_t dv = desc_mn_major(s_v + s * KV_BYTES, HALF_BYTES);
+        if (k0 == 0 && k1 == BN / 16) {
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk)
+            mma_ts(lead, tmem_o, tmem_p + (uint32_t)(kk < 4 ? 8 * kk : 64 + 8 * (kk - 4)), dv + (uint64_t)(128 * kk), idesc_pv, (t >= 2 || kk > 0) ? 1u : 0u);
+        } else {
+          for (int kk = k0; kk < k1; ++kk)
+            mma_ts(lead, tmem_o, tmem_p + (uint32_t)(kk < 4 ? 8 * kk : 64 + 8 * (kk - 4)), dv + (uint64_t)(128 * kk), idesc_pv, (t >= 2 || kk > k0) ? 1u : 0u);
         }
-      }
-    } else {
-      for (int i = 0; i < 2 && ok && sg < tiles; ++i) ok = issue_s(i, true, true);
-      while (ok && g < tiles) {
-        if (!(ok = read(n_x++))) break;
-        for (int t = 0; t < x.count && ok; ++t, ++g) {
-          ok = issue_pv(g & 1, g, g >> 1, t, t < 2, t + 2 >= x.count, true);
-          if (ok && sg < tiles) ok = issue_s(sg & 1, true, true);      // the stream's next scores go behind the product that reads its P
-        }
+        if (t + 2 >= xcount) mma_commit(lead, &o_ready[tq]);      // the stream's last of the stretch
+        mma_commit(lead, &v_empty[s]);
+        if (sg < u1 - u0) ok = issue_s();      // the stream's next scores go behind the product that reads its P
       }
     }
     if (!ok && lane == 0) flag[0] = 1;
   } else {
     // ---------------- softmax: warps 2..9 stream 0, warps 10..17 stream 1; two threads per row
-    constexpr int OD = HD / 2, JD = PAIR ? HD / 2 : HD / 4;      // output dimensions per thread: of its stream's rescaling, of the result
+    constexpr int OD = HD / 2, JD = HD / 4;      // output dimensions per thread: of its stream's rescaling, of the joined result
     const int idx = warp - 2, tq = idx >> 3, hf = (idx >> 2) & 1, quad = warp & 3;
     const int r = quad * 32 + lane;
     const uint32_t lane_sel = (uint32_t)(quad * 32) << 16;
@@ -434,18 +401,12 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
       // which slots the item's rows will find their stretches in, from the block that has its first: (first slot, stretches)
       if (x.stretches > 0 && idx == 0) {
         for (int i = lane; i < x.rows / G; i += 32)
-          if (x.row + i < N) records[(size_t)(x.row + i) * Z.Hkv + x.kvh] = make_int2((blockIdx.x + x.item) * Q_TILES + i / tile_nodes, x.stretches);
+          if (x.row + i < N) records[(size_t)(x.row + i) * Z.Hkv + x.kvh] = make_int2(blockIdx.x + x.item, x.stretches);
       }
-      const int rows = PAIR ? min(x.rows - tq * tile_rows, tile_rows) : x.rows;      // this stream's
-      if (PAIR && rows <= 0) {      // (the last item of a tree may have one tile)
-        g0 += x.count;
-        continue;
-      }
-      const bool live = quad * 32 < rows;        // (the warp has rows)
-      const int first = PAIR ? 0 : (g0 ^ tq) & 1;      // the first tile of the stretch that is this stream's
-      constexpr int EVERY = PAIR ? 1 : 2;
+      const bool live = quad * 32 < x.rows;      // (the warp has rows)
+      const int first = (g0 ^ tq) & 1;           // the first tile of the stretch that is this stream's
       float m_run = -INFINITY, l_part = 0.f;     // the maximum in use (exp2 domain) and this thread's half of the row's sum
-      for (int t = first; t < x.count && ok; t += EVERY) {
+      for (int t = first; t < x.count && ok; t += 2) {
         ok = __all_sync(0xffffffffu, mbar_wait(&s_ready[tq], n_s & 1));
         if (!ok) break;
         ++n_s;
@@ -481,7 +442,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
         const bool grow = m_new > m_run + RESCALE_STEP;
         if (__any_sync(0xffffffffu, grow)) {
           const float corr = grow ? fast_exp2(m_run - m_new) : 1.f;
-          if (t >= EVERY) {
+          if (t >= 2) {
             const float2 c2 = make_float2(corr, corr);
 #pragma unroll
             for (int c = 0; c < OD; c += 32) {
@@ -538,9 +499,10 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
         mbar_arrive(&p_ready[tq]);
       }
       if (!ok) break;
-      // The stretch's end. Warps without rows do not wait here: the barriers below, which keep a row quarter's warps within one stretch of
-      // one another, are not theirs, and a phase that has come round twice cannot be told from one that has not.
-      const bool has[2] = {PAIR ? tq == 0 : x.count > ((g0 ^ 0) & 1), PAIR ? tq == 1 : x.count > ((g0 ^ 1) & 1)};      // streams whose results are joined
+      // the stretch's end: both streams' last products, then the two results joined, a quarter of the dimensions per thread
+      const bool has[2] = {x.count > ((g0 ^ 0) & 1), x.count > ((g0 ^ 1) & 1)};
+      // (warps without rows do not wait here: the barriers below, which keep a row quarter's warps within one stretch of one another,
+      // are not theirs, and a phase that has come round twice cannot be told from one that has not)
       for (int j = 0; j < 2 && ok; ++j) {
         if (has[j] && live) ok = __all_sync(0xffffffffu, mbar_wait(&o_ready[j], n_o[j] & 1));
         n_o[j] += has[j];
@@ -549,44 +511,27 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
       if (!ok) break;
       if (!live) continue;
       tc_fence_after();
-      float m, l, f0 = 1.f, f1 = 0.f;
-      if constexpr (PAIR) {      // this stream's rows alone: two threads a row
-        *mx_mine = l_part;
-        asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
-        m = m_run;
-        l = l_part + *mx_other;
-        asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
-      } else {                   // the two streams' results joined: four threads a row
-        if (hf == 0) s_mx[tq * 2 * BM + r] = m_run;
-        asm volatile("bar.sync %0, 128;" ::"r"(quad_bar) : "memory");
-        const float m0 = s_mx[r], m1 = s_mx[2 * BM + r];
-        m = fmaxf(m0, m1);
-        const float mu = m == -INFINITY ? 0.f : m;
-        asm volatile("bar.sync %0, 128;" ::"r"(quad_bar) : "memory");
-        *mx_mine = l_part;
-        asm volatile("bar.sync %0, 128;" ::"r"(quad_bar) : "memory");
-        f0 = fast_exp2(m0 - mu), f1 = fast_exp2(m1 - mu);      // (a stream without tiles: maximum -inf, weight 0)
-        l = (s_mx[r] + s_mx[BM + r]) * f0 + (s_mx[2 * BM + r] + s_mx[3 * BM + r]) * f1;
-      }
-      const int slot = ((int)blockIdx.x + x.item) * Q_TILES + (PAIR ? tq : 0);
-      const size_t slot0 = (size_t)slot * BM;
-      const bool in_slots = slot < slots;
+      if (hf == 0) s_mx[tq * 2 * BM + r] = m_run;
+      asm volatile("bar.sync %0, 128;" ::"r"(quad_bar) : "memory");
+      const float m0 = s_mx[r], m1 = s_mx[2 * BM + r], m = fmaxf(m0, m1), mu = m == -INFINITY ? 0.f : m;
+      asm volatile("bar.sync %0, 128;" ::"r"(quad_bar) : "memory");
+      *mx_mine = l_part;
+      asm volatile("bar.sync %0, 128;" ::"r"(quad_bar) : "memory");
+      const float f0 = fast_exp2(m0 - mu), f1 = fast_exp2(m1 - mu);      // (a stream without tiles: maximum -inf, weight 0)
+      const float l = (s_mx[r] + s_mx[BM + r]) * f0 + (s_mx[2 * BM + r] + s_mx[3 * BM + r]) * f1;
+      const size_t slot0 = ((size_t)(blockIdx.x + x.item)) * BM;
+      const bool in_slots = (int)blockIdx.x + x.item < slots;
       if (!in_slots && lane == 0) atomicOr(err, FZ_ERR_ROW_RANGE);      // (requests with more rows than the step has)
       // A lane has one row: a store instruction would touch 32 lines with 16 bytes each. So every four lanes exchange first, four vectors
       // of four dimensions each: then a lane has vector `lane % 4` of all four rows, and an instruction writes 64 bytes of eight rows.
-      const int d0 = (PAIR ? hf : tq * 2 + hf) * JD, base = quad * 32 + (lane & ~3);
+      const int d0 = (tq * 2 + hf) * JD, base = quad * 32 + (lane & ~3);
 #pragma unroll 1
       for (int c = 0; c < JD; c += 16) {
-        float a[16];
-        if constexpr (PAIR) {
-          tmem_ld16(tmem_base + 256u + (uint32_t)(tq * HD + d0 + c) + lane_sel, a);
-        } else {
-          float b[16];
-          tmem_ld16(tmem_base + 256u + (uint32_t)(d0 + c) + lane_sel, a);
-          tmem_ld16(tmem_base + 256u + (uint32_t)(HD + d0 + c) + lane_sel, b);
+        float a[16], b[16];
+        tmem_ld16(tmem_base + 256u + (uint32_t)(d0 + c) + lane_sel, a);
+        tmem_ld16(tmem_base + 256u + (uint32_t)(HD + d0 + c) + lane_sel, b);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) a[j] = (has[0] ? a[j] * f0 : 0.f) + (has[1] ? b[j] * f1 : 0.f);
-        }
+        for (int j = 0; j < 16; ++j) a[j] = (has[0] ? a[j] * f0 : 0.f) + (has[1] ? b[j] * f1 : 0.f);
 #pragma unroll
         for (int k = 2; k > 0; k >>= 1) {
           const bool up = lane & k;
@@ -603,14 +548,13 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)      // (a[4 j ..] is now vector lane % 4 of row `base + j`)
-          if (in_slots && base + j < rows)
+          if (in_slots && base + j < x.rows)
             *(float4*)(part_o + (slot0 + base + j) * HD + d0 + c + 4 * (lane & 3)) = make_float4(a[4 * j], a[4 * j + 1], a[4 * j + 2], a[4 * j + 3]);
       }
-      if (in_slots && r < rows && d0 == 0) *(float2*)(part_ml + 2 * (slot0 + r)) = make_float2(m, l);
-      // nobody of this row quarter starts on the next stretch's tiles (whose products overwrite O) before all four have read (PAIR: a
-      // stream's O is read by its own threads alone, and its next product waits for the next P of each of them)
+      if (in_slots && r < x.rows && d0 == 0) *(float2*)(part_ml + 2 * (slot0 + r)) = make_float2(m, l);
+      // nobody of this row quarter starts on the next stretch's tiles (whose products overwrite O) before all four have read
       tc_fence_before();
-      if constexpr (!PAIR) asm volatile("bar.sync %0, 128;" ::"r"(quad_bar) : "memory");
+      asm volatile("bar.sync %0, 128;" ::"r"(quad_bar) : "memory");
     }
     if (!ok) flag[0] = 1;
   }
@@ -627,7 +571,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
 struct Stretches {
   const float *part_o, *part_ml;
   const int2* records;
-  int NB, tile_nodes, Hkv, window, slots;      // NB: nodes of an item
+  int NB, Hkv, window, slots;
   __device__ __forceinline__ int2 early(int n, int kvh) const { return records[(size_t)n * Hkv + kvh]; }
   __device__ __forceinline__ Range range(int2 record, int, int, int node, int head_in_group, int group, int nodes, int start, int pos) const {
     int a, tiles, row_tiles;
@@ -638,11 +582,10 @@ struct Stretches {
       x.extra_from = max(0, pos - window + 1);
       x.extra_to = min(a, start);
     }
-    const int step = NB / tile_nodes;      // (an item of two tiles has two slots)
-    const bool there = tiles > 0 && record.x >= 0 && record.y > 0 && (long long)record.x + (long long)(record.y - 1) * step < slots;
+    const bool there = tiles > 0 && record.x >= 0 && record.y > 0 && record.x <= slots - record.y;
     x.pieces = there ? record.y : 0;
-    x.first = there ? (size_t)record.x * BM + (node % tile_nodes) * group + head_in_group : 0;
-    x.step = BM * step;
+    x.first = there ? (size_t)record.x * BM + (node % NB) * group + head_in_group : 0;
+    x.step = BM;
     return x;
   }
 };
@@ -677,13 +620,13 @@ int pool_map(const void* pool, long long rows, int hd, int box_rows, CUtensorMap
   return encode(pool, 2, dims, strides, box, out);
 }
 
-template <int HD, int BOX, bool PAIR>
+template <int HD, int BOX>
 int launch(const CUtensorMap& qm, const CUtensorMap& kvm, const void* v_pool, const Sizes& Z, const int* table, int mb, int page_size, int num_pages,
            int N, int Hq, float scale_log2, int blocks, int slots, float* part_o, float* part_ml, int2* records, int* err, cudaStream_t stream) {
-  constexpr int HALVES = HD / 64, KS = key_stages(HD), VS = value_stages(HD, PAIR);
-  constexpr size_t smem = (size_t)HALVES * 128 * 128 * ((PAIR ? 2 : 1) + KS + VS) + 4 * BM * 4 + 8 * (8 + 2 * (KS + VS) + RING) + RING * sizeof(Stretch) + 8;
+  constexpr int HALVES = HD / 64, STAGES = HD <= 64 ? 6 : 3;
+  constexpr size_t smem = (size_t)HALVES * 128 * 128 * (1 + 2 * STAGES) + 4 * BM * 4 + 8 * (8 + 4 * STAGES + RING) + RING * sizeof(Stretch) + 8;
   static_assert(smem <= FZ_MOST_SMEM);
-  auto kern = attn_tree_tc_kernel<HD, BOX, PAIR>;
+  auto kern = attn_tree_tc_kernel<HD, BOX>;
   FZ_RAISE_SMEM(kern);
   const cudaError_t e = fz_launch(kern, dim3((unsigned)blocks), dim3(THREADS), smem, stream, qm, kvm, (const __nv_bfloat16*)v_pool, Z, table, mb, page_size,
                                   num_pages, Hq, scale_log2, N, slots, part_o, part_ml, records, err);
@@ -699,15 +642,12 @@ FZ_API int fz_attn_tree_tc_check(int Hq, int Hkv, int hd, int page_size) {
   return FZ_OK;
 }
 
-// Row tiles of an item: two where the requests have more rows than a tile on average.
-static int item_tiles(int N, int S, int Hq, int Hkv) { return (long long)N * (Hq / Hkv) > (long long)BM * S ? 2 : 1; }
-
 // Slots of the scratch (each 128 * (hd + 2) floats; behind them 2 * N * Hkv ints): a step's stretches are fewer than its blocks and items
 // together.
 FZ_API long long fz_attn_tree_tc_slots(int N, int S, int Hq, int Hkv) {
-  const int per = item_tiles(N, S, Hq, Hkv), NB = per * (BM / (Hq / Hkv));
-  const long long items = (long long)N / NB + S;
-  return per * (sm_count() + Hkv * (items < N ? items : N));
+  const int NB = BM / (Hq / Hkv);
+  const long long tiles = (long long)N / NB + S;
+  return sm_count() + Hkv * (tiles < N ? tiles : N);
 }
 
 // As fz_attn_tree; k_pool and v_pool are the two parts of one pool (pages, 2, Hkv, page_size, hd) of num_pages pages.
@@ -721,7 +661,7 @@ FZ_API int fz_attn_tree_tc(const void* q, const void* k_pool, const void* v_pool
   if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out | (uintptr_t)part) & 15) return FZ_BAD_ALIGNMENT;
   const long long pool_rows = (long long)num_pages * 2 * Hkv * page_size;
   if (pool_rows > 2147483647LL) return FZ_TOO_LARGE;
-  const int G = Hq / Hkv, NB = BM / G, per = item_tiles(N, S, Hq, Hkv), blocks = sm_count();
+  const int G = Hq / Hkv, NB = BM / G, blocks = sm_count();
   CUtensorMap qm, kvm;
   int st = query_map(q, N, Hq, hd, G, NB, &qm);
   if (st != FZ_OK) return st;
@@ -732,15 +672,15 @@ FZ_API int fz_attn_tree_tc(const void* q, const void* k_pool, const void* v_pool
   if (slots > 2147483647LL) return FZ_TOO_LARGE;
   float* part_ml = part + (size_t)slots * BM * hd;
   int2* records = (int2*)(part_ml + (size_t)slots * BM * 2);
-  const Sizes Z = {seg, S, per * NB, Hkv, window};
-#define FZ_T(HD_, BOX_) st = (per == 2 ? launch<HD_, BOX_, true> : launch<HD_, BOX_, false>)(qm, kvm, v_pool, Z, table, mb, page_size, num_pages, N, Hq, scale_log2, blocks, (int)slots, part, part_ml, records, err, stream)
+  const Sizes Z = {seg, S, NB, Hkv, window};
+#define FZ_T(HD_, BOX_) st = launch<HD_, BOX_>(qm, kvm, v_pool, Z, table, mb, page_size, num_pages, N, Hq, scale_log2, blocks, (int)slots, part, part_ml, records, err, stream)
   if (hd == 64 && box == 8) FZ_T(64, 8);
   else if (hd == 64) FZ_T(64, 16);
   else if (box == 8) FZ_T(128, 8);
   else FZ_T(128, 16);
 #undef FZ_T
   if (st != FZ_OK) return st;
-  const Stretches P = {part, part_ml, records, per * NB, NB, Hkv, window, (int)slots};
+  const Stretches P = {part, part_ml, records, NB, Hkv, window, (int)slots};
   const TreeArgs R = {pos, seq_row, seg, ancestors, table, S, words, mb, page_stride, page_size, num_pages, N, Hq, Hkv, hd, scale_log2, window, err};
   return launch_merge<__nv_bfloat16>((const __nv_bfloat16*)q, (const __nv_bfloat16*)k_pool, (const __nv_bfloat16*)v_pool, (__nv_bfloat16*)out, P, R, stream);
 }

@@ -31,30 +31,42 @@ constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int MAX_NODES = 1024;      // nodes of a tree
 constexpr float MARGIN = 1e-3f;      // of p(x): a decision nearer than that is taken in float64
 
+constexpr int MOST_TOKENS = 8 << 20;      // of a vocabulary (see `quick_chunk`)
+
+// (Above 1e30: 1e30, where logits of everyday size weigh the same already; times 1 / inf, -inf would be a NaN.)
+__device__ __forceinline__ float temperature_of(const float* temperature, int s) {
+  const float t = temperature[s];
+  return t > 1e30f ? 1e30f : t;
+}
+
 struct Ref {      // a row's scale: token x weighs exp((x - top) / T)
   double scale, top;      // 128 log2(e) / T, and the row's maximum
-  float cut;              // tokens below it weigh as much as it: NOTHING at most
+  unsigned far;           // the high word of the difference at which a token would weigh 2^-1015: below it tokens weigh exactly 0
 };
 constexpr double NOTHING = 1e-290;      // weights and probabilities up to this count as 0
-// reach: how far below the maximum a token weighs 2^-1015 (-inf must not reach the subtraction)
-__device__ __forceinline__ Ref ref_of(float top, double scale, double reach) { return {scale, (double)top, (float)fmax((double)top - reach, -3.0e38)}; }
 
 // The token's weight; 1 for x = top exactly, else off by 3e-12 of itself at most. t = 128 log2 of it, k = t rounded, f = t - k, 2^(t / 128) =
 // 2^(k / 128 div 128) * table[k mod 128] * 2^(f / 128), the last by a Taylor polynomial (the table-driven method of P. T. P. Tang, 1989).
 // tab: this lane's copy of the table, of which shared memory holds sixteen side by side: the lanes of half a warp, whose k are
-// anything, then never meet in a bank (with one copy the reads took as long as the rest: 28 us for 76,000 token pairs of an SM). A
+// anything, then never meet in a bank (with one copy the reads took as long as all the rest of a pass). A
 // row that holds a NaN or +inf is not asked for. Here and where p and q are made from weights the roundings are written out: every place that
 // needs a token's p gets the same bits.
+// LIFT: tokens too far below for a weight get 2^-1015 or so instead of 0, in fewer instructions (the first pass over 64 x 6 rows of 151,936
+// tokens: 130 us with exact zeros, 123 like this): for sums that are divided by no less than 1e-6 after it, where that is NOTHING.
 constexpr int TABLE = 128, COPIES = 16;
+template <bool LIFT = false>
 __device__ __forceinline__ double weight(float x, const Ref& r, const double* tab) {
-  const double d = __dadd_rn((double)fmaxf(x, r.cut), -r.top);
+  double d = __dadd_rn((double)x, -r.top);                // 0 or negative, -inf for x = -inf: the larger high word is the lower number
+  const bool none = (unsigned)__double2hiint(d) > r.far;
+  if (LIFT) d = __hiloint2double((int)min((unsigned)__double2hiint(d), r.far), __double2loint(d));
   const double big = 6755399441055744.0;                  // 1.5 * 2^52: the low bits of the sum are the nearest whole number
   const double shifted = __fma_rn(d, r.scale, big);
   const double f = __fma_rn(d, r.scale, -__dadd_rn(shifted, -big));
   const int k = __double2loint(shifted);
   constexpr double c1 = 0.0054152123481245725, c2 = 1.4662262387640425e-05, c3 = 2.646642144433097e-08;      // (ln 2 / 128)^i / i!
   const double e = __dmul_rn(tab[(k & (TABLE - 1)) * COPIES], __fma_rn(f, __fma_rn(f, __fma_rn(f, c3, c2), c1), 1.0));
-  return __hiloint2double(__double2hiint(e) + (k & ~(TABLE - 1)) * (1048576 / TABLE), __double2loint(e));
+  const double w = __hiloint2double(__double2hiint(e) + (k & ~(TABLE - 1)) * (1048576 / TABLE), __double2loint(e));
+  return !LIFT && none ? 0.0 : w;
 }
 
 __device__ __forceinline__ bool better(float v, int i, float bv, int bi) {      // numpy.argmax: a NaN is the maximum, then the lower index
@@ -215,7 +227,7 @@ __device__ __noinline__ Part first_sums(const float* __restrict__ lrow, const fl
       load_chunk(drow, i0, hi, vec, lane, b);
 #pragma unroll
       for (int j = 0; j < CHUNK; ++j) {      // (tokens from hi on weigh nothing)
-        const double wp = weight(a[j], rp, tab), wq = weight(b[j], rq, tab), over = fma(a0, wp, -wq);
+        const double wp = weight<true>(a[j], rp, tab), wq = weight<true>(b[j], rq, tab), over = fma(a0, wp, -wq);
         sp += wp;
         if (it != step(j)) sq += wq;
         if (__double2hiint(over) >= 0) {      // (the sign bit)
@@ -226,7 +238,7 @@ __device__ __noinline__ Part first_sums(const float* __restrict__ lrow, const fl
     } else {
 #pragma unroll
       for (int j = 0; j < CHUNK; ++j) {
-        const double wp = weight(a[j], rp, tab);
+        const double wp = weight<true>(a[j], rp, tab);
         if (it != step(j)) sp += wp;
       }
     }
@@ -306,7 +318,7 @@ verify_stats_kernel(const float* __restrict__ logits, const float* __restrict__ 
     }
   }
   if (s < 0 || row0 + n > N || n > MAX_NODES) return;
-  const float T = temperature[s];
+  const float T = temperature_of(temperature, s);
   const bool greedy = !(T > 0.f);
   bool with_q = false;
   if (draft && !greedy)
@@ -343,7 +355,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
   const double* tab = sh.tab + lane % COPIES;
   fz_grid_wait();
   const int row0 = seg[4 * s], n = seg[4 * s + 1];
-  const float T = temperature[s];
+  const float T = temperature_of(temperature, s);
   const bool first = rank == 0 && tid == 0;
   if (n <= 0 || row0 < 0 || row0 + n > N || n > MAX_NODES) {      // (the whole cluster)
     if (first) {
@@ -360,7 +372,8 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
   }
   __syncthreads();
   const bool greedy = !(T > 0.f);
-  const double scale = 184.6649652337873 / (double)T, reach = (1015.0 * 0.6931471805599453) * (double)T;      // 128 log2(e) / T
+  const double scale = 184.6649652337873 / (double)T;      // 128 log2(e) / T
+  const unsigned far = (unsigned)__double2hiint(-(1015.0 * 0.6931471805599453) * (double)T);
   const float scale2 = (float)fmin(1.4426950408889634 / (double)T, 3.4e38);
   // this warp's run of tokens: [lo, hi), within the block's part of the vocabulary; multiples of four
   const int per_warp = ((V + BLOCKS * WARPS - 1) / (BLOCKS * WARPS) + 3) & ~3;
@@ -459,7 +472,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     }
     if ((all.bad & 1) || !(all.sum_p > 0.f)) break;      // a row without a distribution: V - 1
     const bool dead_q = with_q && ((all.bad & 2) || !(all.sum_q > 0.f));      // a drafter's row without one: no child stands, p stays
-    const Ref rp = ref_of(all.top_p, scale, reach), rq = ref_of(all.top_q, scale, reach);
+    const Ref rp = {scale, (double)all.top_p, far}, rq = {scale, (double)all.top_q, far};
     const float near_p = 1.f / all.sum_p, near_q = with_q && !dead_q ? 1.f / all.sum_q : 0.f;      // quick
     double inv_p = 0.0, inv_q = 0.0;      // exact
     // what the draw goes by: a warp's or block's part is (sum_p or over + shift * under) * unit of its sums, the whole 1 or all of p
@@ -768,7 +781,7 @@ FZ_API int fz_verify_tree(const float* logits, const float* draft, const float* 
   if (S <= 0) return FZ_OK;
   if (V <= 0 || N < 0 || slices < 0 || slices > MAX_SLICES || (slices > 0 && !scratch)) return FZ_BAD_SHAPE;
   if ((uintptr_t)scratch & 7) return FZ_BAD_ALIGNMENT;
-  if ((long long)S * 16 > 2147483647LL) return FZ_TOO_LARGE;
+  if ((long long)S * 16 > 2147483647LL || V > MOST_TOKENS) return FZ_TOO_LARGE;
   Found* stats = slices > 0 ? (Found*)scratch : nullptr;
   if (stats && N > 0) {
     const cudaError_t e = fz_launch(verify_stats_kernel, dim3((unsigned)N, (unsigned)slices), dim3(AHEAD_THREADS), 0, stream, logits, draft, temperature,

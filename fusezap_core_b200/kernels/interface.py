@@ -473,7 +473,7 @@ class Ops:
                     next_ids: torch.Tensor) -> None:
         """Which nodes of each request's tree stand against the target, and the token behind them. logits (N, V) float32: the
         target's at every node; draft (N, V) float32: the drafter's at every node (row n gave n's children), or None: the children
-        were not drawn from probabilities; temperature (S,) float32, of both; uniform (N,) float64 in [0, 1): a child's own
+        were not drawn from probabilities; temperature (S,) float32, of both (above 1e30: 1e30); uniform (N,) float64 in [0, 1): a child's own
         number, the root's for the draw at the end; tokens, parents (N,) int32: parent = node within the request's rows, before the
         child; node 0 is the root, whose token stands; seg (S, 4) int32 = (first row, rows, anything, anything), at most 1,024 rows.
         From the root on, with p = softmax(logits / T) and q = softmax(draft / T) of the node (draft None: q is all on the child):
@@ -482,7 +482,7 @@ class Ops:
         running sum of p, in index order, first exceeds uniform[root] * total. T <= 0: the first child that is the argmax
         (the order of `argmax`) stands, else the argmax is the next token. float64. A row without a distribution (a NaN, +inf, or
         nothing above -inf): no child stands and the draw gives V - 1 (a drafter's row: no child stands and p is
-        drawn from).
+        drawn from). At most 8,388,608 tokens.
         Results, int32: count[s] kept nodes (the root among them; 0 for no rows, next_ids[s] = -1); path[first row + k] = node of the
         k-th of them, -1 from count[s] to the request's last row; rows of `path` beside the requests' are left."""
         raise NotImplementedError

@@ -419,6 +419,40 @@ def test_verify_small_and_large_temperatures():
     assert_verify(c)
 
 
+def test_verify_temperatures_at_the_ends_of_float32():
+    c = verify_case(20000, [bushy(6, s) for s in range(8)], False, seed=15, greedy=lambda s: False)
+    c["logits"][:, 100:9000] = -np.inf
+    c["temperature"][:] = [1e-45, 1e-38, 1e-30, 1e-10, 1e10, 1e30, 1e-3, 1e4]
+    assert_verify(c)
+    few = run_verify(c | dict(temperature=np.full(8, 1e30, np.float32)))
+    for t in (1e35, np.inf):      # (above 1e30: as 1e30)
+        for a, b in zip(run_verify(c | dict(temperature=np.full(8, t, np.float32))), few):
+            np.testing.assert_array_equal(a, b)
+
+
+def test_verify_masks_of_the_lowest_value():
+    """-inf beside the lowest finite value, alone and under ordinary logits; and rows of large logits."""
+    low = np.finfo(np.float32).min
+    c = verify_case(9000, [bushy(7, s) for s in range(6)], True, seed=16, greedy=lambda s: False)
+    c["logits"][:, 2000:5000], c["logits"][:, 6000:] = low, -np.inf
+    for row in (0, 7, 14):      # (roots: nothing else in the row)
+        c["logits"][row] = np.where(np.arange(9000) % 3 == 0, np.float32(low), np.float32(-np.inf))
+    c["draft"][7] = np.where(np.arange(9000) % 2 == 0, np.float32(low), np.float32(-np.inf))
+    c["logits"][21, :2000] *= 1e30
+    c["logits"][28] += 3e7
+    assert_verify(c)
+
+
+def test_verify_refuses_vocabularies_above_eight_million():
+    from fusezap_core_b200.kernels.table import KernelError
+    vocab = (8 << 20) + 4
+    logits = torch.zeros((1, vocab), device="cuda")
+    out = [torch.zeros(1, dtype=torch.int32, device="cuda") for _ in range(5)]
+    seg = torch.tensor([[0, 1, 0, 0]], dtype=torch.int32, device="cuda")
+    with pytest.raises(KernelError):
+        ops_of("float32").verify_tree(logits, None, torch.ones(1, device="cuda"), torch.zeros(1, dtype=torch.float64, device="cuda"), out[0], out[1] - 1, seg, *out[2:])
+
+
 @pytest.mark.parametrize("drafter", [True, False])
 def test_verify_keeps_the_targets_distribution(drafter):
     """Over many requests the first token behind the root (a child that stands, or the draw) is distributed as softmax(logits / T):

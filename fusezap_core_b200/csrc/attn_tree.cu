@@ -64,7 +64,7 @@ attn_tree_context_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, 
   const int heads = min(GH, G - part * GH), head0 = kvh * G + part * GH;
   fz_grid_wait();
   int s, node0;
-  const bool there = find_tile(blockIdx.x, A.seg, A.S, NB, s, node0);
+  const bool there = find_tile(blockIdx.x, A.seg, A.S, NB, A.N, (long long)A.mb * A.page_size, s, node0);
   int row0 = 0, nodes = 0, start = 0, first = 0, begin = 0, end = 0;
   if (there) {
     row0 = A.seg[4 * s] + node0;
@@ -76,7 +76,7 @@ attn_tree_context_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, 
     end = min(start, begin + piece);
     if (blockIdx.z == 0 && first + (long long)A.pieces * piece < start && threadIdx.x == 0) atomicOr(A.err, FZ_ERR_POS_RANGE);      // longer than announced
   }
-  if (!there || row0 < 0 || row0 + nodes > A.N || begin >= end) return;
+  if (!there || begin >= end) return;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, rows = nodes * heads;
   const int* trow = A.table + (size_t)s * A.mb;
   const long long head_off = (long long)kvh * A.page_size * A.hd;

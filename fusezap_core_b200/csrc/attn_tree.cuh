@@ -13,13 +13,20 @@ __host__ __device__ __forceinline__ int context_first(int start, int window) {
   return (start - window + 1) & ~63;
 }
 
+// Nodes of a request whose rows lie in the step and whose tree begins within its block table (`places` long); else none of it is touched, and
+// its rows are reported.
+__device__ __forceinline__ int sound_nodes(int row0, int nodes, int start, int N, long long places) {
+  return row0 >= 0 && nodes > 0 && nodes <= N - row0 && start >= 0 && start <= places ? nodes : 0;
+}
+
 // Tile number `tile` of a step whose requests' rows are cut into tiles of NB nodes: its request and its first node within it. The
 // whole warp takes part.
-__device__ __forceinline__ bool find_tile(int tile, const int* __restrict__ seg, int S, int NB, int& s, int& node0) {
+__device__ __forceinline__ bool find_tile(int tile, const int* __restrict__ seg, int S, int NB, int N, long long places, int& s, int& node0) {
   const int lane = threadIdx.x & 31;
   int base = 0;
   for (int s0 = 0; s0 < S; s0 += 32) {
-    const int n = s0 + lane < S ? max(seg[4 * (s0 + lane) + 1], 0) : 0;
+    const int* e = seg + 4 * (s0 + lane);
+    const int n = s0 + lane < S ? sound_nodes(e[0], e[1], e[2], N, places) : 0;
     const int t = (n + NB - 1) / NB;
     int upto = t;
 #pragma unroll
@@ -120,7 +127,8 @@ attn_tree_merge_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, co
 #pragma unroll
   for (int i = 0; i < D; ++i) o[i] = 0.f;
   const bool named = s >= 0 && s < A.S;
-  const int row0 = named ? A.seg[4 * s] : 0, nodes = named ? A.seg[4 * s + 1] : 0, start = named ? A.seg[4 * s + 2] : 0;
+  const int row0 = named ? A.seg[4 * s] : 0, start = named ? A.seg[4 * s + 2] : 0;
+  const int nodes = named ? sound_nodes(row0, A.seg[4 * s + 1], start, A.N, (long long)A.mb * A.page_size) : 0;
   if (!named || n < row0 || n - row0 >= nodes) {      // a padding row
     if (s >= 0 && lane == 0) atomicOr(A.err, FZ_ERR_ROW_RANGE);
     if (mine)

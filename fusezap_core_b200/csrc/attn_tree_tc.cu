@@ -72,7 +72,8 @@ __host__ __device__ __forceinline__ void request_units(int n, int start, int win
 
 struct Sizes {
   const int* seg;
-  int S, NB, Hkv, window;
+  int S, NB, Hkv, window, N;
+  long long places;      // of a block table
 };
 
 // A block's share of an item: `count` key tiles of the places [a, b) from place `key0` on, for `rows` (node, head) rows from row `row` on.
@@ -99,7 +100,9 @@ struct Walk {
     int total = 0;
     for (int s = lane; s < Z.S; s += 32) {
       int a, tiles, row_tiles;
-      request_units(Z.seg[4 * s + 1], Z.seg[4 * s + 2], Z.window, Z.NB, a, tiles, row_tiles);
+      const int* e = Z.seg + 4 * s;
+      const int start = e[2];
+      request_units(sound_nodes(e[0], e[1], start, Z.N, Z.places), start, Z.window, Z.NB, a, tiles, row_tiles);
       total += Z.Hkv * row_tiles * tiles;
     }
     return __reduce_add_sync(0xffffffffu, total);
@@ -112,7 +115,7 @@ struct Walk {
       int nn = 0, bb = 0, rr = 0, aa = 0, tt = 0, rt_ = 0;
       if (s0 + lane < Z.S) {
         const int* e = Z.seg + 4 * (s0 + lane);
-        rr = e[0], nn = e[1], bb = e[2];
+        rr = e[0], bb = e[2], nn = sound_nodes(rr, e[1], bb, Z.N, Z.places);
         request_units(nn, bb, Z.window, Z.NB, aa, tt, rt_);
       }
       const int mine_i = Z.Hkv * rt_, mine_u = mine_i * tt;
@@ -673,7 +676,7 @@ FZ_API int fz_attn_tree_tc(const void* q, const void* k_pool, const void* v_pool
   if (slots > 2147483647LL) return FZ_TOO_LARGE;
   float* part_ml = part + (size_t)slots * BM * hd;
   int2* records = (int2*)(part_ml + (size_t)slots * BM * 2);
-  const Sizes Z = {seg, S, NB, Hkv, window};
+  const Sizes Z = {seg, S, NB, Hkv, window, N, (long long)mb * page_size};
 #define FZ_T(HD_, BOX_) st = launch<HD_, BOX_>(qm, kvm, v_pool, Z, table, mb, page_size, num_pages, N, Hq, scale_log2, blocks, (int)slots, part, part_ml, records, err, stream)
   if (hd == 64 && box == 8) FZ_T(64, 8);
   else if (hd == 64) FZ_T(64, 16);

@@ -33,7 +33,7 @@ keep_rows_kernel(const Pool<V> P, const int* __restrict__ table, int S, int mb, 
   if (nodes <= 0 || kept <= 0) return;
   if (threadIdx.x == 0) s_bad = 0;
   __syncthreads();
-  const bool fits = row0 >= 0 && row0 + nodes <= N && kept <= nodes && kept <= KEEP_NODES;
+  const bool fits = row0 >= 0 && nodes <= N - row0 && kept <= nodes && kept <= KEEP_NODES && start >= 0 && start <= (long long)mb * P.page_size;
   for (int k = threadIdx.x; fits && k < kept; k += KEEP_THREADS) {
     const int from = path[row0 + k];
     int bad = from < k || from >= nodes || (k > 0 && from <= path[row0 + k - 1]) ? FZ_ERR_ROW_RANGE : 0;
@@ -41,10 +41,10 @@ keep_rows_kernel(const Pool<V> P, const int* __restrict__ table, int S, int mb, 
     if (!bad) {
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        const int place = start + (w ? k : from), pi = place / P.page_size;
+        const long long place = (long long)start + (w ? k : from), pi = place / P.page_size;
         const int page = pi < mb ? table[(size_t)s * mb + pi] : -1;
         if (page < 0 || page >= P.num_pages) bad = FZ_ERR_NO_PAGE;
-        at[w] = (long long)page * P.page_stride + (long long)(place - pi * P.page_size) * P.width;
+        at[w] = (long long)page * P.page_stride + (place - pi * P.page_size) * P.width;
       }
     }
     if (bad) atomicOr(&s_bad, bad);

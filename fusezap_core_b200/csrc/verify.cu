@@ -317,7 +317,7 @@ verify_stats_kernel(const float* __restrict__ logits, const float* __restrict__ 
       n = __shfl_sync(0xffffffffu, sg.y, who);
     }
   }
-  if (s < 0 || row0 + n > N || n > MAX_NODES) return;
+  if (s < 0 || row0 < 0 || n > N - row0 || n > MAX_NODES) return;
   const float T = temperature_of(temperature, s);
   const bool greedy = !(T > 0.f);
   bool with_q = false;
@@ -357,7 +357,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
   const int row0 = seg[4 * s], n = seg[4 * s + 1];
   const float T = temperature_of(temperature, s);
   const bool first = rank == 0 && tid == 0;
-  if (n <= 0 || row0 < 0 || row0 + n > N || n > MAX_NODES) {      // (the whole cluster)
+  if (n <= 0 || row0 < 0 || n > N - row0 || n > MAX_NODES) {      // (the whole cluster)
     if (first) {
       if (n > 0) atomicOr(err, FZ_ERR_ROW_RANGE);
       count[s] = 0;

@@ -453,7 +453,8 @@ class StepRunner:
     # ---- drafted trees: what stands, and the cache afterwards
     def verify(self, logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.Tensor,
                draft: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-        """`Ops.verify_tree` on the step just run, every row of which was wanted: (path (N,), count (S,), next ids (S,)), on the device.
+        """`Ops.verify_tree` on the step just run, every row of which was wanted: (path (N,), count (S,), next ids (S,)), on the device,
+        until the next call.
         temperature (S,) float32 and uniform (N,) float64 on the device, S and N the step's requests and rows; draft: the drafter's
         logits (N, vocab), or None."""
         meta = self.meta

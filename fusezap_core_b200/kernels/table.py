@@ -863,7 +863,7 @@ class CudaOps(Ops):
             if self.drafts.fz_attn_tree_check(num_heads, num_kv_heads, head_dim) != 0:
                 raise KernelError(f"tree_attention: {num_heads} heads, {num_kv_heads} kv heads, head_dim {head_dim} (need heads % kv_heads == 0, "
                                   f"head_dim % 16 == 0 and head_dim <= 512)")
-            tc = self.use_tensor_cores and self.drafts_tc.fz_attn_tree_tc_check(*key) == 0
+            tc = self.dtype == torch.bfloat16 and self.drafts_tc.fz_attn_tree_tc_check(*key) == 0
             self._tree_sizes[key] = tc
         return tc
 
@@ -888,7 +888,7 @@ class CudaOps(Ops):
             return
         # scratch of the call alone (from the stream's allocator, or the graph's that records it): two calls never share it.
         # Tensor cores: keys and values in one pool, (pages, 2, kv heads, page size, head size)
-        if tc and self.tree_tensor_cores and page_stride == 2 * num_kv_heads * page_size * head_dim and vp - kp == page_stride // 2 * k.element_size():
+        if tc and self.use_tensor_cores and self.tree_tensor_cores and page_stride == 2 * num_kv_heads * page_size * head_dim and vp - kp == page_stride // 2 * k.element_size():
             slots = self.drafts_tc.fz_attn_tree_tc_slots(n, segments, num_heads, num_kv_heads)
             part = torch.empty(slots * 128 * (head_dim + 2) + 2 * n * num_kv_heads, dtype=torch.float32, device=self.device)
             self._launch(self.drafts_tc.fz_attn_tree_tc, "tree_attention (tensor cores)",

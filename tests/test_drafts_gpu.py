@@ -193,6 +193,28 @@ def test_tree_attention_rows_that_see_nothing(dtype):
     assert_tree(c, out)
 
 
+# what no request's (first row, rows, first place) is, by field
+BAD_SEGMENTS = [(0, -4), (0, 2 ** 31 - 3), (1, 2 ** 31 - 1), (1, 60), (2, -100), (2, 2 ** 31 - 1)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("field,value", BAD_SEGMENTS)
+def test_tree_attention_reports_requests_outside_the_step(dtype, field, value):
+    from fusezap_core_b200.kernels.table import KernelError
+    c = tree_case(dtype, 8, 2, 64, 16, [(45, bushy(6)), (150, bushy(9)), (20, bushy(5))], pad=2)
+    good = [*range(6), *range(15, 22)]
+    c.meta.seg[1, field] = value
+    q, cache, meta = on_gpu(c)
+    out = torch.full_like(q, NAN)
+    ops = ops_of(dtype)
+    ops.tree_attention(q, cache, meta, out, c.heads, c.kv, c.hd, c.scale, 0)
+    with pytest.raises(KernelError, match="outside the step"):
+        ops.check_errors()
+    assert (out[6:15] == 0).all()
+    c.meta.seg[1] = torch.tensor([6, 9, 150, -1])
+    assert_tree(c, out, good)
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("bad", [NAN, float("inf")])
 def test_tree_attention_unseen_places_take_no_part(dtype, bad):
@@ -538,6 +560,28 @@ def test_keep_rows_leaves_a_request_whose_path_is_none():
             ops.check_errors()
         bad = [0, 1] if why != "no page" else [2]
         assert torch.equal(now[:, bad], was[:, bad])
+
+
+@pytest.mark.parametrize("field,value", BAD_SEGMENTS)
+def test_moved_rows_and_verdicts_of_requests_outside_the_step(field, value):
+    from fusezap_core_b200.kernels.table import KernelError
+    ops = ops_of("float32")
+    table = torch.tensor([[0, 1, 4], [2, 3, 5]], dtype=torch.int32, device="cuda")
+    seg = torch.tensor([[0, 6, 1, -1], [6, 5, 3, -1]], dtype=torch.int32)
+    seg[1, field] = value
+    pool = torch.randn(2, 6, 2, 3, 4, 8, device="cuda")
+    path = torch.tensor([0, 2, 4, -1, -1, -1, 0, 4, -1, -1, -1], dtype=torch.int32, device="cuda")
+    was, now = pool.clone(), pool.clone()
+    ops.keep_rows(now, table, seg.cuda(), path, torch.tensor([3, 2], dtype=torch.int32, device="cuda"))
+    with pytest.raises(KernelError, match="outside the step"):
+        ops.check_errors()
+    assert torch.equal(now[:, [2, 3, 5]], was[:, [2, 3, 5]]) and not torch.equal(now[:, [0, 1, 4]], was[:, [0, 1, 4]])
+    if field == 2:
+        return      # (verdicts do not read it)
+    c = verify_case(3000, [chain(6), chain(5)], True, greedy=lambda s: False)
+    c["seg"][1, field] = value
+    with pytest.raises(KernelError, match="outside the step"):
+        run_verify(c)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])

@@ -4,8 +4,8 @@
 // and values are fetched once for all of them. Work is counted in units, a key tile of 128 places for one (request, kv head, row
 // tile) item; the persistent grid has one block per SM and every block takes an equal run of the units, whatever the requests'
 // lengths: a run cuts items where it must, at most one at either end. Each stretch of an item leaves unnormalised rows and
-// (maximum, sum) in float32 scratch, in slot block + item (both rise along the runs, so no two stretches share one); the merge
-// kernel finds a row's stretches by the same arithmetic. Nothing is planned on the host and no launch size depends on the requests'
+// (maximum, sum) in float32 scratch, from scratch row 128 * block + the rows of the items before (both rise along the runs, and an
+// item has 128 rows at most, so no two stretches overlap); the merge kernel finds a row's stretches by a record. Nothing is planned on the host and no launch size depends on the requests'
 // lengths. (The cuts follow from all requests of the step together: a row's last bits may depend on its neighbours.)
 // Bound by HBM up to about 128 rows per kv head: 64 KB of keys and values per unit at head size 128, 1.5 us of an SM's share of
 // the bandwidth, against 1,024 clocks of MMA and as many of exponentials. Blocks of 19 warps:
@@ -77,9 +77,9 @@ struct Sizes {
 };
 
 // A block's share of an item: `count` key tiles of the places [a, b) from place `key0` on, for `rows` (node, head) rows from row `row` on.
-// stretches: how many the item has in all where this is its first, else 0.
+// before: (node, head) rows of the items before it; stretches: how many the item has in all where this is its first, else 0.
 struct Stretch {
-  int s, kvh, row, rows, key0, count, a, b, item, stretches;
+  int s, kvh, row, rows, key0, count, a, b, before, stretches;
 };
 constexpr int RING = 8;      // stretches that the key producer may be ahead of the others' reading (the queries' one buffer keeps it within four)
 
@@ -90,9 +90,9 @@ constexpr int RING = 8;      // stretches that the key producer may be ahead of 
 struct Walk {
   int G, u, u1;                                    // the next unit, the run's end
   int s, n, row0, a, b, tiles, row_tiles;          // the request
-  int end, first_item;                             // its last unit + 1, its first item
-  int chunk, chunk_units, chunk_items;             // where the look-up goes on: 32 requests from `chunk`, units and items before them
-  int kvh, rt, item;                               // the item
+  int end, nodes_before;                           // its last unit + 1, nodes of the requests before it
+  int chunk, chunk_units, chunk_nodes;             // where the look-up goes on: 32 requests from `chunk`, units and nodes before them
+  int kvh, rt;                                     // the item
 
   // Sum of all requests' units.
   static __device__ __forceinline__ int sum(const Sizes& Z) {
@@ -110,7 +110,7 @@ struct Walk {
   // The request that holds unit u, and the item and tile within it.
   __device__ __forceinline__ void find(const Sizes& Z) {
     const int lane = threadIdx.x & 31;
-    int units = chunk_units, items = chunk_items;
+    int units = chunk_units, nodes = chunk_nodes;
     for (int s0 = chunk; s0 < Z.S; s0 += 32) {
       int nn = 0, bb = 0, rr = 0, aa = 0, tt = 0, rt_ = 0;
       if (s0 + lane < Z.S) {
@@ -118,32 +118,31 @@ struct Walk {
         rr = e[0], bb = e[2], nn = sound_nodes(rr, e[1], bb, Z.N, Z.places);
         request_units(nn, bb, Z.window, Z.NB, aa, tt, rt_);
       }
-      const int mine_i = Z.Hkv * rt_, mine_u = mine_i * tt;
-      int iu = mine_u, ii = mine_i;
+      const int mine_u = Z.Hkv * rt_ * tt;
+      int iu = mine_u, in = nn;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, iu, o), y = __shfl_up_sync(0xffffffffu, ii, o);
-        if (lane >= o) { iu += x; ii += y; }
+        const int x = __shfl_up_sync(0xffffffffu, iu, o), y = __shfl_up_sync(0xffffffffu, in, o);
+        if (lane >= o) { iu += x; in += y; }
       }
       const unsigned hit = __ballot_sync(0xffffffffu, units + iu > u);
       if (hit) {
         const int who = __ffs(hit) - 1;
-        chunk = s0, chunk_units = units, chunk_items = items;
+        chunk = s0, chunk_units = units, chunk_nodes = nodes;
         s = s0 + who;
         n = __shfl_sync(0xffffffffu, nn, who), b = __shfl_sync(0xffffffffu, bb, who), row0 = __shfl_sync(0xffffffffu, rr, who);
         a = __shfl_sync(0xffffffffu, aa, who), tiles = __shfl_sync(0xffffffffu, tt, who), row_tiles = __shfl_sync(0xffffffffu, rt_, who);
         end = units + __shfl_sync(0xffffffffu, iu, who);
         const int begin = end - __shfl_sync(0xffffffffu, mine_u, who);
-        first_item = items + __shfl_sync(0xffffffffu, ii - mine_i, who);
+        nodes_before = nodes + __shfl_sync(0xffffffffu, in - nn, who);
         const int within = u - begin, k = within / tiles;
         kvh = k / row_tiles;
         rt = k - kvh * row_tiles;
-        item = first_item + k;
         tile = within - k * tiles;
         return;
       }
       units += __shfl_sync(0xffffffffu, iu, 31);
-      items += __shfl_sync(0xffffffffu, ii, 31);
+      nodes += __shfl_sync(0xffffffffu, in, 31);
     }
   }
   int tile;      // the stretch's first within its item
@@ -154,11 +153,11 @@ struct Walk {
       find(Z);
     } else {
       tile = 0;
-      ++item;
       if (++rt == row_tiles) rt = 0, ++kvh;
     }
     const int node0 = rt * Z.NB, count = min(tiles - tile, u1 - u);
-    x = {s, kvh, row0 + node0, min(Z.NB, n - node0) * G, (a / BN + tile) * BN, count, a, b, item,
+    x = {s, kvh, row0 + node0, min(Z.NB, n - node0) * G, (a / BN + tile) * BN, count, a, b,
+         (nodes_before * Z.Hkv + kvh * n + node0) * G,
          tile == 0 ? (u + tiles - 1) / share - u / share + 1 : 0};
     u += count;
     return true;
@@ -169,7 +168,7 @@ template <int HD, int BOX>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map, const __nv_bfloat16* __restrict__ v_pool,
                     const Sizes Z, const int* __restrict__ table, int mb, int page_size, int num_pages, int Hq, float scale_log2,
-                    int N, int slots, float* __restrict__ part_o, float* __restrict__ part_ml, int2* __restrict__ records, int* err) {
+                    int N, float* __restrict__ part_o, float* __restrict__ part_ml, int2* __restrict__ records, int* err) {
   constexpr int HALVES = HD / 64;                     // 64-column halves of a head
   constexpr int STAGES = HD <= 64 ? 6 : 3;            // key tiles and value tiles in flight
   constexpr int HALF_BYTES = 128 * 128;               // 128 rows of 128 bytes
@@ -243,7 +242,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     const int rows_per_page = 2 * Z.Hkv * page_size;
     int g = 0, n_q = 0;
     Walk walk;
-    walk.G = G, walk.u = u0, walk.u1 = u1, walk.end = walk.chunk = walk.chunk_units = walk.chunk_items = 0;
+    walk.G = G, walk.u = u0, walk.u1 = u1, walk.end = walk.chunk = walk.chunk_units = walk.chunk_nodes = 0;
     while (ok && g < u1 - u0) {
       if (is_v) {
         if (!(ok = read(n_q++))) break;
@@ -402,10 +401,10 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     int g0 = 0, n_x = 0, n_s = 0, n_o[2] = {0, 0};      // tiles of the block, of this stream, and stretches with tiles of either stream so far
     while (ok && g0 < u1 - u0) {
       if (!(ok = read(n_x++))) break;
-      // which slots the item's rows will find their stretches in, from the block that has its first: (first slot, stretches)
+      // where the item's rows will find their stretches, from the block that has its first: (scratch row of the first, stretches)
       if (x.stretches > 0 && idx == 0) {
         for (int i = lane; i < x.rows / G; i += 32)
-          if (x.row + i < N) records[(size_t)(x.row + i) * Z.Hkv + x.kvh] = make_int2(blockIdx.x + x.item, x.stretches);
+          records[(size_t)(x.row + i) * Z.Hkv + x.kvh] = make_int2(blockIdx.x * BM + x.before, x.stretches);
       }
       const bool live = quad * 32 < x.rows;      // (the warp has rows)
       const int first = (g0 ^ tq) & 1;           // the first tile of the stretch that is this stream's
@@ -523,9 +522,9 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
       asm volatile("bar.sync %0, 128;" ::"r"(quad_bar) : "memory");
       const float f0 = fast_exp2(m0 - mu), f1 = fast_exp2(m1 - mu);      // (a stream without tiles: maximum -inf, weight 0)
       const float l = (s_mx[r] + s_mx[BM + r]) * f0 + (s_mx[2 * BM + r] + s_mx[3 * BM + r]) * f1;
-      const size_t slot0 = ((size_t)(blockIdx.x + x.item)) * BM;
-      const bool in_slots = (int)blockIdx.x + x.item < slots;
-      if (!in_slots && lane == 0) atomicOr(err, FZ_ERR_ROW_RANGE);      // (requests with more rows than the step has)
+      const size_t row0 = (size_t)blockIdx.x * BM + x.before;
+      const bool fits = x.before >= 0 && x.before <= N * Hq - x.rows;
+      if (!fits && lane == 0) atomicOr(err, FZ_ERR_ROW_RANGE);      // (requests that share rows)
       // A lane has one row: a store instruction would touch 32 lines with 16 bytes each. So every four lanes exchange first, four vectors
       // of four dimensions each: then a lane has vector `lane % 4` of all four rows, and an instruction writes 64 bytes of eight rows.
       const int d0 = (tq * 2 + hf) * JD, base = quad * 32 + (lane & ~3);
@@ -552,10 +551,10 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)      // (a[4 j ..] is now vector lane % 4 of row `base + j`)
-          if (in_slots && base + j < x.rows)
-            *(float4*)(part_o + (slot0 + base + j) * HD + d0 + c + 4 * (lane & 3)) = make_float4(a[4 * j], a[4 * j + 1], a[4 * j + 2], a[4 * j + 3]);
+          if (fits && base + j < x.rows)
+            *(float4*)(part_o + (row0 + base + j) * HD + d0 + c + 4 * (lane & 3)) = make_float4(a[4 * j], a[4 * j + 1], a[4 * j + 2], a[4 * j + 3]);
       }
-      if (in_slots && r < x.rows && d0 == 0) *(float2*)(part_ml + 2 * (slot0 + r)) = make_float2(m, l);
+      if (fits && r < x.rows && d0 == 0) *(float2*)(part_ml + 2 * (row0 + r)) = make_float2(m, l);
       // nobody of this row quarter starts on the next stretch's tiles (whose products overwrite O) before all four have read
       tc_fence_before();
       asm volatile("bar.sync %0, 128;" ::"r"(quad_bar) : "memory");
@@ -575,7 +574,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
 struct Stretches {
   const float *part_o, *part_ml;
   const int2* records;
-  int NB, Hkv, window, slots;
+  int NB, Hkv, window, rows;      // rows: of the scratch
   __device__ __forceinline__ int2 early(int n, int kvh) const { return records[(size_t)n * Hkv + kvh]; }
   __device__ __forceinline__ Range range(int2 record, int, int, int node, int head_in_group, int group, int nodes, int start, int pos) const {
     int a, tiles, row_tiles;
@@ -586,9 +585,9 @@ struct Stretches {
       x.extra_from = max(0, pos - window + 1);
       x.extra_to = min(a, start);
     }
-    const bool there = tiles > 0 && record.x >= 0 && record.y > 0 && record.x <= slots - record.y;
+    const bool there = tiles > 0 && record.x >= 0 && record.y > 0 && record.y <= rows / BM && record.x <= rows - BM * record.y;
     x.pieces = there ? record.y : 0;
-    x.first = there ? (size_t)record.x * BM + (node % NB) * group + head_in_group : 0;
+    x.first = there ? (size_t)record.x + (node % NB) * group + head_in_group : 0;
     x.step = BM;
     return x;
   }
@@ -626,14 +625,14 @@ int pool_map(const void* pool, long long rows, int hd, int box_rows, CUtensorMap
 
 template <int HD, int BOX>
 int launch(const CUtensorMap& qm, const CUtensorMap& kvm, const void* v_pool, const Sizes& Z, const int* table, int mb, int page_size, int num_pages,
-           int N, int Hq, float scale_log2, int blocks, int slots, float* part_o, float* part_ml, int2* records, int* err, cudaStream_t stream) {
+           int N, int Hq, float scale_log2, int blocks, float* part_o, float* part_ml, int2* records, int* err, cudaStream_t stream) {
   constexpr int HALVES = HD / 64, STAGES = HD <= 64 ? 6 : 3;
   constexpr size_t smem = (size_t)HALVES * 128 * 128 * (1 + 2 * STAGES) + 4 * BM * 4 + 8 * (8 + 4 * STAGES + RING) + RING * sizeof(Stretch) + 8;
   static_assert(smem <= FZ_MOST_SMEM);
   auto kern = attn_tree_tc_kernel<HD, BOX>;
   FZ_RAISE_SMEM(kern);
   const cudaError_t e = fz_launch(kern, dim3((unsigned)blocks), dim3(THREADS), smem, stream, qm, kvm, (const __nv_bfloat16*)v_pool, Z, table, mb, page_size,
-                                  num_pages, Hq, scale_log2, N, slots, part_o, part_ml, records, err);
+                                  num_pages, Hq, scale_log2, N, part_o, part_ml, records, err);
   return e == cudaSuccess ? FZ_OK : (int)e;
 }
 }  // namespace
@@ -646,13 +645,9 @@ FZ_API int fz_attn_tree_tc_check(int Hq, int Hkv, int hd, int page_size) {
   return FZ_OK;
 }
 
-// Slots of the scratch (each 128 * (hd + 2) floats; behind them 2 * N * Hkv ints): a step's stretches are fewer than its blocks and items
-// together.
-FZ_API long long fz_attn_tree_tc_slots(int N, int S, int Hq, int Hkv) {
-  const int NB = BM / (Hq / Hkv);
-  const long long tiles = (long long)N / NB + S;
-  return sm_count() + Hkv * (tiles < N ? tiles : N);
-}
+// Rows of the scratch (each hd + 2 floats; behind them 2 * N * Hkv ints): every (node, head) once, and once more where a block's run cuts its
+// item.
+FZ_API long long fz_attn_tree_tc_rows(int N, int Hq) { return (long long)N * Hq + (long long)BM * sm_count(); }
 
 // As fz_attn_tree; k_pool and v_pool are the two parts of one pool (pages, 2, Hkv, page_size, hd) of num_pages pages.
 FZ_API int fz_attn_tree_tc(const void* q, const void* k_pool, const void* v_pool, const int* pos, const int* seq_row, const int* seg, int S,
@@ -672,19 +667,19 @@ FZ_API int fz_attn_tree_tc(const void* q, const void* k_pool, const void* v_pool
   const int box = page_size == 8 ? 8 : 16;
   if ((st = pool_map(k_pool, pool_rows, hd, box, &kvm)) != FZ_OK) return st;
   const float scale_log2 = scale * 1.4426950408889634f;
-  const long long slots = fz_attn_tree_tc_slots(N, S, Hq, Hkv);
-  if (slots > 2147483647LL) return FZ_TOO_LARGE;
-  float* part_ml = part + (size_t)slots * BM * hd;
-  int2* records = (int2*)(part_ml + (size_t)slots * BM * 2);
+  const long long rows = fz_attn_tree_tc_rows(N, Hq);
+  if (rows > 2147483647LL) return FZ_TOO_LARGE;
+  float* part_ml = part + (size_t)rows * hd;
+  int2* records = (int2*)(part_ml + (size_t)rows * 2);
   const Sizes Z = {seg, S, NB, Hkv, window, N, (long long)mb * page_size};
-#define FZ_T(HD_, BOX_) st = launch<HD_, BOX_>(qm, kvm, v_pool, Z, table, mb, page_size, num_pages, N, Hq, scale_log2, blocks, (int)slots, part, part_ml, records, err, stream)
+#define FZ_T(HD_, BOX_) st = launch<HD_, BOX_>(qm, kvm, v_pool, Z, table, mb, page_size, num_pages, N, Hq, scale_log2, blocks, part, part_ml, records, err, stream)
   if (hd == 64 && box == 8) FZ_T(64, 8);
   else if (hd == 64) FZ_T(64, 16);
   else if (box == 8) FZ_T(128, 8);
   else FZ_T(128, 16);
 #undef FZ_T
   if (st != FZ_OK) return st;
-  const Stretches P = {part, part_ml, records, NB, Hkv, window, (int)slots};
+  const Stretches P = {part, part_ml, records, NB, Hkv, window, (int)rows};
   const TreeArgs R = {pos, seq_row, seg, ancestors, table, S, words, mb, page_stride, page_size, num_pages, N, Hq, Hkv, hd, scale_log2, window, err};
   return launch_merge<__nv_bfloat16>((const __nv_bfloat16*)q, (const __nv_bfloat16*)k_pool, (const __nv_bfloat16*)v_pool, (__nv_bfloat16*)out, P, R, stream);
 }

@@ -464,7 +464,8 @@ class Ops:
         the places b + i for the bits i set in meta.ancestors[n] (int32 (N, words), bit i % 32 of word i // 32; a node's own bit
         among them; bits at and beyond the tree's rows count as unset). A place that a row does not see takes no part whatever
         it holds. A row that sees no place, and a row of padding, gives zeros. meta.max_context: no b + rows is larger.
-        The places' pages: meta.table(cache.group). float32: a row's sums do not depend on the other requests of the step; a
+        scale > 0. Requests share no rows; one whose rows lie outside the step, or whose tree begins behind its table, is an error and its rows
+        give zeros. The places' pages: meta.table(cache.group). float32: a row's sums do not depend on the other requests of the step; a
         table may cut long contexts of bfloat16 steps by the step's size."""
         raise NotImplementedError
 
@@ -479,7 +480,7 @@ class Ops:
         From the root on, with p = softmax(logits / T) and q = softmax(draft / T) of the node (draft None: q is all on the child):
         the node's children x in rising order: x stands if uniform * q(x) < p(x), and the walk goes on from it; else p = max(p - q, 0)
         over its sum (if that is not 0) and q loses x, scaled to sum 1. No child stands: next_ids[s] is the token at which the
-        running sum of p, in index order, first exceeds uniform[root] * total. T <= 0: the first child that is the argmax
+        running sum of p, in index order, first exceeds uniform[root] * total. T <= 0 or a NaN: the first child that is the argmax
         (the order of `argmax`) stands, else the argmax is the next token. float64. A row without a distribution (a NaN, +inf, or
         nothing above -inf): no child stands and the draw gives V - 1 (a drafter's row: no child stands and p is
         drawn from). At most 8,388,608 tokens.

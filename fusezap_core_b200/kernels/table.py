@@ -241,7 +241,7 @@ class CudaOps(Ops):
         if self._drafts_tc is None:
             lib = load("fzb200_drafts_tc")
             P, I, L, F = c_void_p, c_int, c_longlong, c_float
-            lib.fz_attn_tree_tc_slots.restype = L
+            lib.fz_attn_tree_tc_rows.restype = L
             lib.fz_attn_tree_tc.argtypes = [P] * 6 + [I, P, I, P, I, L, I, I, P, I, I, I, I, F, I, P, P, P]
             self._drafts_tc = lib
         return self._drafts_tc
@@ -882,6 +882,8 @@ class CudaOps(Ops):
         self._here(pos, "positions", torch.int32, (n,))
         self._here(row, "table rows", torch.int32, (n,))
         self._here(bits, "ancestors", torch.int32, (n, words))
+        if not scale > 0:
+            raise KernelError(f"tree_attention: the scale is {scale}; it has to be positive")
         page_size, kp, vp = cache.page_size, k.data_ptr(), v.data_ptr()
         tc = self._tree_kernel(num_heads, num_kv_heads, head_dim, page_size)
         if n == 0:
@@ -889,8 +891,7 @@ class CudaOps(Ops):
         # scratch of the call alone (from the stream's allocator, or the graph's that records it): two calls never share it.
         # Tensor cores: keys and values in one pool, (pages, 2, kv heads, page size, head size)
         if tc and self.use_tensor_cores and self.tree_tensor_cores and page_stride == 2 * num_kv_heads * page_size * head_dim and vp - kp == page_stride // 2 * k.element_size():
-            slots = self.drafts_tc.fz_attn_tree_tc_slots(n, segments, num_heads, num_kv_heads)
-            part = torch.empty(slots * 128 * (head_dim + 2) + 2 * n * num_kv_heads, dtype=torch.float32, device=self.device)
+            part = torch.empty(self.drafts_tc.fz_attn_tree_tc_rows(n, num_heads) * (head_dim + 2) + 2 * n * num_kv_heads, dtype=torch.float32, device=self.device)
             self._launch(self.drafts_tc.fz_attn_tree_tc, "tree_attention (tensor cores)",
                          (q.data_ptr(), kp, vp, pos.data_ptr(), row.data_ptr(), seg.data_ptr(), segments, bits.data_ptr(), words, table.data_ptr(), pages,
                           page_stride, page_size, k.shape[0], out.data_ptr(), n, num_heads, num_kv_heads, head_dim, scale, window, part.data_ptr(),

@@ -182,6 +182,19 @@ def test_tree_attention_many_requests_and_empty_ones(dtype):
     assert (out[-5:] == 0).all()
 
 
+def test_tree_attention_requests_that_share_rows_are_reported():
+    """Two requests that name the same rows: the scratch has room for every row once."""
+    from fusezap_core_b200.kernels.table import KernelError
+    c = tree_case("bfloat16", 8, 2, 64, 16, [(300, bushy(30)), (300, bushy(30, 1))])
+    c.meta.seg[0] = c.meta.seg[1]
+    c.meta.seg[:, 0], c.meta.seg[:, 1] = 0, 60
+    q, cache, meta = on_gpu(c)
+    ops = ops_of("bfloat16")
+    ops.tree_attention(q, cache, meta, torch.empty_like(q), c.heads, c.kv, c.hd, c.scale, 0)
+    with pytest.raises(KernelError, match="outside the step"):
+        ops.check_errors()
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_tree_attention_rows_that_see_nothing(dtype):
     c = tree_case(dtype, 8, 2, 64, 16, [(0, bushy(6)), (50, bushy(6))])
@@ -620,12 +633,14 @@ def test_refusals():
     q, cache, meta = on_gpu(c)
     out = torch.empty_like(q)
 
-    def refused(match, q=q, cache=cache, out=out, heads=8, kv=2, hd=64, **other):
+    def refused(match, q=q, cache=cache, out=out, heads=8, kv=2, hd=64, scale=0.1, **other):
         m = SimpleNamespace(**{**vars(meta), **other})
         with pytest.raises(KernelError, match=match):
-            ops.tree_attention(q, cache, m, out, heads, kv, hd, 0.1, 0)
+            ops.tree_attention(q, cache, m, out, heads, kv, hd, scale, 0)
 
     refused("dtype", q=q.float())
+    refused("scale", scale=0.0)
+    refused("scale", scale=NAN)
     refused("is on cpu", q=q.cpu())
     refused("shape", out=out[:-1])
     refused("shape", pos=meta.pos[:-1])

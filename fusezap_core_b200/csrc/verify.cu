@@ -39,6 +39,9 @@ __device__ __forceinline__ float temperature_of(const float* temperature, int s)
   return t > 1e30f ? 1e30f : t;
 }
 
+// Whether a request has rows, all of them in the step, and no more than a tree may have; else it has no verdict, and no row is its own.
+__device__ __forceinline__ bool sound(int row0, int n, int N) { return n > 0 && row0 >= 0 && n <= N - row0 && n <= MAX_NODES; }
+
 struct Ref {      // a row's scale: token x weighs exp((x - top) / T)
   double scale, top;      // 128 log2(e) / T, and the row's maximum
   unsigned far;           // the high word of the difference at which a token would weigh 2^-1015: below it tokens weigh exactly 0
@@ -309,7 +312,7 @@ verify_stats_kernel(const float* __restrict__ logits, const float* __restrict__ 
   int s = -1, row0 = 0, n = 0;
   for (int s0 = 0; s0 < S && s < 0; s0 += 32) {
     const int2 sg = s0 + lane < S ? make_int2(seg[4 * (s0 + lane)], seg[4 * (s0 + lane) + 1]) : make_int2(0, 0);
-    const unsigned hit = __ballot_sync(0xffffffffu, row >= sg.x && row - sg.x < sg.y);
+    const unsigned hit = __ballot_sync(0xffffffffu, sound(sg.x, sg.y, N) && row >= sg.x && row - sg.x < sg.y);
     if (hit) {
       const int who = __ffs(hit) - 1;
       s = s0 + who;
@@ -317,7 +320,7 @@ verify_stats_kernel(const float* __restrict__ logits, const float* __restrict__ 
       n = __shfl_sync(0xffffffffu, sg.y, who);
     }
   }
-  if (s < 0 || row0 < 0 || n > N - row0 || n > MAX_NODES) return;
+  if (s < 0) return;
   const float T = temperature_of(temperature, s);
   const bool greedy = !(T > 0.f);
   bool with_q = false;
@@ -357,7 +360,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
   const int row0 = seg[4 * s], n = seg[4 * s + 1];
   const float T = temperature_of(temperature, s);
   const bool first = rank == 0 && tid == 0;
-  if (n <= 0 || row0 < 0 || n > N - row0 || n > MAX_NODES) {      // (the whole cluster)
+  if (!sound(row0, n, N)) {      // (the whole cluster)
     if (first) {
       if (n > 0) atomicOr(err, FZ_ERR_ROW_RANGE);
       count[s] = 0;

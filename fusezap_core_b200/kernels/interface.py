@@ -476,7 +476,8 @@ class Ops:
         target's at every node; draft (N, V) float32: the drafter's at every node (row n gave n's children), or None: the children
         were not drawn from probabilities; temperature (S,) float32, of both (above 1e30: 1e30); uniform (N,) float64 in [0, 1): a child's own
         number, the root's for the draw at the end; tokens, parents (N,) int32: parent = node within the request's rows, before the
-        child; node 0 is the root, whose token stands; seg (S, 4) int32 = (first row, rows, anything, anything), at most 1,024 rows.
+        child; node 0 is the root, whose token stands; seg (S, 4) int32 = (first row, rows, anything, anything), at most 1,024 rows. Requests
+        share no rows; one whose rows do not lie in the step is an error and has no verdict, the others have theirs.
         From the root on, with p = softmax(logits / T) and q = softmax(draft / T) of the node (draft None: q is all on the child):
         the node's children x in rising order: x stands if uniform * q(x) < p(x), and the walk goes on from it; else p = max(p - q, 0)
         over its sum (if that is not 0) and q loses x, scaled to sum 1. No child stands: next_ids[s] is the token at which the
@@ -484,7 +485,7 @@ class Ops:
         (the order of `argmax`) stands, else the argmax is the next token. float64. A row without a distribution (a NaN, +inf, or
         nothing above -inf): no child stands and the draw gives V - 1 (a drafter's row: no child stands and p is
         drawn from). At most 8,388,608 tokens.
-        Results, int32: count[s] kept nodes (the root among them; 0 for no rows, next_ids[s] = -1); path[first row + k] = node of the
+        Results, int32: count[s] kept nodes (the root among them; 0 for no rows and for no verdict, next_ids[s] = -1); path[first row + k] = node of the
         k-th of them, -1 from count[s] to the request's last row; rows of `path` beside the requests' are left."""
         raise NotImplementedError
 

@@ -526,6 +526,35 @@ def test_verify_reports_bad_trees():
         run_verify(c)
 
 
+# ---- verdicts: requests that are none beside sound ones, and sums near their borders
+
+@pytest.mark.parametrize("drafter", [True, False])
+@pytest.mark.parametrize("bad", [(0, 2 ** 31 - 1), (0, 17), (-4, 20), (-(2 ** 31), 2 ** 31 - 1), (-(2 ** 31), 2 ** 31 - 8), (2 ** 31 - 1, 3), (3, 0), (2, -7)])
+def test_verify_beside_requests_that_are_none(bad, drafter):
+    """A first request whose rows do not lie in the step but would cover the others': it alone has no verdict. Steps whose rows' statistics
+    are taken ahead of the walks (2 to 6 rows a request), the scratch holding what it likes."""
+    from fusezap_core_b200.kernels.table import KernelError
+    c = verify_case(3000, [chain(4), bushy(4, 1), chain(4), bushy(4, 2)], drafter, seed=21, greedy=lambda s: s == 2)
+    c["seg"][0, :2] = bad
+    dev = {k: None if v is None else torch.from_numpy(v).cuda() for k, v in c.items()}
+    out = [torch.full((k,), -7, dtype=torch.int32, device="cuda") for k in (16, 4, 4)]
+    ops = ops_of("float32")
+    garbage = [torch.full((16 * 24 * k,), 255, dtype=torch.uint8, device="cuda") for k in (1, 2, 4)]
+    del garbage
+    ops.verify_tree(dev["logits"], dev["draft"], dev["temperature"], dev["uniform"], dev["tokens"], dev["parents"], dev["seg"], *out)
+    if bad[1] > 0:
+        with pytest.raises(KernelError, match="outside the step"):
+            ops.check_errors()
+    ops.check_errors()
+    path, count, ids = (t.cpu().numpy() for t in out)
+    c["seg"][0, :2] = 0
+    rpath, rcount, rids = plain.verify(c["logits"], c["draft"], c["temperature"], c["uniform"], c["tokens"], c["parents"], c["seg"])
+    np.testing.assert_array_equal(count, rcount)
+    np.testing.assert_array_equal(ids, rids)
+    np.testing.assert_array_equal(path[4:], rpath[4:])
+    assert (path[:4] == -7).all()
+
+
 # ---------------------------------------------------------------------------------------------- rows and pages moved
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])

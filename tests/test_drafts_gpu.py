@@ -555,6 +555,29 @@ def test_verify_beside_requests_that_are_none(bad, drafter):
     assert (path[:4] == -7).all()
 
 
+def test_verify_draws_at_a_rounding_from_the_border():
+    """Rows of two tokens and numbers just below and above the first one's share, taken to 40 digits. The share is off by at most
+    1.7e-15 of itself: a weight exp(-t), t <= 4, by 4 * 2^-52 for its exponent's rounded scale and 6e-16 for the table, the polynomial and
+    their products, then a sum and a product. The numbers are 2^-48 = 3.6e-15 away."""
+    from decimal import Decimal, localcontext
+    rng = np.random.default_rng(22)
+    S = 3000
+    temperature = rng.uniform(0.5, 2.0, S).astype(np.float32)
+    logits = (rng.uniform(-1, 1, (S, 2)) * temperature[:, None]).astype(np.float32)
+    above = rng.integers(0, 2, S)
+    uniform = np.empty(S)
+    with localcontext() as ctx:
+        ctx.prec = 40
+        for s in range(S):
+            share = 1 / (1 + ((Decimal(float(logits[s, 1])) - Decimal(float(logits[s, 0]))) / Decimal(float(temperature[s]))).exp())
+            uniform[s] = float(share * (1 + (1 if above[s] else -1) * Decimal(2) ** -48))
+    seg = np.stack([np.arange(S), np.ones(S), np.zeros(S), np.zeros(S)], 1).astype(np.int32)
+    _, count, ids = run_verify(dict(logits=logits, draft=None, temperature=temperature, uniform=uniform, tokens=np.zeros(S, np.int32),
+                                    parents=np.full(S, -1, np.int32), seg=seg))
+    assert (count == 1).all()
+    np.testing.assert_array_equal(ids, above)
+
+
 # ---------------------------------------------------------------------------------------------- rows and pages moved
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])

@@ -1,4 +1,5 @@
-// The verdict on a tree of drafted tokens against the target's logits, from given random numbers (float64 throughout).
+// The verdict on a tree of drafted tokens against the target's logits, from given random numbers: float64's, taken in float32 where that
+// cannot differ.
 //
 // A request's walk starts at its root, the token already chosen. At a node, p = softmax(logits / T) is the target's distribution
 // of the next token, q that of the drafter, from which the node's children were drawn one after the other without replacement
@@ -11,11 +12,14 @@
 // row pair each, ended by one exchange through distributed shared memory, after which all blocks know the sums and take the same
 // decisions. Only the rows of nodes that the walk visits are read. The kinds of pass:
 //   quick   maximum and sum of p's and q's row, exponentials in float32, once per visited node. Whether a child stands is decided from
-//           these sums unless u q(x) lies within MARGIN of p(x); the sums are off by 6e-6 at most (see `quick_chunk`);
+//           these sums unless u q(x) lies within MARGIN of p(x); the sums are off by 5e-6 (short rows) to 4e-4 at most (see `quick_chunk`);
 //   first   float64, where a child falls, or is too near to call, or the draw is due: the exact sums, and with them at once the sum of
 //           max(p - q, 0). That one takes p's and q's exact sums beforehand, which are not known yet: with the quick sums' ratio a0 for
-//           a, S(a) = sum max(a p - q, 0) is S(a0) + (a - a0) times the p for which a0 p > q, up to the tokens that change sides
-//           between a0 and a (a part of 1e-6 of those within 1e-6);
+//           a, S(a) = sum max(a p - q, 0) is S(a0) + (a - a0) times the p for which a0 p > q, but for tokens that change sides between a0
+//           and a. Those within 2^-19 of their border are therefore left out, and added with the exact a by a second exchange where there
+//           are any; where a0 turns out to be off by more than half of that, or a lane has met several, a `next` pass does it. (Taken
+//           for good, what changes sides is |a - a0| times its p, with nothing to compare it to: a token that has nearly all of p and q makes the
+//           sum wrong by a thousandth, and it scales all that follows.)
 //   next    float64, for every further sibling that falls: the sums of the new p and q.
 // Sums are kept per warp, whose tokens are one run each, so the last pass before the draw already says in whose run the drawn token
 // lies: its block's threads walk that run again, a few neighbouring tokens each. A draw's place among 100,000 running sums needs more
@@ -93,6 +97,7 @@ __device__ __forceinline__ double warp_sum_d(double v) {
 
 struct alignas(16) Slot {      // what a block tells the others after a pass
   double sum_p, sum_q, over, under;
+  int near;
 };
 struct alignas(8) Found {     // a node's rows, quick; or the argmax (p.top, arg)
   float top_p, sum_p, top_q, sum_q;
@@ -220,27 +225,42 @@ __device__ __forceinline__ Found find_warp(const float* __restrict__ lrow, const
 }
 
 // A warp's part of the first exact pass: of p's weights (without token `gone`'s where there is no drafter), q's without it, max(a0 p - q,
-// 0), and the p for which that is not 0.
-struct Part { double sum_p, sum_q, over, under; };
+// 0), and the p for which that is not 0, these two without the tokens whose a0 p is within 2^-NEAR of q: on which side of a p they lie is
+// for the exact a to say. A lane keeps one such token (`at`: the lane's own, -1 for none); near: how many lanes have one, MANY for each that
+// has met several.
+constexpr int NEAR = 19, MANY = 1 << 16;
+struct Part {
+  double sum_p, sum_q, over, under;
+  int near, at;
+};
 __device__ __noinline__ Part first_sums(const float* __restrict__ lrow, const float* __restrict__ drow, int lo, int hi, bool vec, int lane, const Ref& rp_,
                                         const Ref& rq_, const double* tab, double a0, int gone) {
   const Ref rp = rp_, rq = rq_;
   double sp = 0.0, sq = 0.0, so = 0.0, su = 0.0;
+  int near = 0, at = -1;
   for (int i0 = lo; i0 < hi; i0 += 32 * CHUNK) {
     float a[CHUNK], b[CHUNK];
     load_chunk(lrow, i0, hi, vec, lane, a);
     const int it = gone - i0 - 4 * lane;
     if (drow) {
       load_chunk(drow, i0, hi, vec, lane, b);
+      unsigned close = 0;
 #pragma unroll
       for (int j = 0; j < CHUNK; ++j) {      // (tokens from hi on weigh nothing)
         const double wp = weight<true>(a[j], rp, tab), wq = weight<true>(b[j], rq, tab), over = fma(a0, wp, -wq);
         sp += wp;
         if (it != step(j)) sq += wq;
-        if (__double2hiint(over) >= 0) {      // (the sign bit)
+        // (high words compare as the numbers do, and 2^-NEAR is a subtraction there; weights below 2^-1004 are never near)
+        const bool here = (__double2hiint(over) & 0x7fffffff) <= __double2hiint(wq) - (NEAR << 20);
+        if (here) close |= 1u << j;
+        if (!here && __double2hiint(over) >= 0) {      // (the sign bit)
           so += over;
           su += wp;
         }
+      }
+      if (close) {
+        at = i0 + 4 * lane + step(__ffs(close) - 1);
+        near = near || (close & (close - 1)) ? MANY : 1;
       }
     } else {
 #pragma unroll
@@ -250,7 +270,7 @@ __device__ __noinline__ Part first_sums(const float* __restrict__ lrow, const fl
       }
     }
   }
-  return {warp_sum_d(sp), warp_sum_d(sq), warp_sum_d(so), warp_sum_d(su)};
+  return {warp_sum_d(sp), warp_sum_d(sq), warp_sum_d(so), warp_sum_d(su), __reduce_add_sync(0xffffffffu, near), at};
 }
 
 // A child that has fallen: its token, 1 / the sum of p after it, 1 / the sum of q before it.
@@ -288,7 +308,7 @@ __device__ __noinline__ Part next_sums(const float* __restrict__ lrow, const flo
       sq += (qv[0] + qv[1]) + (qv[2] + qv[3]);
     }
   }
-  return {warp_sum_d(sp), warp_sum_d(sq), 0.0, 0.0};
+  return {warp_sum_d(sp), warp_sum_d(sq), 0.0, 0.0, 0, -1};
 }
 
 struct Shared {
@@ -395,7 +415,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     if (BLOCKS > 1) {
       cluster.sync();
       if (warp == 0) {
-        Slot r = {0.0, 0.0, 0.0, 0.0};
+        Slot r = {0.0, 0.0, 0.0, 0.0, 0};
         if (lane < BLOCKS) sh.block[lane] = r = *cluster.map_shared_rank(&sh.slot[turn], lane);
 #pragma unroll
         for (int o = BLOCKS >> 1; o > 0; o >>= 1) {
@@ -403,6 +423,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
           r.sum_q += __shfl_xor_sync(0xffffffffu, r.sum_q, o);
           r.over += __shfl_xor_sync(0xffffffffu, r.over, o);
           r.under += __shfl_xor_sync(0xffffffffu, r.under, o);
+          r.near += __shfl_xor_sync(0xffffffffu, r.near, o);
         }
         if (lane == 0) sh.sums = r;
       }
@@ -505,19 +526,20 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     auto add_up = [&](const Part& part) {
       if (lane == 0) sh.part[warp] = part;
       __syncthreads();
-      Slot mine = {0.0, 0.0, 0.0, 0.0};
+      Slot mine = {0.0, 0.0, 0.0, 0.0, 0};
       if (warp == 0) {
-        const Part z = lane < WARPS ? sh.part[lane] : Part{0.0, 0.0, 0.0, 0.0};
-        mine = {warp_sum_d(z.sum_p), warp_sum_d(z.sum_q), warp_sum_d(z.over), warp_sum_d(z.under)};
+        const Part z = lane < WARPS ? sh.part[lane] : Part{0.0, 0.0, 0.0, 0.0, 0, -1};
+        mine = {warp_sum_d(z.sum_p), warp_sum_d(z.sum_q), warp_sum_d(z.over), warp_sum_d(z.under), __reduce_add_sync(0xffffffffu, z.near)};
       }
       return exchange_sums(mine);
     };
     // The first pass in float64: exact sums, and if a child x has fallen (x = -1: none) the sums of p and q after it. Returns false where
-    // the sum of max(p - q, 0) came out too small to be had this way (p and q nearly the same).
+    // the sum of max(p - q, 0) is not to be had this way: too small (p and q nearly the same), more than one token of a lane near its border,
+    // or a0 further off than the border's width covers.
     auto first_pass = [&](int gone, float lg, float dg, bool fell) -> bool {
       const double a0 = with_q ? (double)near_p / (double)near_q : 0.0;
-      const Part mine = first_sums(lrow, with_q ? drow : nullptr, lo, hi, vec, lane, rp, rq, tab, a0, gone);
-      const Slot sum = add_up(mine);
+      Part mine = first_sums(lrow, with_q ? drow : nullptr, lo, hi, vec, lane, rp, rq, tab, a0, gone);
+      Slot sum = add_up(mine);
       const double wg = gone >= 0 ? weight(lg, rp, tab) : 0.0, dgw = gone >= 0 && with_q ? weight(dg, rq, tab) : 0.0;
       const double all_p = with_q ? sum.sum_p : sum.sum_p + wg, all_q = sum.sum_q + dgw;
       inv_p = 1.0 / all_p;
@@ -529,9 +551,21 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
       double left = 0.0;
       bool good = true;
       if (with_q) {
-        const double da = all_q / all_p - a0;
+        double da = all_q / all_p - a0;
+        good = fabs(da) <= a0 * (0.5 / (1 << NEAR)) && sum.near < MANY;
+        if (good && sum.near > 0) {      // the tokens near the border, now that it is known
+          double over = 0.0;
+          if (mine.at >= 0) {
+            const double wp = weight<true>(lrow[mine.at], rp, tab), wq = weight<true>(drow[mine.at], rq, tab);
+            over = fmax(fma(da, wp, fma(a0, wp, -wq)), 0.0);
+          }
+          mine.over = fma(da, mine.under, mine.over) + warp_sum_d(over);
+          mine.under = da = 0.0;
+          sum = add_up(mine);
+          own_over = mine.over, own_under = 0.0;
+        }
         left = (sum.over + da * sum.under) / all_q;
-        good = left > 1e-6;
+        good = good && left > 1e-6;
         if (good) shift = da, unit = 1.0 / (all_q * left), total = 1.0, plain = false, by_over = true;
       } else if (sum.sum_p > NOTHING) {
         left = sum.sum_p / all_p;
@@ -621,7 +655,7 @@ verify_kernel(const float* __restrict__ logits, const float* __restrict__ draft,
     if (lane == 0) sh.run[warp] = (by_over ? fmax(fma(shift, own_under, own_over), 0.0) : own_p) * unit;
     __syncthreads();
     if (warp == 0) {
-      const Slot b = lane < BLOCKS ? sh.block[lane] : Slot{0.0, 0.0, 0.0, 0.0};
+      const Slot b = lane < BLOCKS ? sh.block[lane] : Slot{0.0, 0.0, 0.0, 0.0, 0};
       double run = (by_over ? fmax(fma(shift, b.under, b.over), 0.0) : b.sum_p) * unit;
 #pragma unroll
       for (int o = 1; o < BLOCKS; o <<= 1) {

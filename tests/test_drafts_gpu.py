@@ -578,6 +578,89 @@ def test_verify_draws_at_a_rounding_from_the_border():
     np.testing.assert_array_equal(ids, above)
 
 
+def border_case(rows, seed, sibling, pad=0):
+    """rows: (logits, the drafter's logits, token) each: that token is a child and falls; then (`sibling`) a second child or else the draw has
+    its number close beside its border, alternately above and below, at the distance that 64 bits resolve: p and q are known to 2^-48 of
+    themselves at best (exponents up to 12, a sum), so max(p - q, 0) over its sum `left` to 2^-47 / left in either computation, its running
+    sums to vocab 2^-53 more; 2^-42 / left + vocab 2^-51 leaves room for both."""
+    rng = np.random.default_rng(seed)
+    vocab, n = len(rows[0][0]), 3 if sibling else 2
+    S = len(rows)
+    N = S * n + pad
+    logits, draft = np.zeros((N, vocab), np.float32), np.zeros((N, vocab), np.float32)
+    tokens, parents, uniform = np.zeros(N, np.int32), np.full(N, -1, np.int32), rng.random(N)
+    for s, (a, b, x) in enumerate(rows):
+        at = s * n
+        logits[at:at + n], draft[at:at + n], parents[at + 1:at + n] = a, b, 0
+        tokens[at + 1], uniform[at + 1] = x, 1.0 - 2.0 ** -53
+        p, q = plain.softmax64(a, 1.0), plain.softmax64(b, 1.0)
+        assert q[x] > 1.004 * p[x]
+        rest = np.maximum(p - q, 0.0)
+        left = rest.sum()
+        off = (2.0 ** -42 / left + vocab * 2.0 ** -51) * (1 if s % 2 else -1)
+        if sibling:
+            q[x] = 0.0
+            odds = np.where(q > 0, rest / left / np.maximum(q / q.sum(), 1e-300), 0.0)
+            could = np.flatnonzero((odds > 1e-3) & (odds < 0.999))
+            y = int(could[rng.integers(len(could))])
+            # (what one token's odds are known to: its own difference counts, not the whole)
+            own = 2.0 ** -42 * p[y] / rest[y]
+            tokens[at + 2], uniform[at + 2] = y, odds[y] * (1 + off + np.sign(off) * own)
+        else:
+            upto = np.cumsum(rest / left)
+            could = np.flatnonzero((rest / left > 8 * abs(off)) & (upto < 1 - 8 * abs(off)))
+            u = upto[could[rng.integers(len(could))]] + off if len(could) else 0.5
+            if np.abs(upto - u).min() >= 0.5 * abs(off):      # (no other border there)
+                uniform[at] = u
+    seg = np.stack([n * np.arange(S), np.full(S, n), np.zeros(S), np.zeros(S)], 1).astype(np.int32)
+    return dict(logits=logits, draft=draft, temperature=np.ones(S, np.float32), uniform=uniform, tokens=tokens, parents=parents, seg=seg)
+
+
+@pytest.mark.parametrize("ahead", [True, False])
+@pytest.mark.parametrize("small,sibling", [(0.3, False), (3.0, True), (3e-3, False), (3e-5, False), (6e-6, False)])
+def test_verify_a_token_as_likely_for_the_drafter(small, sibling, ahead):
+    """Rows with one token that has much of p and of q, or nearly all, within 1e-7 of the same: whether p exceeds q there is not for float32 sums
+    to say. The others, `small` times as likely in all, go round, so that p's and q's sums are the same but for a change of one of them."""
+    rng = np.random.default_rng(int(small * 1e7) + sibling)
+    rows = []
+    for _ in range(2000):
+        a = np.concatenate([[0.0], np.log(small * rng.dirichlet(np.ones(5)) + 1e-3 * small)]).astype(np.float32)
+        b = a.copy()
+        b[1:] = np.roll(a[1:], 1)
+        b[3] += np.float32(rng.uniform(-1e-7, 1e-7) / np.exp(float(b[3])))
+        p, q = plain.softmax64(a, 1.0), plain.softmax64(b, 1.0)
+        falls = [x for x in range(1, 6) if q[x] > 1.01 * p[x]]
+        if not falls:
+            continue
+        if sibling:      # (some token has less of what is left than the drafter has of it)
+            rest, q[falls[0]] = np.maximum(p - q, 0.0), 0.0
+            odds = rest / rest.sum() / np.maximum(q / q.sum(), 1e-300)
+            if not ((odds > 1e-3) & (odds < 0.999)).any():
+                continue
+        order = rng.permutation(6)
+        rows.append((a[order], b[order], int(np.flatnonzero(order == falls[0])[0])))
+    assert len(rows) > 400
+    assert_verify(border_case(rows, 23, sibling, pad=0 if ahead else 8 * len(rows)))
+
+
+@pytest.mark.parametrize("requests", [1, 8, 14, 30, 70, 80])
+@pytest.mark.parametrize("error", [0.3, 1e-2, 1e-3, 1e-4, 1e-5, 4e-6])
+def test_verify_drafters_near_the_target(error, requests):
+    """The drafter's logits are the target's but for `error`, and one unlikely token's that falls; numbers close beside the borders of what
+    is left, with as many blocks a request as a step of that many takes."""
+    rng = np.random.default_rng(requests)
+    vocab = 33001
+    for sibling in (True, False):
+        rows = []
+        for _ in range(requests):
+            a = (rng.standard_normal(vocab) * 2).astype(np.float32)
+            b = (a.astype(np.float64) + rng.standard_normal(vocab) * error).astype(np.float32)
+            x = int(a.argmin())
+            b[x] = a[x] + np.float32(0.1 + 2 * error)
+            rows.append((a, b, x))
+        assert_verify(border_case(rows, 24, sibling))
+
+
 # ---------------------------------------------------------------------------------------------- rows and pages moved
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])

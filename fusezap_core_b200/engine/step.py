@@ -36,6 +36,7 @@ import torch
 
 from ..cache import CacheManager
 from ..parts import LayerCache, PendingSum
+from ..parts.base import can_take_trees
 from .model import DecoderModel
 
 MAX_TREE_NODES = 1024      # of a drafted tree (what `Ops.verify_tree` takes)
@@ -341,7 +342,10 @@ class StepRunner:
         model = self.model
         if not 0 < max_tree_nodes <= MAX_TREE_NODES:
             raise ValueError(f"max_tree_nodes is {max_tree_nodes}: 1 to {MAX_TREE_NODES}")
-        wrong = sorted({type(layer.mixer).__name__ for layer in model.layers if not getattr(layer.mixer, "takes_trees", False)})
+        mixers = [layer.mixer for layer in model.layers]
+        encodings = [model.positions[m.position_name()] for m in mixers if m.position_name() is not None]
+        wrong = sorted({type(m).__name__ for m in mixers if not can_take_trees(m, "forward", "forward_pending")} |
+                       {type(e).__name__ for e in encodings if not can_take_trees(e, "rotate_and_store", "project_rotate_store")})
         if wrong:
             raise ValueError(f"drafted trees are not taken by {', '.join(wrong)}")
         if model.embed_extras or model.state_needs():

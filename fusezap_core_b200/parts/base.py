@@ -151,6 +151,17 @@ def can_leave_product(part: Any) -> Callable | None:
     return _LEAVES_PRODUCT.get(getattr(type(part), "forward", None))
 
 
+def can_take_trees(part: Any, *methods: str) -> bool:
+    """Whether the part's class says that these methods of it run steps of drafted trees (`takes_trees`). What a class says holds for the
+    methods that it has, not for those that a class derived from it brings."""
+    for c in type(part).__mro__:
+        if "takes_trees" in vars(c):
+            return c.takes_trees
+        if any(m in vars(c) for m in methods):
+            return False
+    return False
+
+
 @dataclass
 class PendingProduct:
     """A pending residual term that is still to be computed, rows . weight^T + bias, with nothing read or written in between: what a
@@ -212,7 +223,9 @@ class Part:
 
 
 class Mixer(Part):
-    takes_trees = False      # whether forward runs steps of drafted trees (meta.tree): rows that are not consecutive places
+    # Whether `forward` runs steps of drafted trees (meta.tree): rows that are not consecutive places. A derived class with a `forward` of
+    # its own says it anew.
+    takes_trees = False
 
     def cache_need(self) -> "KVNeed | LatentNeed | None":
         return None
@@ -240,6 +253,10 @@ class Norm(Part):
 
 
 class PositionEncoding(Part):
+    # Whether rows are stored at their places (meta.place, where it is not None) instead of at their positions, as `Ops.rope_kv_write`
+    # does it. A derived class that brings one of the methods below says it anew.
+    takes_trees = False
+
     def prepare(self, max_len: int, device: torch.device) -> None:
         raise NotImplementedError
 

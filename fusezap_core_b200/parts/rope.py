@@ -38,6 +38,8 @@ def inverse_frequencies(head_dim: int, theta: float, kind: str = "default", fact
 
 @register_position("rope")
 class RotaryEncoding(PositionEncoding):
+    takes_trees = True
+
     def __init__(self, head_dim: int, theta: float, kind: str = "default", factor: float = 1.0,
                  low_freq_factor: float = 1.0, high_freq_factor: float = 4.0,
                  original_max_position_embeddings: int = 0, precise: bool = False, turns_fast: float = 32.0,

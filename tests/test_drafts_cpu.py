@@ -186,6 +186,53 @@ def test_windows_and_other_mixers_refuse(models, tmp_path):
             StepRunner(other, cache, max_rows=8, max_tree_nodes=4)
 
 
+def test_parts_with_methods_of_their_own_refuse(models, monkeypatch):
+    """What a mixer or a position encoding says of trees holds for the methods it has, not for those that a derived class brings."""
+    from fusezap_core_b200.parts.attention import GQAttention
+    from fusezap_core_b200.parts.rope import RotaryEncoding
+    model, _, opts, _ = models["tiny_llama"]
+
+    class Derived(GQAttention):
+        def cache_need(self):
+            return super().cache_need()
+
+    class Own(GQAttention):
+        def forward(self, ctx, h, cache):
+            raise NotImplementedError
+
+    class Below(Own):
+        pass
+
+    class OwnForTrees(Own):
+        takes_trees = True
+
+    class Rope(RotaryEncoding):
+        pass
+
+    class Store(RotaryEncoding):
+        def rotate_and_store(self, ctx, qkv, q_out, cache, num_heads, num_kv_heads, head_dim):
+            raise NotImplementedError
+
+    class Product(RotaryEncoding):
+        def project_rotate_store(self, *a):
+            return False
+
+    class StoreForTrees(Store):
+        takes_trees = True
+
+    mixer = model.layers[-1].mixer
+    for part, kinds in ((mixer, ((Derived, True), (Own, False), (Below, False), (OwnForTrees, True))),
+                        (model.positions[mixer.position_name()], ((Rope, True), (Store, False), (Product, False), (StoreForTrees, True)))):
+        for kind, takes in kinds:
+            with monkeypatch.context() as m:
+                m.setattr(part, "__class__", kind)
+                if takes:
+                    runner_for(model, opts)
+                else:
+                    with pytest.raises(ValueError, match=f"not taken by {kind.__name__}"):
+                        runner_for(model, opts)
+
+
 class _Anything:
     """A kernel table that takes every size and runs nothing."""
     dtype = torch.float32

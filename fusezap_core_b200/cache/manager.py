@@ -134,6 +134,11 @@ class KVGroup:
         tail[:] = -1
         self.lens[req] = keep
 
+    def shares_from(self, req: Hashable, n_tokens: int) -> bool:
+        """Whether a page that holds place n_tokens or a later one has other holders."""
+        row = self.rows.get(req)
+        return row is not None and any(p >= 0 and self.allocator.holders(p) > 1 for p in row[n_tokens // self.page_size: self.lens[req]].tolist())
+
     def fork_pages(self, req: Hashable, computed: int) -> tuple[int, int]:
         """(pages of `req` that a fork shares, pages it gets of its own): those full of computed tokens, and the one that is not."""
         row, full = self.rows.get(req), computed // self.page_size
@@ -281,9 +286,13 @@ class CacheManager:
             self.states.acquire(req)
 
     def commit(self, req: Hashable, n_computed: int) -> None:
-        """Positions [0, n_computed) of `req` are in the cache: window groups give back what lies before the window."""
-        if req not in self.computed:
+        """Positions [0, n_computed) of `req` are in the cache: window groups give back what lies before the window. A request may be set
+        back, but not into pages that it shares with a fork."""
+        before = self.computed.get(req)
+        if before is None:
             raise KeyError(f"request {req!r} holds nothing")
+        if n_computed < before and any(g.shares_from(req, n_computed) for g in self.groups):
+            raise ValueError(f"request {req!r} cannot be set back from {before} to {n_computed} tokens: it shares pages behind them with a fork")
         self.computed[req] = n_computed
         for g in self.groups:
             g.release_before(req, n_computed)

@@ -325,6 +325,29 @@ def test_fork_over_windows_latents_and_random_orders(computed):
     assert all(g.allocator.num_free == 40 for g in m.groups)
 
 
+def test_a_request_is_not_set_back_into_pages_that_it_shares():
+    """What it would write anew there is what the other has computed."""
+    m = manager({0: KVNeed(2, 16, 0), 1: LatentNeed(24)})
+    m.ensure("a", 14)
+    m.commit("a", 14)
+    m.commit("a", 13)
+    m.commit("a", 14)
+    m.fork("a", "b")
+    for req in ("a", "b"):
+        m.commit(req, 13)      # (the page that is not full is each one's own)
+        m.commit(req, 12)
+        for n in (11, 8, 1, 0):
+            with pytest.raises(ValueError, match="shares"):
+                m.commit(req, n)
+            assert m.computed[req] == 12
+    m.check()
+    m.free("b")
+    m.commit("a", 5)
+    m.ensure("a", 9)
+    m.commit("a", 9)
+    m.check()
+
+
 def test_fork_refusals_and_state():
     m = manager(pages=3)
     m.ensure("a", 10)

@@ -481,9 +481,12 @@ class StepRunner:
 
     def commit_kept(self, portions: Sequence[Portion], starts: Sequence[int], counts: Sequence[int]) -> None:
         """The host's books after `keep`: each request has so many tokens more, and pages that only held other nodes go back."""
-        for p, s, n in zip(portions, starts, counts):
+        if len(counts) != len(portions) or len(starts) < len(portions):
+            raise ValueError(f"commit_kept: {len(portions)} requests, {len(starts)} starts, {len(counts)} counts of kept tokens")
+        for p, n in zip(portions, counts):
             if not 1 <= n <= len(p.tokens):
                 raise ValueError(f"request {p.req!r}: {n} of its {len(p.tokens)} tokens kept")
+        for p, s, n in zip(portions, starts, counts):
             self.cache.commit(p.req, s + int(n))
             self.cache.trim(p.req)
 

@@ -171,6 +171,23 @@ def test_refusals(models):
         run.keep(None, None)
 
 
+def test_kept_counts_that_do_not_fit_the_step_change_no_books(models):
+    model, _, opts, _ = models["tiny_llama"]
+    run, cache = runner_for(model, opts, nodes=6)
+    portions = [Portion("a", [1, 2, 3], range(3), parents=[-1, 0, 0]), Portion("b", [4, 5], range(2), parents=[-1, 0])]
+    starts = run.prepare(portions)
+    run.forward()
+    for counts in ([2], [2, 1, 1], [], [2, 0], [2, 3]):
+        with pytest.raises(ValueError, match="kept"):
+            run.commit_kept(portions, starts, counts)
+        assert cache.computed == {"a": 0, "b": 0}
+    with pytest.raises(ValueError, match="kept"):
+        run.commit_kept(portions, starts[:1], [2, 1])
+    run.commit_kept(portions, starts, [2, 1])
+    assert cache.computed == {"a": 2, "b": 1}
+    cache.check()
+
+
 def test_windows_and_other_mixers_refuse(models, tmp_path):
     model, cfg, opts, _ = models["tiny_window"]
     run, cache = runner_for(model, opts)

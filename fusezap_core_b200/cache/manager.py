@@ -139,11 +139,10 @@ class KVGroup:
         row = self.rows.get(req)
         return row is not None and any(p >= 0 and self.allocator.holders(p) > 1 for p in row[n_tokens // self.page_size: self.lens[req]].tolist())
 
-    def fork_pages(self, req: Hashable, computed: int) -> tuple[int, int]:
-        """(pages of `req` that a fork shares, pages it gets of its own): those full of computed tokens, and the one that is not."""
+    def fork_pages(self, req: Hashable, computed: int) -> int:
+        """Pages that a fork of `req` gets of its own: one, where a page is not full of computed tokens, else none."""
         row, full = self.rows.get(req), computed // self.page_size
-        held = 0 if row is None else int((row[: min(full, self.lens[req])] >= 0).sum())
-        return held, 1 if row is not None and computed % self.page_size and self.lens[req] > full and row[full] >= 0 else 0
+        return 1 if row is not None and computed % self.page_size and self.lens[req] > full and row[full] >= 0 else 0
 
     def fork(self, req: Hashable, new: Hashable, computed: int) -> list[tuple[int, int]]:
         """Gives `new` a block table over the first `computed` places of `req`: the full pages are shared, the last, which both go on
@@ -155,7 +154,7 @@ class KVGroup:
         n = min(full, self.lens[req])
         row[:n] = old[:n]
         copies = []
-        if self.fork_pages(req, computed)[1]:
+        if self.fork_pages(req, computed):
             row[full] = self.allocator.allocate(1)[0]
             copies = [(int(old[full]), int(row[full]))]
             n = full + 1
@@ -309,7 +308,7 @@ class CacheManager:
         if self.has_state and req in self.states.owner and not self.states.num_free:
             return False
         c = self.computed[req]
-        return all(g.fork_pages(req, c)[1] <= g.allocator.num_free for g in self.groups)
+        return all(g.fork_pages(req, c) <= g.allocator.num_free for g in self.groups)
 
     def fork(self, req: Hashable, new: Hashable) -> tuple[list[list[tuple[int, int]]], tuple[int, int] | None]:
         """A second request `new` over what `req` has computed: the pages that are full are shared between the two, the last one and

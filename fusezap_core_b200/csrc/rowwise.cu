@@ -728,14 +728,6 @@ FZ_API int fz_rope_kv_write_at(const float* qkv, const float* cos_t, const float
   return FZ_OK;
 }
 
-FZ_API int fz_rope_kv_write(const float* qkv, const float* cos_t, const float* sin_t, const int* pos,
-                            const int* seq_row, const int* table, int mb, void* k_pool, void* v_pool,
-                            long long page_stride, int page_size, int write, void* q_out, int dtype, int N, int Hq,
-                            int Hkv, int hd, int max_len, int* err, cudaStream_t stream) {
-  return fz_rope_kv_write_at(qkv, cos_t, sin_t, pos, nullptr, seq_row, table, mb, k_pool, v_pool, page_stride, page_size, write, q_out, dtype,
-                             N, Hq, Hkv, hd, max_len, err, stream);
-}
-
 // ------------------------------------------------------------------------------------------------ SwiGLU
 // kind 1: silu(g); 2: the tanh form of gelu, 0.5 g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))).
 __device__ __forceinline__ float gate_act(float g, int kind) {

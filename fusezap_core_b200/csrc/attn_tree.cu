@@ -10,8 +10,9 @@
 //
 // `attn_tree_context_kernel` here is the general kernel of the first kind, plain float32 FMA from tiles in shared memory: the
 // float32 path, and head and page sizes that the tensor-core kernel (attn_tree_tc.cu) refuses.
-// Keys are cut at places that depend on the request's own length only, and a tile's rows do not mix: a row's result does not
-// depend on the other requests of the step.
+// Keys are cut at places that depend on the request's own length only, and a tile's rows do not mix: what this kernel leaves of a row
+// does not depend on the other requests of the step, and in float32 the row's result does not either. (In bfloat16 the kernel that joins adds a
+// row's terms up in another order where a step has many rows, see `launch_merge`.)
 #include "attn_tree.cuh"
 
 namespace {

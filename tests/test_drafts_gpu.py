@@ -283,6 +283,25 @@ def test_tree_attention_float32_rows_do_not_depend_on_the_step():
         at += n
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("window", [0, 2000])
+def test_tree_attention_float32_rows_are_the_same_in_either_tile(hd, window):
+    """A step of 44 rows by 7 heads and 32 pieces, whose tiles have 64 rows (more than 16 a request, and 512 blocks), against its requests one
+    by one, whose tiles have 16 (256 blocks at most)."""
+    reqs = [(300, bushy(9)), (2900, chain(4)), (1700, bushy(30, 2)), (0, [-1])]
+    c = tree_case("float32", 14, 2, hd, 16, reqs, window=window, seed=4)
+    whole, at, m = run_tree(c), 0, c.meta
+    assert_tree(c, whole)
+    for s, (b, parents) in enumerate(reqs):
+        n, seg = len(parents), m.seg[s:s + 1].clone()
+        seg[0, 0] = 0
+        alone = SimpleNamespace(**{**vars(c), "q": c.q[at:at + n], "meta": SimpleNamespace(
+            pos=m.pos[at:at + n], seq_row=torch.zeros(n, dtype=torch.int32), seg=seg, ancestors=m.ancestors[at:at + n], tables=m.tables[s:s + 1],
+            max_context=m.max_context)})
+        assert torch.equal(run_tree(alone), whole[at:at + n])
+        at += n
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_tree_attention_replayed_with_other_lengths(dtype):
     """One recorded call, replayed after the metadata, the queries and the cache have changed under it."""

@@ -63,7 +63,7 @@ constexpr double NOTHING = 1e-290;      // weights and probabilities up to this 
 // row that holds a NaN or +inf is not asked for. Here and where p and q are made from weights the roundings are written out: every place that
 // needs a token's p gets the same bits.
 // LIFT: tokens too far below for a weight get 2^-1015 or so instead of 0, in fewer instructions (the first pass over 64 x 6 rows of 151,936
-// tokens: 130 us with exact zeros, 123 like this): for sums that are divided by no less than 1e-6 after it, where that is NOTHING.
+// tokens, the whole call: 130 us with exact zeros, 129 like this): for sums that are divided by no less than 1e-6 after it, where that is NOTHING.
 constexpr int TABLE = 128, COPIES = 16;
 template <bool LIFT = false>
 __device__ __forceinline__ double weight(float x, const Ref& r, const double* tab) {
@@ -791,8 +791,8 @@ int launch(const float* logits, const float* draft, const float* temperature, co
 }  // namespace
 
 // Blocks per request: as many as the chip holds at once beside the other requests' (8 clusters of sixteen, 14 of eight, 32 of four, 74 of
-// two), each with 2,048 tokens and more. us at 128,256 tokens with 2, 4, 8 and 16 blocks: one request with 5 nodes 36, 23, 18, 16; 8 with 16
-// 163, 94, 64, 50; 64 with 6 at 151,936 tokens 137, 140, 195, 408.
+// two), each with 2,048 tokens and more. us at 128,256 tokens with 2, 4, 8 and 16 blocks: one request with 5 nodes 28, 21, 18, 17; 8 with 16
+// 131, 76, 54, 44; 64 with 6 at 151,936 tokens 129, 145, 182, 265.
 FZ_API int fz_verify_blocks(int S, int V) {
   int b = S <= 8 ? 16 : S <= 14 ? 8 : S <= 32 ? 4 : S <= 74 ? 2 : 1;
   while (b > 1 && V < 2048 * b) b >>= 1;
@@ -801,8 +801,8 @@ FZ_API int fz_verify_blocks(int S, int V) {
 
 // Slices of a row whose quick statistics a kernel of its own takes ahead of the walks (0: none; the scratch: N * slices * 24 bytes).
 // It reads rows that no walk visits, but all SMs share it evenly, while walks differ in length: it pays where trees are small, two to six
-// nodes on average (us without and with it, a drafter's logits throughout: 64 chains of up to 6 nodes over 151,936 tokens 141 and 123, 16 of
-// 8 over 128,256 82 and 57; 30 trees of 10 71 and 101, 8 of 16 45 and 61; single nodes, 64 of them 31 and 37).
+// nodes on average (us without and with it, a drafter's logits throughout: 64 chains of up to 6 nodes over 151,936 tokens 141 and 129, 16 of
+// 8 over 128,256 83 and 59; 30 trees of 10 73 and 107, 8 of 16 43 and 64; single nodes, 64 of them 32 and 37).
 FZ_API int fz_verify_ahead(int S, int N, int V) {
   if (N < 2 * S || N > 6 * S) return 0;
   int slices = (8 * 148 + N - 1) / N;

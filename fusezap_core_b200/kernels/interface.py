@@ -482,7 +482,8 @@ class Ops:
         the node's children x in rising order: x stands if uniform * q(x) < p(x), and the walk goes on from it; else p = max(p - q, 0)
         over its sum (if that is not 0) and q loses x, scaled to sum 1. No child stands: next_ids[s] is the token at which the
         running sum of p, in index order, first exceeds uniform[root] * total. T <= 0 or a NaN: the first child that is the argmax
-        (the order of `argmax`) stands, else the argmax is the next token. float64. A row without a distribution (a NaN, +inf, or
+        (the order of `argmax`) stands, else the argmax is the next token. float64: p and q are known to some 2^-48 of themselves, what is
+        left of p behind rejections to 2^-47 over its sum. A row without a distribution (a NaN, +inf, or
         nothing above -inf): no child stands and the draw gives V - 1 (a drafter's row: no child stands and p is
         drawn from). At most 8,388,608 tokens.
         Results, int32: count[s] kept nodes (the root among them; 0 for no rows and for no verdict, next_ids[s] = -1); path[first row + k] = node of the
@@ -493,10 +494,12 @@ class Ops:
         """pool: a cache group's (slots, pages, .., page_size, width), any element type of 2 bytes and more; table (S, MB) int32 its
         block tables. For every request s and k < count[s]: the row at place seg[s, 2] + path[seg[s, 0] + k] goes to place seg[s, 2] +
         k, in all slots, keys and values, as if all were read before one is written. path (N,), count (S,) int32 as `verify_tree`
-        leaves them: rising nodes; a path that is none (or a place without a page) is an error and leaves the request's rows."""
+        leaves them: rising nodes; a path that is none (or a place without a page) is an error and leaves the request's rows. At most 65,535
+        requests, and 1,024 kept rows of each."""
         raise NotImplementedError
 
     def copy_pages(self, pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Page src[i] of a cache group's pool goes to page dst[i], in all slots; src, dst int32 (M,). A page may be a source
-        several times, but a destination only once and not both. A page outside the pool is an error and is left out."""
+        several times, but a destination only once and not both. A page outside the pool is an error and is left out. At most 65,535 pages,
+        and as many slots."""
         raise NotImplementedError

@@ -483,7 +483,7 @@ class Ops:
         over its sum (if that is not 0) and q loses x, scaled to sum 1. No child stands: next_ids[s] is the token at which the
         running sum of p, in index order, first exceeds uniform[root] * total. T <= 0 or a NaN: the first child that is the argmax
         (the order of `argmax`) stands, else the argmax is the next token. float64: p and q are known to some 2^-48 of themselves, what is
-        left of p behind rejections to 2^-47 over its sum. A row without a distribution (a NaN, +inf, or
+        left of p behind rejections to 2^-47 over its sum; weights and probabilities of 1e-290 and less are 0. A row without a distribution (a NaN, +inf, or
         nothing above -inf): no child stands and the draw gives V - 1 (a drafter's row: no child stands and p is
         drawn from). At most 8,388,608 tokens.
         Results, int32: count[s] kept nodes (the root among them; 0 for no rows and for no verdict, next_ids[s] = -1); path[first row + k] = node of the
